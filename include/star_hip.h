@@ -217,6 +217,71 @@ int star_attn_fwd(const void* qkv, void* out, float* lse, int NB, int L, int H, 
 int star_attn_bwd(const void* qkv, const void* out, const void* dout, const float* lse, float* delta,
                   void* dqkv, int NB, int L, int H, int hd, int dt, void* stream);
 
+/* ---- rotary positions, sliding-window attention with sinks, rolling key/value cache --------------------------------------
+ * No counterpart in the reference: for sequences that run over many frames, which the dense attention above cannot hold.  Rows are
+ * packed as above but with KV <= H key/value heads (H % KV == 0; query head h reads key head h / (H / KV)): a row is
+ * [H query heads | KV key heads | KV value heads] x hd, rows `ld` elements apart (16-byte aligned).  dt: STAR_BF16 or STAR_F32;
+ * statistics and sums are float32.
+ *
+ * star_rope: y = x with the first rot_heads heads of every row turned: pair i of a head by theta = 2 pi pos[axis[i]] rev[i] --
+ *   y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin -- or by -theta (inverse != 0: the backward pass).  The pair is elements (i, i + pairs),
+ *   or (2 i, 2 i + 1) when interleaved; elements from 2 * pairs on do not turn.  pos int32 [axes] rows of R, pos_ld elements apart.
+ *   y == x: in place, only the turning elements are touched; else every one of the W columns is written.  W % 8 == 0, hd % 16 == 0,
+ *   pairs % 8 == 0.  Angles are formed in float64. */
+typedef struct StarRope {
+    double rev[64];       /* revolutions per unit of position */
+    uint8_t axis[64];     /* which row of pos */
+    int32_t pairs, axes, interleaved, reserved;
+} StarRope;
+int star_rope(const void* x, int64_t x_ld, void* y, int64_t y_ld, const int32_t* pos, int64_t pos_ld, const StarRope* h_rope, int R, int W,
+              int rot_heads, int hd, int inverse, int dt, void* stream);
+/* star_attn_window_fwd: key j is visible to query i iff j <= i + right and (j >= i - left or j < sinks), both inside the sequence.
+ * Sequence b is rows [b L, (b + 1) L) or, with offsets int64 [NB + 1] on the device, rows [offsets[b], offsets[b+1]), of which the first
+ * L are used (L = the longest sequence); rows of no sequence are neither read nor written.  hd in {16, 32, 64, 128}.
+ *   out dt [R, H*hd]; lse float32 [H, R]: log2-domain log-sum-exp of every row (optional in the forward pass).
+ * star_attn_window_bwd: reads out, lse, dout dt [R, H*hd]; writes dqkv dt [R, (H + 2 KV) hd] (dense rows; gradients of a shared key/value head
+ *   are summed over its query heads) and the workspace delta float32 [H, R].  No atomics: bitwise reproducible. */
+typedef struct StarAttnWindow {
+    const void* qkv;
+    const int64_t* offsets;   /* optional */
+    void* out;
+    float* lse;
+    const void* dout;         /* backward only, as dqkv and delta */
+    void* dqkv;
+    float* delta;
+    int64_t ld, R;            /* R: rows of qkv (NB * L without offsets) */
+    int32_t NB, L, H, KV, hd, left, right, sinks;
+    float scale;
+    int32_t dt;
+} StarAttnWindow;
+int star_attn_window_fwd(const StarAttnWindow* g, void* stream);
+int star_attn_window_bwd(const StarAttnWindow* g, void* stream);
+/* Rolling cache dt [2 (keys, values), NB, KV, cap, hd]: the token at position p lies in slot p for p < sinks, else in slot
+ * sinks + (p - sinks) % (cap - sinks).  lengths int32 [NB]: the sequence's tokens INCLUDING the new ones.
+ * star_kv_append: the key/value heads of the rows of sequence b (L of them, or offsets[b] .. offsets[b+1]) become its newest tokens; of
+ *   more new tokens than the ring holds the newest stay. */
+int star_kv_append(const void* qkv, int64_t ld, const int64_t* offsets, void* cache, const int32_t* lengths, int64_t R, int NB, int L, int H, int KV,
+                   int hd, int cap, int sinks, int dt, void* stream);
+/* star_attn_window_step: one new token per sequence.  Row b of qkv is the token at position lengths[b] - 1: its query and key heads are turned
+ *   (h_rope, a HOST pointer, with pos int32 [axes, NB]; NULL: as they are), key and value go into the cache, and out dt [NB, H*hd] is the
+ *   attention over the tokens it sees (left and sinks as above; left + sinks < cap).  lengths[b] <= 0: an idle entry, its out row is zeros and
+ *   nothing of its cache is touched.  ws float32 [star_attn_window_step_ws(...)]. */
+typedef struct StarAttnStep {
+    const void* qkv;
+    void* cache;
+    const int32_t* lengths;
+    const int32_t* pos;
+    const StarRope* h_rope;
+    void* out;
+    float* ws;
+    int64_t ld, pos_ld;
+    int32_t NB, H, KV, hd, cap, left, sinks;
+    float scale;
+    int32_t dt;
+} StarAttnStep;
+int64_t star_attn_window_step_ws(int NB, int H, int KV, int hd, int cap, int left, int sinks);
+int star_attn_window_step(const StarAttnStep* g, void* stream);
+
 /* ---- K1: voxel -> patch gather ------------------------------------------------------------------------
  * Replaces the im2col half of Conv2d(13, D, k=p, s=p) + flatten(2).transpose(1,2) (timm PatchEmbed;
  * mae_base.py:269, multiagent_mae.py:960-962).  Frame f = ba*T + t is imgs1[ba] for t = 0 and

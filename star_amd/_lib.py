@@ -37,6 +37,23 @@ class StarWgradJob(C.Structure):
                 ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("tap", C.c_int32)]
 
 
+class StarRope(C.Structure):
+    _fields_ = [("rev", C.c_double * 64), ("axis", C.c_uint8 * 64), ("pairs", C.c_int32), ("axes", C.c_int32), ("interleaved", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class StarAttnWindow(C.Structure):
+    _fields_ = [("qkv", C.c_void_p), ("offsets", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("dout", C.c_void_p), ("dqkv", C.c_void_p),
+                ("delta", C.c_void_p), ("ld", C.c_int64), ("R", C.c_int64), ("NB", C.c_int32), ("L", C.c_int32), ("H", C.c_int32), ("KV", C.c_int32),
+                ("hd", C.c_int32), ("left", C.c_int32), ("right", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float), ("dt", C.c_int32)]
+
+
+class StarAttnStep(C.Structure):
+    _fields_ = [("qkv", C.c_void_p), ("cache", C.c_void_p), ("lengths", C.c_void_p), ("pos", C.c_void_p), ("h_rope", C.POINTER(StarRope)),
+                ("out", C.c_void_p), ("ws", C.c_void_p), ("ld", C.c_int64), ("pos_ld", C.c_int64), ("NB", C.c_int32), ("H", C.c_int32), ("KV", C.c_int32),
+                ("hd", C.c_int32), ("cap", C.c_int32), ("left", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float), ("dt", C.c_int32)]
+
+
 WGRAD_GROUP_MAX = 8
 _P, _I, _L, _F = C.c_void_p, C.c_int, C.c_int64, C.c_float
 _SIGS = {
@@ -59,6 +76,12 @@ _SIGS = {
     "star_gemm_wgrad_group": (C.c_int, [C.POINTER(StarWgradJob), _I, _P, _L, _I, _P]),
     "star_attn_fwd": (C.c_int, [_P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "star_attn_bwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "star_rope": (C.c_int, [_P, _L, _P, _L, _P, _L, C.POINTER(StarRope), _I, _I, _I, _I, _I, _I, _P]),
+    "star_attn_window_fwd": (C.c_int, [C.POINTER(StarAttnWindow), _P]),
+    "star_attn_window_bwd": (C.c_int, [C.POINTER(StarAttnWindow), _P]),
+    "star_kv_append": (C.c_int, [_P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "star_attn_window_step_ws": (C.c_int64, [_I, _I, _I, _I, _I, _I, _I]),
+    "star_attn_window_step": (C.c_int, [C.POINTER(StarAttnStep), _P]),
     "star_gemm_res_ln_supported": (C.c_int, [_I, _I, _I]),
     "star_gemm_res_ln_prefers": (C.c_int, [_I, _I, _I, _I]),
     "star_gemm_res_ln": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, C.c_float, _P, _P, _P, _I, _I, _I, _I, _P]),

@@ -1,6 +1,8 @@
 """Tensor-level wrappers over the C ABI (one per kernel group).  PyTorch only allocates and hands over
 device pointers here; all arithmetic happens in libstar_hip.so."""
+import contextlib
 import ctypes as C
+import functools
 import math
 
 import numpy as np
@@ -368,6 +370,196 @@ def attn_bwd(qkv, out, dout, lse, nb, l, h, hd):
     with _timed("attn_bwd", 10.0 * nb * h * l * l * hd):
         L.check(L.lib().star_attn_bwd(p(qkv), p(out), p(dout), p(lse), p(delta), p(dqkv), nb, l, h, hd, dt, L.stream()))
     return dqkv
+
+
+# ---- rotary positions, sliding-window attention with sinks, rolling key/value cache ------------------------------------
+def _on(first, *rest):
+    """The device that a call runs on: the operands' own, which need not be the current one.  -> a context to launch in."""
+    _cuda(first, *rest)
+    dev = first.device
+    if any(t is not None and t.device != dev for t in rest):
+        raise RuntimeError("star_amd ops need all tensors on one device (got %s)" % ", ".join(sorted({str(t.device) for t in (first,) + rest if t is not None})))
+    return torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _rows2d(t, name):
+    """A matrix whose rows are dense and may lie apart: what the kernels take of packed qkv rows."""
+    assert t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1), "%s must be a matrix with dense rows" % name
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+@functools.lru_cache(maxsize=256)
+def rope_plan(sections, base=10000.0, per_axis=False, interleaved=False):
+    """The frequencies of a rotation as star_rope takes them.  sections: how many pairs of a head turn by each position axis, in order;
+    pair i of all n turns by pos[its axis] * base**(-i / n), or with per_axis by base**(-k / m) for the k-th of its axis' m pairs."""
+    n = sum(sections)
+    if any(s < 0 for s in sections) or not 0 < n <= 64 or n % 8 or len(sections) > 8:
+        raise ValueError("sections of at most 8 axes must add up to a multiple of 8 pairs, at most 64 (got %r)" % (sections,))
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError("base must be positive (got %r)" % (base,))
+    f = L.StarRope(pairs=n, axes=len(sections), interleaved=int(interleaved))
+    i = 0
+    for axis, m in enumerate(sections):
+        for k in range(m):
+            f.rev[i] = float(base) ** (-(k / m if per_axis else i / n)) / (2.0 * math.pi)
+            f.axis[i] = axis
+            i += 1
+    return f
+
+
+def _positions(pos, plan, r):
+    if pos.dim() == 1:
+        pos = pos.unsqueeze(0)
+    assert pos.dtype == torch.int32 and pos.dim() == 2 and pos.shape == (plan.axes, r), "positions must be int32 [%d, %d]" % (plan.axes, r)
+    assert pos.stride(1) == 1 or r <= 1, "positions of one axis must be dense"
+    return pos, (pos.stride(0) if plan.axes > 1 else max(pos.stride(0), r))
+
+
+def _rope(x, pos, rot_heads, hd, sections, base, per_axis, interleaved, out, inverse):
+    with _on(x, pos, out):
+        ld = _rows2d(x, "x")
+        r, w = x.shape
+        plan = rope_plan(tuple(sections), float(base), bool(per_axis), bool(interleaved))
+        pos, pos_ld = _positions(pos, plan, r)
+        if out is None:
+            out = torch.empty(r, w, dtype=x.dtype, device=x.device)
+        assert out.shape == x.shape and out.dtype == x.dtype
+        out_ld = _rows2d(out, "out")
+        if r:
+            with _timed("rope", 0.0, 2.0 * r * w * x.element_size()):
+                L.check(L.lib().star_rope(p(x), ld, p(out), out_ld, p(pos), pos_ld, C.byref(plan), r, w, rot_heads, hd, inverse, L.dt_of(x), L.stream()))
+    return out
+
+
+def rope_fwd(x, pos, rot_heads, hd, sections, base=10000.0, per_axis=False, interleaved=False, out=None):
+    """Rotary positions with several axes.  x [R, W] (bf16 / float32, dense rows that may lie apart): the first rot_heads heads of hd elements
+    of every row turn (packed qkv rows: the query and key heads, H + KV of them), the other columns are copied.  pos int32 [axes, R]: the
+    tokens' coordinates, one row per entry of `sections` (see rope_plan).  interleaved: pairs are neighbours (2 i, 2 i + 1) instead of
+    (i, i + n).  out=x turns in place.  -> [R, W]"""
+    return _rope(x, pos, rot_heads, hd, sections, base, per_axis, interleaved, out, 0)
+
+
+def rope_bwd(dy, pos, rot_heads, hd, sections, base=10000.0, per_axis=False, interleaved=False, out=None):
+    """Gradient of rope_fwd: the inverse rotation of dy (in place with out=dy)."""
+    return _rope(dy, pos, rot_heads, hd, sections, base, per_axis, interleaved, out, 1)
+
+
+def _window(qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale):
+    ld = _rows2d(qkv, "qkv")
+    kv = h if kv_heads is None else kv_heads
+    r, w = qkv.shape
+    assert w == (h + 2 * kv) * hd, "qkv rows of %d columns are not %d + 2 * %d heads of %d" % (w, h, kv, hd)
+    if offsets is not None:
+        assert offsets.dtype == torch.int64 and offsets.is_contiguous() and offsets.shape == (nb + 1,), "offsets must be int64 [nb + 1]"
+    else:
+        assert r == nb * l, "%d rows for %d sequences of %d" % (r, nb, l)
+    return L.StarAttnWindow(qkv=p(qkv), offsets=p(offsets), ld=ld, R=r, NB=nb, L=l, H=h, KV=kv, hd=hd, left=l if left is None else left,
+                            right=l if right is None else right, sinks=sinks, scale=hd ** -0.5 if scale is None else scale, dt=L.dt_of(qkv))
+
+
+def _fresh(r, w, like, offsets):
+    """an output of r rows: with offsets, rows of no sequence are left as they were -- zeros in a new tensor"""
+    return (torch.empty if offsets is None else torch.zeros)(r, w, dtype=like.dtype, device=like.device)
+
+
+def attn_window_fwd(qkv, nb, l, h, hd, kv_heads=None, left=None, right=0, sinks=0, offsets=None, scale=None, want_lse=True, out=None):
+    """Sliding-window attention with sinks.  qkv [R, (h + 2 kv_heads) hd]: packed rows (bf16 / float32, dense rows that may lie apart), query head i
+    reads key/value head i // (h // kv_heads).  Key j is visible to query i iff j <= i + right and (j >= i - left or j < sinks); None: no
+    bound (right=0: causal; left=right=None: everything).  nb sequences of l rows, or ragged: offsets int64 [nb + 1] on the device, l >= the
+    longest sequence (of a longer one only the first l rows take part).  Rows outside every sequence are neither read nor written.
+    -> (out [R, h*hd], lse float32 [h, R] or None)"""
+    with _on(qkv, offsets, out):
+        g = _window(qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale)
+        r = qkv.shape[0]
+        if out is None:
+            out = _fresh(r, h * hd, qkv, offsets)
+        assert out.shape == (r, h * hd) and out.dtype == qkv.dtype and out.is_contiguous()
+        lse = torch.empty(h, r, dtype=torch.float32, device=qkv.device) if want_lse else None
+        if r:
+            g.out, g.lse = p(out), p(lse)
+            with _timed("attn_window_fwd", 0.0, float(r) * (qkv.shape[1] + h * hd) * qkv.element_size()):
+                L.check(L.lib().star_attn_window_fwd(C.byref(g), L.stream()))
+    return out, lse
+
+
+def attn_window_bwd(qkv, out, dout, lse, nb, l, h, hd, kv_heads=None, left=None, right=0, sinks=0, offsets=None, scale=None, dqkv=None):
+    """Gradient of attn_window_fwd (the same arguments): dout [R, h*hd] -> dqkv [R, (h + 2 kv_heads) hd].  Two launches, each recomputing the scores
+    from the stored row log-sum-exp; no atomics, bitwise reproducible."""
+    with _on(qkv, out, dout, lse, offsets, dqkv):
+        g = _window(qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale)
+        r, w = qkv.shape
+        for t in (out, dout):
+            assert t.shape == (r, h * hd) and t.dtype == qkv.dtype and t.is_contiguous()
+        assert lse.shape == (h, r) and lse.dtype == torch.float32 and lse.is_contiguous()
+        if dqkv is None:
+            dqkv = _fresh(r, w, qkv, offsets)
+        assert dqkv.shape == (r, w) and dqkv.dtype == qkv.dtype and dqkv.is_contiguous()
+        if r:
+            delta = torch.empty(h, r, dtype=torch.float32, device=qkv.device)
+            g.out, g.lse, g.dout, g.dqkv, g.delta = p(out), p(lse), p(dout), p(dqkv), p(delta)
+            with _timed("attn_window_bwd", 0.0, float(r) * 2 * (w + h * hd) * qkv.element_size()):
+                L.check(L.lib().star_attn_window_bwd(C.byref(g), L.stream()))
+    return dqkv
+
+
+def _cache_dims(cache, qkv, nb, hd_heads, h, lengths):
+    assert cache.dim() == 5 and cache.shape[0] == 2 and cache.shape[1] == nb and cache.is_contiguous(), "cache must be a dense [2, nb, kv_heads, capacity, hd]"
+    kv, cap, hd = cache.shape[2:]
+    assert cache.dtype == qkv.dtype and hd_heads == (h + 2 * kv) * hd, "qkv rows of %d columns are not %d + 2 * %d heads of %d" % (hd_heads, h, kv, hd)
+    assert lengths.dtype == torch.int32 and lengths.is_contiguous() and lengths.shape == (nb,), "lengths must be int32 [nb]"
+    return kv, cap, hd
+
+
+def kv_append(qkv, cache, lengths, l, h, sinks=0, offsets=None):
+    """Put the key and value heads of packed rows into a rolling cache, in place.  cache [2, nb, kv_heads, capacity, hd]: the token at position p
+    lies in slot p for p < sinks, else in slot sinks + (p - sinks) % (capacity - sinks): the sinks stay, the ring behind them holds the newest
+    tokens (capacity >= the longest sequence: an ordinary cache).  lengths int32 [nb]: a sequence's tokens with the new ones, which are
+    its last: l rows of each (qkv [nb*l, ...]) or rows offsets[b] .. offsets[b+1], at most l.  -> cache"""
+    nb = cache.shape[1]
+    with _on(qkv, cache, lengths, offsets):
+        ld = _rows2d(qkv, "qkv")
+        r = qkv.shape[0]
+        kv, cap, hd = _cache_dims(cache, qkv, nb, qkv.shape[1], h, lengths)
+        if offsets is not None:
+            assert offsets.dtype == torch.int64 and offsets.is_contiguous() and offsets.shape == (nb + 1,), "offsets must be int64 [nb + 1]"
+        else:
+            assert r == nb * l, "%d rows for %d sequences of %d" % (r, nb, l)
+        if r and nb:
+            with _timed("kv_append", 0.0, float(r) * 4 * kv * hd * qkv.element_size()):
+                L.check(L.lib().star_kv_append(p(qkv), ld, p(offsets), p(cache), p(lengths), r, nb, l, h, kv, hd, cap, sinks, L.dt_of(qkv), L.stream()))
+    return cache
+
+
+def attn_window_step(qkv, cache, lengths, h, left=None, sinks=0, pos=None, sections=None, base=10000.0, per_axis=False, interleaved=False,
+                     scale=None, out=None):
+    """One new token per sequence over its rolling cache (see kv_append): rotate, store and attend.  qkv [nb, (h + 2 kv_heads) hd]: the rows
+    as the qkv Linear lays them out, of the tokens at positions lengths - 1.  With `sections`, query and key heads are turned by pos int32
+    [axes, nb] first (rope_fwd's arguments).  The key (turned) and the value go into the cache, then the token attends to itself, to the
+    `left` tokens before it and to the first `sinks`; None: to all that the ring holds.  left + sinks < capacity.  lengths[b] = 0: an idle
+    entry, its row of the result is zeros and its cache stays as it is.  -> out [nb, h*hd]"""
+    nb = cache.shape[1]
+    with _on(qkv, cache, lengths, pos, out):
+        ld = _rows2d(qkv, "qkv")
+        assert qkv.shape[0] == nb, "%d rows for %d cache entries" % (qkv.shape[0], nb)
+        kv, cap, hd = _cache_dims(cache, qkv, nb, qkv.shape[1], h, lengths)
+        plan, pos_ld = None, 0
+        if sections is not None:
+            plan = rope_plan(tuple(sections), float(base), bool(per_axis), bool(interleaved))
+            pos, pos_ld = _positions(pos, plan, nb)
+        if left is None:
+            left = cap - sinks - 1
+        if out is None:
+            out = torch.empty(nb, h * hd, dtype=qkv.dtype, device=qkv.device)
+        assert out.shape == (nb, h * hd) and out.dtype == qkv.dtype and out.is_contiguous()
+        if nb:
+            need = L.lib().star_attn_window_step_ws(nb, h, kv, hd, cap, left, sinks)
+            ws = torch.empty(need, dtype=torch.float32, device=qkv.device) if need else None
+            g = L.StarAttnStep(qkv=p(qkv), cache=p(cache), lengths=p(lengths), pos=p(pos) if plan is not None else None,
+                               h_rope=C.pointer(plan) if plan is not None else None, out=p(out), ws=p(ws), ld=ld, pos_ld=pos_ld, NB=nb, H=h, KV=kv,
+                               hd=hd, cap=cap, left=left, sinks=sinks, scale=hd ** -0.5 if scale is None else scale, dt=L.dt_of(qkv))
+            with _timed("attn_window_step", 0.0, float(nb) * min(cap, left + 1 + sinks) * 2 * kv * hd * qkv.element_size()):
+                L.check(L.lib().star_attn_window_step(C.byref(g), L.stream()))
+    return out
 
 
 # ---------------------------------------------------------------------------------------------------

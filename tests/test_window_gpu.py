@@ -1,0 +1,414 @@
+"""Sliding-window attention with sinks, rotary positions and the rolling key/value cache against float64, at the sizes, windows and layouts
+where they can go wrong.  Bounds are derived in window_util."""
+import pytest
+import torch
+
+from window_util import assert_within, half, heads, reference, rotate, slot_of, unpack
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from star_amd import ops
+
+DEV = "cuda"
+TYPES = [torch.bfloat16, torch.float32]
+
+
+def _rand(g, *shape, dtype=torch.float32, mul=1.0):
+    return (torch.randn(*shape, generator=g) * mul).to(DEV).to(dtype)
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _check(qkv, dout, lens, h, kv, hd, left, right, sinks, offsets=None, l=None, scale=None, backward=True):
+    """forward and backward of a batch against float64, sequence by sequence; -> (out, lse, dqkv)"""
+    nb, l = len(lens), max(lens) if l is None else l
+    kw = dict(kv_heads=kv, left=left, right=right, sinks=sinks, offsets=offsets, scale=scale)
+    out, lse = ops.attn_window_fwd(qkv, nb, l, h, hd, **kw)
+    dqkv = ops.attn_window_bwd(qkv, out, dout, lse, nb, l, h, hd, **kw) if backward else None
+    at = 0 if offsets is None else int(offsets[0])
+    for n in lens:
+        if n:
+            q, k, v = unpack(qkv[at:at + n].contiguous(), h, kv, hd)
+            want = reference(q, k, v, left, right, sinks, scale, heads(dout[at:at + n], hd) if backward else None, qkv.dtype)
+            assert_within(heads(out[at:at + n], hd), want["out"], want["tol_out"], "out of %d" % n)
+            assert_within(lse[:, at:at + n].cpu().double(), want["lse"], want["tol_lse"], "lse of %d" % n)
+            if backward:
+                assert_within(heads(dqkv[at:at + n], hd), want["dqkv"], want["tol_dqkv"], "dqkv of %d" % n)
+        at += n
+    return out, lse, dqkv
+
+
+WINDOWS = [(None, 0, 0), (None, None, 0), (0, 0, 0), (5, 0, 1), (63, 0, 4), (64, 7, 0), (65, 0, 70), (20, None, 2), (128, 128, 1), (40, 3, 1000)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("window", WINDOWS)
+def test_window_attention_against_float64(dtype, hd, window):
+    left, right, sinks = window
+    g = _gen(hd + sinks)
+    for n, h, kv in ((1, 2, 1), (33, 3, 3), (129, 4, 2), (321, 2, 1)):
+        qkv = _rand(g, 2 * n, (h + 2 * kv) * hd, dtype=dtype, mul=1.3)
+        _check(qkv, _rand(g, 2 * n, h * hd, dtype=dtype), [n, n], h, kv, hd, left, right, sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [2, 31, 32, 63, 64, 65, 127, 128, 257, 512])
+def test_every_tile_border(dtype, n):
+    g = _gen(n)
+    h, kv, hd = 2, 2, 64
+    qkv = _rand(g, n, (h + 2 * kv) * hd, dtype=dtype)
+    for left, right, sinks in ((31, 0, 1), (n, n, 0), (64, 1, 33), (1, 0, 65)):
+        _check(qkv, _rand(g, n, h * hd, dtype=dtype), [n], h, kv, hd, left, right, sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ragged_batch_leaves_rows_outside_every_sequence(dtype):
+    g = _gen(5)
+    h, kv, hd, lens = 6, 2, 32, [0, 1, 200, 0, 65, 31]
+    first, rows = 3, 3 + sum(lens) + 9
+    qkv = _rand(g, rows, (h + 2 * kv) * hd, dtype=dtype)
+    dout = _rand(g, rows, h * hd, dtype=dtype)
+    for t in (qkv, dout):                  # what no sequence holds is not read, whatever it is
+        t[:first] = float("nan")
+        t[first + sum(lens):] = float("inf")
+    offsets = torch.tensor([first] + [first + sum(lens[:i + 1]) for i in range(len(lens))], device=DEV)
+    out, lse, dqkv = _check(qkv, dout, lens, h, kv, hd, 40, 2, 3, offsets=offsets, l=256)
+    for t in (out, dqkv):
+        assert not t[:first].any() and not t[first + sum(lens):].any()
+    kw = dict(kv_heads=kv, left=40, right=2, sinks=3, offsets=offsets)
+    kept, grad = torch.full_like(out, 7.0), torch.full_like(dqkv, 7.0)
+    ops.attn_window_fwd(qkv, len(lens), 256, h, hd, out=kept, **kw)
+    ops.attn_window_bwd(qkv, out, dout, lse, len(lens), 256, h, hd, dqkv=grad, **kw)
+    body = slice(first, first + sum(lens))
+    assert torch.equal(kept[body], out[body]) and torch.equal(grad[body], dqkv[body])
+    for t in (kept, grad):
+        assert (t[:first] == 7).all() and (t[body.stop:] == 7).all()
+    # a sequence over l rows takes part with its first l; offsets that lie outside the rows stay harmless
+    short, _ = ops.attn_window_fwd(qkv[first:], 1, 64, h, hd, kv_heads=kv, offsets=torch.tensor([1, 201], device=DEV))
+    want, _ = ops.attn_window_fwd(qkv[first + 1:first + 65].contiguous(), 1, 64, h, hd, kv_heads=kv)
+    assert torch.equal(short[1:65], want) and not short[65:].any()
+    wild, _ = ops.attn_window_fwd(qkv, 3, 64, h, hd, kv_heads=kv, offsets=torch.tensor([-5, -1, rows + 4, rows + 900], device=DEV))
+    assert wild.shape == (rows, h * hd)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strided_rows_and_scale(dtype):
+    g = _gen(9)
+    n, h, kv, hd = 150, 4, 1, 64
+    w = (h + 2 * kv) * hd
+    wide = _rand(g, 2 * n, w + 64, dtype=dtype)
+    _check(wide[:, 32:32 + w], _rand(g, 2 * n, h * hd, dtype=dtype), [n, n], h, kv, hd, 70, 0, 2, scale=0.31)
+
+
+def test_sharp_and_growing_scores():
+    """scores that grow along the keys raise the running maximum in every tile; scores of hundreds leave one weight"""
+    h, hd, n = 2, 64, 320
+    for dtype in TYPES:
+        g = _gen(3)
+        qkv = _rand(g, n, 3 * h * hd, dtype=dtype)
+        ramp = torch.linspace(0, 6, n, device=DEV)[:, None].to(dtype)
+        qkv[:, h * hd:2 * h * hd] = ramp
+        qkv[:, :h * hd] = qkv[:, :h * hd].abs()
+        _check(qkv, _rand(g, n, h * hd, dtype=dtype), [n], h, h, hd, None, 0, 0)
+        _check(qkv.flip(0).contiguous(), _rand(g, n, h * hd, dtype=dtype), [n], h, h, hd, 100, None, 5)
+    sharp = _rand(_gen(4), n, 3 * h * hd, mul=12.0)
+    _check(sharp, _rand(_gen(4), n, h * hd), [n], h, h, hd, 90, 0, 2)
+
+
+def test_unbounded_window_is_the_dense_attention():
+    nb, l, h, hd = 2, 200, 4, 32
+    qkv = _rand(_gen(1), nb * l, 3 * h * hd)
+    dout = _rand(_gen(2), nb * l, h * hd)
+    out, lse = ops.attn_window_fwd(qkv, nb, l, h, hd, left=None, right=None)
+    ref, rlse = ops.attn_fwd(qkv, nb, l, h, hd)
+    torch.testing.assert_close(out, ref, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(lse.view(h, nb, l).transpose(0, 1), rlse, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(ops.attn_window_bwd(qkv, out, dout, lse, nb, l, h, hd, left=None, right=None),
+                               ops.attn_bwd(qkv, ref, dout, rlse, nb, l, h, hd), rtol=1e-4, atol=1e-5)
+
+
+def test_gradient_against_differences():
+    """float32: (f(x + e d) - f(x - e d)) / 2e against <gradient, d>.  f = sum w out; out is off by some 1e-6 of its size, so the quotient by
+    2^-24 * 16 * sqrt(elements) / e, and the third-order term by e^2: both under 2e-3 of the value's scale sqrt(elements)."""
+    g = _gen(11)
+    n, h, kv, hd, e = 90, 4, 2, 32, 2e-2
+    args = (1, n, h, hd)
+    kw = dict(kv_heads=kv, left=17, right=1, sinks=2)
+    x, w, d = (_rand(g, n, c) for c in ((h + 2 * kv) * hd, h * hd, (h + 2 * kv) * hd))
+    out, lse = ops.attn_window_fwd(x, *args, **kw)
+    grad = ops.attn_window_bwd(x, out, w, lse, *args, **kw)
+    up, down = (ops.attn_window_fwd(x + s * e * d, *args, **kw)[0].double() for s in (1, -1))
+    slope, want = float(((up - down) * w.double()).sum() / (2 * e)), float((grad.double() * d.double()).sum())
+    assert abs(slope - want) < 2e-3 * (n * h * hd) ** 0.5, (slope, want)
+
+
+def test_same_bits_every_time_and_on_another_stream():
+    g = _gen(8)
+    nb, l, h, kv, hd = 3, 500, 8, 2, 64
+    qkv, dout = _rand(g, nb * l, (h + 2 * kv) * hd, dtype=torch.bfloat16), _rand(g, nb * l, h * hd, dtype=torch.bfloat16)
+    kw = dict(kv_heads=kv, left=100, sinks=4)
+
+    def both():
+        out, lse = ops.attn_window_fwd(qkv, nb, l, h, hd, **kw)
+        return out, lse, ops.attn_window_bwd(qkv, out, dout, lse, nb, l, h, hd, **kw)
+
+    first = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = both()
+    again = both()
+    torch.cuda.synchronize()
+    for a, b, c in zip(first, other, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+# ---- rotary positions ---------------------------------------------------------------------------------------------------------
+def _rope_tol(x, dtype):
+    """two products and a sum in float32, cosine and sine within 2^-22, then the rounding to the row type"""
+    big = x.detach().cpu().double().abs().amax() * 1.5
+    return big * (6 * 2.0 ** -24 + 2 * 2.0 ** -22 + half(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,sections", [(16, (2, 3, 3)), (32, (4, 6, 6)), (32, (0, 8)), (64, (8, 8, 8)), (128, (16, 24, 24)), (128, (64,)), (144, (8, 8))])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_against_float64(dtype, hd, sections, interleaved):
+    g = _gen(hd)
+    for r, rot, more in ((1, 1, 0), (77, 5, 24), (1500, 3, 2 * hd)):
+        w = rot * hd + more
+        x = _rand(g, r, w, dtype=dtype)
+        pos = torch.randint(-50, 3000000, (len(sections), r), generator=g).to(torch.int32).to(DEV)
+        kw = dict(per_axis=r == 77, interleaved=interleaved, base=500.0 if r == 1 else 10000.0)
+        y = ops.rope_fwd(x, pos, rot, hd, sections, **kw)
+        want = rotate(x, pos, hd, rot, sections, **kw)
+        assert_within(y.cpu().double(), want, _rope_tol(x, dtype), "rope")
+        assert torch.equal(y[:, rot * hd:], x[:, rot * hd:])
+        back = ops.rope_bwd(x, pos, rot, hd, sections, **kw)
+        assert_within(back.cpu().double(), rotate(x, pos, hd, rot, sections, sign=-1.0, **kw), _rope_tol(x, dtype), "rope gradient")
+        # in place, in rows of a wider matrix
+        wide = torch.full((r, w + 40), 3.0, dtype=dtype, device=DEV)
+        view = wide[:, 16:16 + w]
+        view.copy_(x)
+        assert ops.rope_fwd(view, pos, rot, hd, sections, out=view, **kw) is view
+        assert torch.equal(view, y) and (wide[:, :16] == 3).all() and (wide[:, 16 + w:] == 3).all()
+        assert torch.equal(ops.rope_fwd(view.copy_(x), pos, rot, hd, sections, **kw), y)
+
+
+def test_rope_gradient_is_the_adjoint_and_matches_differences():
+    """a linear map: <rope(x), w> = <x, rope_bwd(w)>, and its difference quotient along d is <d, rope_bwd(w)> exactly but for rounding:
+    sums of n products, each within 2^-21 of 2, in float64 -> n^0.5 * 2^-20 * 8"""
+    g = _gen(2)
+    r, rot, hd, sections = 200, 6, 64, (8, 12, 12)
+    x, w, d = (_rand(g, r, (rot + 2) * hd) for _ in range(3))
+    pos = torch.randint(0, 100000, (3, r), generator=g).to(torch.int32).to(DEV)
+    f = lambda v: ops.rope_fwd(v, pos, rot, hd, sections).double()      # noqa: E731
+    grad = ops.rope_bwd(w, pos, rot, hd, sections).double()
+    tol = x.numel() ** 0.5 * 2.0 ** -17
+    assert abs(float((f(x) * w.double()).sum() - (x.double() * grad).sum())) < tol
+    slope = float(((f(x + d) - f(x - d)) * w.double()).sum() / 2)
+    assert abs(slope - float((d.double() * grad).sum())) < 4 * tol
+
+
+# ---- the rolling cache ----------------------------------------------------------------------------------------------------------
+def _append_reference(cache, qkv, spans, lengths, h, sinks):
+    kv, cap, hd = cache.shape[2:]
+    ring = cap - sinks
+    want = cache.clone()
+    x = qkv.reshape(qkv.shape[0], h + 2 * kv, hd)
+    for b, (lo, hi) in enumerate(spans):
+        for t in range(lo, hi):
+            p = lengths[b] - (hi - t)
+            if p >= 0 and (p < sinks or p >= lengths[b] - ring):
+                want[0, b, :, slot_of(p, sinks, cap)] = x[t, h:h + kv]
+                want[1, b, :, slot_of(p, sinks, cap)] = x[t, h + kv:]
+    return want
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,kv,h,cap,sinks", [(16, 3, 3, 40, 4), (64, 2, 8, 33, 0), (128, 1, 2, 300, 70), (32, 4, 4, 5, 4)])
+def test_kv_append(dtype, hd, kv, h, cap, sinks):
+    g = _gen(cap)
+    for lens, before in (([3, 3], 0), ([1, 1], 500), ([0, 90, 7, 400], 11), ([64], 2)):
+        ragged = len(set(lens)) > 1
+        nb, rows = len(lens), sum(lens) + (5 if ragged else 0)
+        wide = _rand(g, rows, (h + 2 * kv) * hd + 32, dtype=dtype)
+        qkv = wide[:, :(h + 2 * kv) * hd]
+        starts = [sum(lens[:b]) for b in range(nb)]
+        lengths = [before + n for n in lens]
+        cache = _rand(g, 2, nb, kv, cap, hd, dtype=dtype)
+        want = _append_reference(cache, qkv, [(s, s + n) for s, n in zip(starts, lens)], lengths, h, sinks)
+        offsets = torch.tensor(starts + [sum(lens)], device=DEV) if ragged else None
+        got = ops.kv_append(qkv, cache, torch.tensor(lengths, dtype=torch.int32, device=DEV), max(lens), h, sinks=sinks, offsets=offsets)
+        assert got is cache and torch.equal(cache, want), (lens, before)
+
+
+def _step_reference(qkv, cache, lengths, h, left, sinks, pos, rope, scale):
+    """float64 result, its bound and the cache afterwards (its type's values)"""
+    nb = qkv.shape[0]
+    kv, cap, hd = cache.shape[2:]
+    rep = h // kv
+    x = rotate(qkv, pos, hd, h + kv, **rope) if rope else qkv.detach().cpu().double()
+    x = x.view(nb, h + 2 * kv, hd)
+    want = cache.clone()
+    out, tol = torch.zeros(nb, h, hd, dtype=torch.float64), torch.full((nb, h, hd), 1e-30, dtype=torch.float64)
+    for b in range(nb):
+        p = lengths[b] - 1
+        if p < 0:
+            continue
+        new = slot_of(p, sinks, cap)
+        want[0, b, :, new], want[1, b, :, new] = x[b, h:h + kv].to(cache.dtype).to(DEV), x[b, h + kv:].to(cache.dtype).to(DEV)
+        at = sorted(set(range(min(sinks, p + 1))) | set(range(max(0, p - left), p + 1)))
+        at = [slot_of(i, sinks, cap) for i in at]
+        k, v = (t[b][:, at].cpu().double().repeat_interleave(rep, 0) for t in want)
+        q = x[b, :h, None]
+        s = (q @ k.transpose(1, 2)) * scale
+        w = torch.softmax(s, 2)
+        # float32 throughout: the turned query within 2^-20 of its size, sums of hd, the new key possibly one rounding step of its type off
+        es = (scale * (q.abs() @ k.abs().transpose(1, 2))).amax(2, keepdim=True) * (2.0 ** -24 * (hd + 4) + 2.0 ** -20)
+        rel = 2 * es + 2.0 ** -24 * (2 * len(at) + 16)
+        out[b] = (w @ v)[:, 0]
+        new_key = scale * (q.abs()[:, 0] * k.abs()[:, -1]).sum(1) * 2 * half(cache.dtype) if rope else torch.zeros(h)
+        tol[b] = (rel * (w @ v.abs()))[:, 0] + half(cache.dtype) * out[b].abs() + new_key[:, None] * 2 * (w @ v.abs())[:, 0] * w[:, 0, -1:] + 1e-30
+    return out.view(nb, -1), tol.view(nb, -1), want
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,kv,h", [(16, 2, 2), (32, 1, 3), (64, 2, 10), (64, 12, 12), (128, 2, 16), (128, 1, 12)])
+def test_step(dtype, hd, kv, h):
+    g = _gen(hd + h)
+    rope = dict(sections=(hd // 8, hd // 8, hd // 4), interleaved=hd == 32)
+    for cap, left, sinks, lengths in ((40, 35, 4, [1, 4, 5, 0, 39, 40, 41, 200]), (700, 600, 70, [700, 3000, 65, 71, 601]), (9, 0, 8, [3, 50]), (2000, None, 0, [1999, 2001])):
+        for rp in (rope, None):
+            nb = len(lengths)
+            qkv = _rand(g, nb, (h + 2 * kv) * hd + 16, dtype=dtype)[:, :(h + 2 * kv) * hd]
+            cache = _rand(g, 2, nb, kv, cap, hd, dtype=dtype)
+            for b, n in enumerate(lengths):          # slots that hold no token yet are not read, whatever they are
+                cache[:, b, :, min(cap, max(0, n - 1)):] = float("nan")
+            if left is not None and left < cap - sinks - 1:
+                for b, n in enumerate(lengths):      # nor are tokens that lie between the sinks and the window
+                    for q in range(sinks, n - 1 - left):
+                        if q >= n - (cap - sinks):
+                            cache[:, b, :, slot_of(q, sinks, cap)] = float("inf")
+            pos = torch.randint(0, 300000, (3, nb), generator=g).to(torch.int32).to(DEV) if rp else None
+            bound = cap - sinks - 1 if left is None else left
+            want, tol, after = _step_reference(qkv, cache, lengths, h, bound, sinks, pos, rp, hd ** -0.5)
+            n32 = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+            out = ops.attn_window_step(qkv, cache, n32, h, left=left, sinks=sinks, pos=pos, **(rp or {}))
+            assert_within(out.cpu().double(), want, tol, "step cap %d" % cap)
+            assert not out[[i for i, n in enumerate(lengths) if n == 0]].any()
+            same = (cache == after) | (cache.isnan() & after.isnan())
+            if rp and not same.all():      # a turned key may round to the neighbouring value
+                off = (cache.double() - after.double()).abs()[~same]
+                assert (off <= 2 * 2 * half(dtype) * after.double().abs()[~same] + 2.0 ** -20).all()
+            else:
+                assert same.all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prefill_then_steps_are_the_whole_sequence(dtype):
+    """rotate + attend + fill the cache for a prompt, then single tokens: the rows of one forward pass over the whole sequence"""
+    g = _gen(21)
+    h, kv, hd, left, sinks, cap, prompt, total = 8, 2, 64, 50, 3, 60, 100, 131
+    sections = (8, 12, 12)
+    qkv = _rand(g, total, (h + 2 * kv) * hd, dtype=dtype)
+    t = torch.arange(total, device=DEV)
+    pos = torch.stack((4000 + t // 16, t // 4 % 4, t % 4)).to(torch.int32)
+    turned = ops.rope_fwd(qkv, pos, h + kv, hd, sections)
+    whole, _ = ops.attn_window_fwd(turned, 1, total, h, hd, kv_heads=kv, left=left, sinks=sinks, want_lse=False)
+    cache = torch.full((2, 1, kv, cap, hd), float("nan"), dtype=dtype, device=DEV)
+    n = torch.tensor([prompt], dtype=torch.int32, device=DEV)
+    ops.kv_append(turned[:prompt], cache, n, prompt, h, sinks=sinks)
+    q, k, v = unpack(turned, h, kv, hd)
+    want = reference(q, k, v, left, 0, sinks, dtype=dtype)
+    assert_within(heads(whole, hd), want["out"], want["tol_out"], "whole")
+    for i in range(prompt, total):
+        n += 1
+        row = ops.attn_window_step(qkv[i:i + 1], cache, n, h, left=left, sinks=sinks, pos=pos[:, i:i + 1].contiguous(), sections=sections)
+        # the step turns the query without rounding it to the row type: one rounding of q more in the whole pass' scores
+        more = 4 * half(dtype) * (q[:, i].abs()[:, None] @ k.abs().repeat_interleave(h // kv, 0).transpose(1, 2)).amax() * hd ** -0.5 * v.abs().max()
+        assert_within(heads(row, hd)[:, 0], want["out"][:, i], want["tol_out"][:, i] + more, "token %d" % i)
+
+
+def test_training_chain_against_float64():
+    """rotate, attend, backward through both: the gradient of the packed rows before the rotation"""
+    g = _gen(31)
+    n, h, kv, hd, sections = 140, 4, 2, 32, (4, 6, 6)
+    x, w = _rand(g, n, (h + 2 * kv) * hd), _rand(g, n, h * hd)
+    pos = torch.randint(0, 5000, (3, n), generator=g).to(torch.int32).to(DEV)
+    turned = ops.rope_fwd(x, pos, h + kv, hd, sections)
+    out, lse = ops.attn_window_fwd(turned, 1, n, h, hd, kv_heads=kv, left=30, sinks=2)
+    grad = ops.attn_window_bwd(turned, out, w, lse, 1, n, h, hd, kv_heads=kv, left=30, sinks=2)
+    grad = ops.rope_bwd(grad, pos, h + kv, hd, sections, out=grad)
+    q, k, v = unpack(rotate(x, pos, hd, h + kv, sections), h, kv, hd)
+    want = reference(q, k, v, 30, 0, 2, dout=heads(w, hd))
+    rows = rotate(want["dqkv"].transpose(0, 1).reshape(n, -1), pos, hd, h + kv, sections, sign=-1.0)
+    # float32 rotations of q, k (2^-20 of their size) move the scores by some 1e-5; everything is of size one
+    torch.testing.assert_close(grad.cpu().double(), rows, rtol=1e-4, atol=2e-4)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_captured_and_replayed(dtype):
+    """one graph of a training pass and one of a decoding step; replays interleaved with eager work give the eager results every time"""
+    g = _gen(41)
+    nb, l, h, kv, hd, cap, sinks = 2, 300, 4, 2, 64, 700, 5
+    sections = (8, 12, 12)
+    w = (h + 2 * kv) * hd
+    x, dout = _rand(g, nb * l, w, dtype=dtype), _rand(g, nb * l, h * hd, dtype=dtype)
+    pos = torch.randint(0, 5000, (3, nb * l), generator=g).to(torch.int32).to(DEV)
+    row, rpos = _rand(g, nb, w, dtype=dtype), torch.randint(0, 5000, (3, nb), generator=g).to(torch.int32).to(DEV)
+    lengths = torch.tensor([l, l], dtype=torch.int32, device=DEV)
+    cache = torch.zeros(2, nb, kv, cap, hd, dtype=dtype, device=DEV)
+
+    def train():
+        t = ops.rope_fwd(x, pos, h + kv, hd, sections)
+        out, lse = ops.attn_window_fwd(t, nb, l, h, hd, kv_heads=kv, left=80, sinks=sinks)
+        return out, ops.rope_bwd(ops.attn_window_bwd(t, out, dout, lse, nb, l, h, hd, kv_heads=kv, left=80, sinks=sinks), pos, h + kv, hd, sections)
+
+    def step():
+        lengths.add_(1)
+        return ops.attn_window_step(row, cache, lengths, h, sinks=sinks, pos=rpos, sections=sections)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        train(), step()
+    torch.cuda.current_stream().wait_stream(side)
+    lengths.fill_(l)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    with torch.cuda.graph(graphs[0]):
+        got_train = train()
+    with torch.cuda.graph(graphs[1]):
+        got_step = step()
+    for i in range(4):
+        x.copy_(_rand(g, nb * l, w, dtype=dtype))
+        row.copy_(_rand(g, nb, w, dtype=dtype))
+        lengths.fill_(l + 100 * i)
+        before = cache.clone()
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in (*got_train, got_step, cache, lengths)]
+        cache.copy_(before)
+        lengths.fill_(l + 100 * i)
+        eager = (*train(), step(), cache, lengths)
+        for a, b in zip(kept, eager):
+            assert torch.equal(a, b), i
+
+
+def test_empty_batches():
+    none = torch.zeros(0, 192, device=DEV)
+    out, lse = ops.attn_window_fwd(none, 2, 0, 4, 16, offsets=torch.zeros(3, dtype=torch.int64, device=DEV))
+    assert out.shape == (0, 64) and lse.shape == (4, 0)
+    assert ops.attn_window_bwd(none, out, out, lse, 2, 0, 4, 16, offsets=torch.zeros(3, dtype=torch.int64, device=DEV)).shape == (0, 192)
+    assert ops.rope_fwd(none, torch.zeros(1, 0, dtype=torch.int32, device=DEV), 8, 16, (8,)).shape == (0, 192)
+    cache = torch.ones(2, 2, 4, 8, 16, device=DEV)
+    ops.kv_append(none, cache, torch.zeros(2, dtype=torch.int32, device=DEV), 0, 4)
+    out = ops.attn_window_step(torch.ones(2, 192, device=DEV), cache, torch.zeros(2, dtype=torch.int32, device=DEV), 4)
+    assert not out.any() and (cache == 1).all()
+    idle, _ = ops.attn_window_fwd(torch.ones(5, 192, device=DEV), 2, 4, 4, 16, offsets=torch.zeros(3, dtype=torch.int64, device=DEV))
+    assert not idle.any()
