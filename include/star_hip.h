@@ -240,21 +240,22 @@ int star_rope(const void* x, int64_t x_ld, void* y, int64_t y_ld, const int32_t*
  * L are used (L = the longest sequence); rows of no sequence are neither read nor written.  hd in {16, 32, 64, 128}.
  *   out dt [R, H*hd]; lse float32 [H, R]: log2-domain log-sum-exp of every row (optional in the forward pass).
  * star_attn_window_bwd: reads out, lse, dout dt [R, H*hd]; writes dqkv dt [R, (H + 2 KV) hd] (dense rows; gradients of a shared key/value head
- *   are summed over its query heads) and the workspace delta float32 [H, R].  No atomics: bitwise reproducible. */
+ *   are summed over its query heads).  ws float32 [star_attn_window_bwd_ws(...)], any content.  No atomics: bitwise reproducible. */
 typedef struct StarAttnWindow {
     const void* qkv;
     const int64_t* offsets;   /* optional */
     void* out;
     float* lse;
-    const void* dout;         /* backward only, as dqkv and delta */
+    const void* dout;         /* backward only, as dqkv and ws */
     void* dqkv;
-    float* delta;
+    float* ws;
     int64_t ld, R;            /* R: rows of qkv (NB * L without offsets) */
     int32_t NB, L, H, KV, hd, left, right, sinks;
     float scale;
     int32_t dt;
 } StarAttnWindow;
 int star_attn_window_fwd(const StarAttnWindow* g, void* stream);
+int64_t star_attn_window_bwd_ws(int64_t R, int NB, int L, int H, int KV, int hd, int left, int sinks);
 int star_attn_window_bwd(const StarAttnWindow* g, void* stream);
 /* Rolling cache dt [2 (keys, values), NB, KV, cap, hd]: the token at position p lies in slot p for p < sinks, else in slot
  * sinks + (p - sinks) % (cap - sinks).  lengths int32 [NB]: the sequence's tokens INCLUDING the new ones.

@@ -44,7 +44,7 @@ class StarRope(C.Structure):
 
 class StarAttnWindow(C.Structure):
     _fields_ = [("qkv", C.c_void_p), ("offsets", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("dout", C.c_void_p), ("dqkv", C.c_void_p),
-                ("delta", C.c_void_p), ("ld", C.c_int64), ("R", C.c_int64), ("NB", C.c_int32), ("L", C.c_int32), ("H", C.c_int32), ("KV", C.c_int32),
+                ("ws", C.c_void_p), ("ld", C.c_int64), ("R", C.c_int64), ("NB", C.c_int32), ("L", C.c_int32), ("H", C.c_int32), ("KV", C.c_int32),
                 ("hd", C.c_int32), ("left", C.c_int32), ("right", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float), ("dt", C.c_int32)]
 
 
@@ -78,6 +78,7 @@ _SIGS = {
     "star_attn_bwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "star_rope": (C.c_int, [_P, _L, _P, _L, _P, _L, C.POINTER(StarRope), _I, _I, _I, _I, _I, _I, _P]),
     "star_attn_window_fwd": (C.c_int, [C.POINTER(StarAttnWindow), _P]),
+    "star_attn_window_bwd_ws": (C.c_int64, [_L, _I, _I, _I, _I, _I, _I, _I]),
     "star_attn_window_bwd": (C.c_int, [C.POINTER(StarAttnWindow), _P]),
     "star_kv_append": (C.c_int, [_P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "star_attn_window_step_ws": (C.c_int64, [_I, _I, _I, _I, _I, _I, _I]),

@@ -495,8 +495,8 @@ def attn_window_bwd(qkv, out, dout, lse, nb, l, h, hd, kv_heads=None, left=None,
             dqkv = _fresh(r, w, qkv, offsets)
         assert dqkv.shape == (r, w) and dqkv.dtype == qkv.dtype and dqkv.is_contiguous()
         if r:
-            delta = torch.empty(h, r, dtype=torch.float32, device=qkv.device)
-            g.out, g.lse, g.dout, g.dqkv, g.delta = p(out), p(lse), p(dout), p(dqkv), p(delta)
+            ws = torch.empty(L.lib().star_attn_window_bwd_ws(r, nb, l, h, g.KV, hd, g.left, sinks), dtype=torch.float32, device=qkv.device)
+            g.out, g.lse, g.dout, g.dqkv, g.ws = p(out), p(lse), p(dout), p(dqkv), p(ws)
             with _timed("attn_window_bwd", 0.0, float(r) * 2 * (w + h * hd) * qkv.element_size()):
                 L.check(L.lib().star_attn_window_bwd(C.byref(g), L.stream()))
     return dqkv

@@ -20,7 +20,7 @@ def _refused(rc, *words):
 
 
 def _attn(**kw):
-    a = dict(qkv=1 << 20, out=1 << 20, lse=1 << 20, dout=1 << 20, dqkv=1 << 20, delta=1 << 20, ld=8 * 64, R=40, NB=2, L=20, H=4, KV=2, hd=64,
+    a = dict(qkv=1 << 20, out=1 << 20, lse=1 << 20, dout=1 << 20, dqkv=1 << 20, ws=1 << 20, ld=8 * 64, R=40, NB=2, L=20, H=4, KV=2, hd=64,
              left=5, right=0, sinks=1, scale=0.125, dt=L.BF16)
     a.update(kw)
     return L.StarAttnWindow(**a)
@@ -39,7 +39,7 @@ def test_window_attention_refuses(change, words):
     _refused(L.lib().star_attn_window_fwd(None, None), "null")
 
 
-@pytest.mark.parametrize("field", ["lse", "dout", "dqkv", "delta"])
+@pytest.mark.parametrize("field", ["lse", "dout", "dqkv", "ws"])
 def test_window_backward_refuses_missing_operands(field):
     _refused(L.lib().star_attn_window_bwd(C.byref(_attn(**{field: None})), None), "star_attn_window_bwd", "null")
 
