@@ -14,17 +14,13 @@
 // per lane in both, so the tile layout and the address arithmetic are shared.
 #include "common.h"
 #include <atomic>
-#ifndef DQ_OCC
-#define DQ_OCC 2
-#endif
-#ifndef DKV_OCC
-#define DKV_OCC 1
-#endif
+#include <type_traits>
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) short short4_t;
 typedef __attribute__((ext_vector_type(8))) short short8_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 
 #define WT 256                    // threads of a block: four waves of 32 queries (backward of K and V: 32 keys)
@@ -43,100 +39,137 @@ template <typename T, int HD, int ROWS = sizeof(T) == 2 ? 64 : 32> struct WCfg {
     static constexpr int KT = ROWS;                         // rows of a tile
     static constexpr int KB = KT / 32;
     static constexpr int TILE = KT * RB;
-    static constexpr int NLD = (KT * CH + WT - 1) / WT;     // 16-byte loads of a thread per tile
-    // rows per 256 bytes of LDS: the chunk index is XORed with the row's number inside that, so that 16 lanes reading one chunk of 16
-    // successive rows (or one row's 16 chunks) touch all banks once
-    static constexpr int SH = RB >= 256 ? 0 : (RB == 128 ? 1 : (RB == 64 ? 2 : 3));
-    static constexpr int XM = CH < 16 ? CH - 1 : 15;
+    static constexpr int RPP = 1024 / RB;                   // rows of a 1-KiB piece: what one wave's LDS-DMA instruction fills
+    static constexpr int NP = TILE / 1024;                  // pieces of an image
+    static constexpr int NI = 2 * NP / 4;                   // pieces that each of the four waves brings per pair of images
+    // The 16-byte chunks of a row are permuted by the row's number, so that neither 16 lanes reading one chunk of 16 successive rows nor
+    // 32 lanes of a transposing read (4 rows x 4 chunks) hit one of the 64 banks twice.
     static __device__ __forceinline__ int swizzle(int row) {
-        if constexpr (CH == 2) return (row >> 2) & 1;
-        else if constexpr (CH == 4) return (row & 2) | ((row >> 2) & 1);
-        else return ((row & 3) << 1) | ((row >> 2) & 1);
+        if constexpr (CH == 2) return (row >> 3) & 1;
+        else if constexpr (CH == 4) return (row >> 2) & 3;
+        else if constexpr (CH == 8) return ES == 2 ? ((row >> 1 & 1) << 2) | (row >> 2 & 3) : (row >> 1) & 7;
+        else return ES == 2 ? ((row & 3) << 2) | (row >> 2 & 3) : row & 15;
     }
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swizzle(row)) << 4); }
 };
 
-template <typename T, int HD> __device__ __forceinline__ int img_off(int row, int chunk) {
-    using C = WCfg<T, HD>;
-#ifndef OLD_SWZ
-    return row * C::RB + ((chunk ^ C::swizzle(row)) << 4);
-#endif
-    return row * C::RB + ((chunk ^ ((row >> C::SH) & C::XM)) << 4);
-}
-
-template <class C> struct TileRegs { uint4 v[C::NLD]; };
-
-// Byte offsets of a thread's 16-byte chunks inside a tile of rows `ld` elements apart, and the loads of the tile that starts at row0: buffer
-// loads, whose range check makes the rows from nrows on zeros without a branch.
-template <class C> struct TileAt {
-    unsigned off[C::NLD];
-    __device__ __forceinline__ TileAt(int64_t ld, int tid) {
-#pragma unroll
-        for (int i = 0; i < C::NLD; ++i) {
-            const int id = tid + i * WT;
-            off[i] = id < C::KT * C::CH ? (unsigned)(id / C::CH * ld * C::ES + (id % C::CH) * 16) : 0x7ffffff0u;
-        }
-    }
-};
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int64_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (unsigned)(bytes < 0 ? 0 : bytes > 0x7fffffe0 ? 0x7fffffe0 : bytes), 0x00020000);
 }
-template <class C, typename T>
-__device__ __forceinline__ void load_tile(TileRegs<C>& t, const TileAt<C>& at, const T* __restrict__ base, int64_t ld, int row0, int nrows) {
-    typedef __attribute__((ext_vector_type(4))) unsigned u4;
-    const __amdgpu_buffer_rsrc_t rs = rows_rsrc(base + row0 * ld, ((nrows - 1 - row0) * ld + C::HDIM) * C::ES);
-#pragma unroll
-    for (int i = 0; i < C::NLD; ++i) t.v[i] = __builtin_bit_cast(uint4, (u4)__builtin_amdgcn_raw_buffer_load_b128(rs, at.off[i], 0, 0));
+// Where a lane's 16 bytes of piece `p` of an image lie in memory: LDS-DMA fills LDS lane by lane, so the image's permutation is applied to
+// the source.  Rows past the descriptor's end arrive as zeros.
+template <class C> __device__ __forceinline__ unsigned piece_src(int p, int lane, int64_t ld) {
+    const int row = p * C::RPP + lane / C::CH;
+    return (unsigned)(row * ld * C::ES) + (((lane % C::CH) ^ C::swizzle(row)) << 4);
 }
-template <class C> __device__ __forceinline__ void store_tile(unsigned char* lds, const TileRegs<C>& t, int tid) {
-#pragma unroll
-    for (int i = 0; i < C::NLD; ++i) {
-        const int id = tid + i * WT;
-        if (id < C::KT * C::CH) *reinterpret_cast<uint4*>(lds + img_off<typename C::Type, C::HDIM>(id / C::CH, id % C::CH)) = t.v[i];
-    }
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned char* lds, unsigned off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 16, off, 0, 0, 0);
+}
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// every wave's DMA of the tile has landed, and every wave is done with the stage that is filled next
+template <int N> __device__ __forceinline__ void tile_ready(bool last) {
+    if (last) wait_vm<0>();
+    else wait_vm<N>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// 16 bytes of a row.  (A compiler-visible read through another type, uint4 or a builtin, would be given a wait for every LDS-DMA in flight.)
+template <typename T> struct Frag { typedef short8_t V; };
+template <> struct Frag<float> { typedef f32x4_t V; };
+template <class C> __device__ __forceinline__ typename Frag<typename C::Type>::V row_frag(const unsigned char* lds, int row, int chunk) {
+    return *reinterpret_cast<const typename Frag<typename C::Type>::V*>(lds + C::at(row, chunk));
+}
+// a global load consumed here: the compiler then has no wait of its own to put into the loop
+template <typename V> __device__ __forceinline__ void pin(V& v) {
+    i32x4_t t = __builtin_bit_cast(i32x4_t, v);
+    asm volatile("" : "+v"(t));
+    v = __builtin_bit_cast(V, t);
 }
 
 // acc += A B^T over one 16-byte fragment of each operand (bf16: 8 + 8 elements of the two lane halves, float32: 4 + 4)
-template <typename T> __device__ __forceinline__ f32x16_t mma_frag(uint4 a, uint4 b, f32x16_t c) {
+template <typename T> __device__ __forceinline__ f32x16_t mma_frag(typename Frag<T>::V a, typename Frag<T>::V b, f32x16_t c) {
     if constexpr (sizeof(T) == 2) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     } else {
-        const f32x4_t x = __builtin_bit_cast(f32x4_t, a), y = __builtin_bit_cast(f32x4_t, b);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
         return c;
     }
 }
 
-// acc += B A^T for the 32 rows blk .. blk+31 of an image: A = the image transposed (MFMA row = column 32 db + 0..31 of the image), B = the
-// 32 x 32 accumulator block s as it lies (its rows are the image's rows).  bf16: the image is read by the transposing LDS read in the row
-// order in which an accumulator holds its registers; float32: register e of the two halves is one product step.
-template <typename T, int HD> __device__ __forceinline__ f32x16_t mma_tr(const unsigned char* lds, int blk, int db, const f32x16_t& s, f32x16_t acc, int lane) {
-    if constexpr (sizeof(T) == 2) {
-        const int g = lane >> 4, i = lane & 15, h2 = g >> 1;
-        const int colbyte = (db * 32 + (HD >= 32 ? (g & 1) : 0) * 16 + 4 * (i & 3)) * 2;
+// Products with a transposed image: acc[db] += A_db B for rows blk .. blk+31 of the image, A_db = its columns 32 db .. 32 db + 31 as MFMA rows, B
+// = the 32 x 32 accumulator block s as it lies (its rows are the image's rows).
+// bf16: transposing LDS reads, in the row order in which an accumulator holds its registers.  They are issued in assembly, because the compiler
+// puts a wait for every LDS-DMA in flight before its own, and waited for in the same block.  float32: register e of the two lane halves is one
+// product step, its operand an ordinary read.
+template <class C> struct TrAt {
+    unsigned lo[C::DB], hi[C::DB];          // bf16: byte offsets of rows (0 | 8) + 4 h2 + i / 4 in the image
+    __device__ __forceinline__ TrAt(int lane) {
+        const int g = lane >> 4, i = lane & 15;
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-            bf16x8_t p;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = (__bf16)s[8 * s2 + j];
-            const int row = blk + 16 * s2 + 4 * h2 + (i >> 2);
-            const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) short4_t*)(lds + img_off<T, HD>(row, colbyte >> 4) + (colbyte & 15)));
-            const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) short4_t*)(lds + img_off<T, HD>(row + 8, colbyte >> 4) + (colbyte & 15)));
-            const short8_t a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), p, acc, 0, 0, 0);
-        }
-    } else {
-        const int d = db * 32 + (HD >= 32 ? (lane & 31) : (lane & 15)), h2 = lane >> 5;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int row = blk + (e & 3) + 8 * (e >> 2) + 4 * h2;
-            const float a = *reinterpret_cast<const float*>(lds + img_off<T, HD>(row, d >> 2) + (d & 3) * 4);
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[e], acc, 0, 0, 0);
+        for (int db = 0; db < C::DB; ++db) {
+            const int col = db * 64 + (C::HDIM >= 32 ? (g & 1) * 32 : 0) + (i & 3) * 8, row = 4 * (g >> 1) + (i >> 2);
+            lo[db] = C::at(row, col >> 4) + (col & 15);
+            hi[db] = C::at(row + 8, col >> 4) + (col & 15);
         }
     }
-    return acc;
+};
+template <int OFF, int STEP> __device__ __forceinline__ void tr_read(unsigned lo, unsigned hi, short4_t (&r)[4]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %5 offset:%6\n\t"
+                 "ds_read_b64_tr_b16 %2, %4 offset:%7\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+                 : "v"(lo), "v"(hi), "n"(OFF), "n"(OFF + STEP)
+                 : "memory");
+}
+template <int OFF, int STEP> __device__ __forceinline__ void tr_read2(unsigned lo, unsigned hi, unsigned lo2, unsigned hi2, short4_t (&r)[4], short4_t (&s)[4]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %2, %8 offset:%13\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %11 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %6, %10 offset:%13\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
+                 : "v"(lo), "v"(hi), "v"(lo2), "v"(hi2), "n"(OFF), "n"(OFF + STEP)
+                 : "memory");
+}
+__device__ __forceinline__ f32x16_t mma_tr16(const short4_t (&r)[4], bf16x8_t p0, bf16x8_t p1, f32x16_t acc) {
+    const short8_t a = {r[0][0], r[0][1], r[0][2], r[0][3], r[1][0], r[1][1], r[1][2], r[1][3]};
+    const short8_t b = {r[2][0], r[2][1], r[2][2], r[2][3], r[3][0], r[3][1], r[3][2], r[3][3]};
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), p0, acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, b), p1, acc, 0, 0, 0);
+}
+template <class C, int BLK> __device__ __forceinline__ void mma_tr(const unsigned char* img, const TrAt<C>& at, const f32x16_t& s, f32x16_t (&acc)[C::DB], int lane) {
+    if constexpr (C::ES == 2) {
+        const unsigned base = lds_u32(img);
+        bf16x8_t p0, p1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            p0[j] = (__bf16)s[j];
+            p1[j] = (__bf16)s[8 + j];
+        }
+        short4_t r[4], t[4];
+        if constexpr (C::DB == 1) {
+            tr_read<BLK * C::RB, 16 * C::RB>(base + at.lo[0], base + at.hi[0], r);
+            acc[0] = mma_tr16(r, p0, p1, acc[0]);
+        } else {
+#pragma unroll
+            for (int db = 0; db < C::DB; db += 2) {
+                tr_read2<BLK * C::RB, 16 * C::RB>(base + at.lo[db], base + at.hi[db], base + at.lo[db + 1], base + at.hi[db + 1], r, t);
+                acc[db] = mma_tr16(r, p0, p1, acc[db]);
+                acc[db + 1] = mma_tr16(t, p0, p1, acc[db + 1]);
+            }
+        }
+    } else {
+        const int h2 = lane >> 5;
+#pragma unroll
+        for (int db = 0; db < C::DB; ++db) {
+            const int d = db * 32 + (C::HDIM >= 32 ? (lane & 31) : (lane & 15));
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                    *reinterpret_cast<const float*>(img + C::at(BLK + (e & 3) + 8 * (e >> 2) + 4 * h2, d >> 2) + (d & 3) * 4), s[e], acc[db], 0, 0, 0);
+        }
+    }
 }
 
 // row index of accumulator register e on lane half h2
@@ -220,11 +253,32 @@ template <int KT> __device__ __forceinline__ int key_tiles(int q0, int q1, int l
     return ns + hi / KT - w0 + 1;
 }
 
-// The K and V tiles are double-buffered in LDS: while one pair is worked on the next is on its way through registers, K first (written
-// before the softmax), then V, so that only one image's worth of registers is held; one barrier per tile.
+// A ring of STAGES (K image | V image) stages: while one tile is worked on the next STAGES - 1 are on their way, without registers.
+template <class C> struct KvRing {
+    static constexpr int STAGE = 2 * C::TILE, STAGES = STAGE > 16384 ? 2 : 3;
+    const typename C::Type* k;              // key 0 of the head; its value lies v columns further on
+    int64_t ld;
+    int v, len, wave;
+    unsigned src[C::NI];
+    __device__ __forceinline__ KvRing(const typename C::Type* k_, int64_t ld_, int v_, int len_, int wave_, int lane) : k(k_), ld(ld_), v(v_), len(len_), wave(wave_) {
+#pragma unroll
+        for (int j = 0; j < C::NI; ++j) {
+            const int p = wave * C::NI + j, isv = p >= C::NP;
+            src[j] = piece_src<C>(isv ? p - C::NP : p, lane, ld) + (isv ? v * C::ES : 0);
+        }
+    }
+    __device__ __forceinline__ void issue(int tile, unsigned char* stage) const {
+        const int64_t row0 = (int64_t)tile * C::KT;
+        const __amdgpu_buffer_rsrc_t rs = rows_rsrc(k + row0 * ld, ((len - 1 - row0) * ld + v + C::HDIM) * C::ES);     // row `len` starts behind this
+#pragma unroll
+        for (int j = 0; j < C::NI; ++j) dma16(rs, stage + (wave * C::NI + j) * 1024, src[j]);
+    }
+};
+
 template <typename T, int HD>
 __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_fwd_kernel(WArgs a) {
     using C = WCfg<T, HD>;
+    using Ring = KvRing<C>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int nrb = (a.L + WROWS - 1) / WROWS;
     const int work = xcd_remap(blockIdx.x, gridDim.x);      // the row blocks of one head run on one XCD and share its L2
@@ -234,18 +288,16 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_fw
     if (rblk * WROWS >= len) return;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h2 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = a.H + h / (a.H / a.KV);
     const T* base = (const T*)a.qkv + start * a.ld;
-    const T *kb_ = base + hk * HD, *vb_ = kb_ + a.KV * HD;
     const int q0 = rblk * WROWS + wave * 32, q = q0 + r;
     const float c = a.scale * LOG2E;
 
-    uint4 qf[C::FR];
+    typename Frag<T>::V qf[C::FR] = {};
 #pragma unroll
-    for (int j = 0; j < C::FR; ++j) {
-        qf[j] = make_uint4(0, 0, 0, 0);
-        if (q < len) qf[j] = *reinterpret_cast<const uint4*>(base + (int64_t)q * a.ld + h * HD + (2 * j + h2) * (16 / C::ES));
-    }
+    for (int j = 0; j < C::FR; ++j)
+        if (q < len) qf[j] = *reinterpret_cast<const typename Frag<T>::V*>(base + (int64_t)q * a.ld + h * HD + (2 * j + h2) * (16 / C::ES));
+#pragma unroll
+    for (int j = 0; j < C::FR; ++j) pin(qf[j]);
     f32x16_t o[C::DB];
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) o[db] = splat16(0.f);
@@ -254,79 +306,64 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_fw
     int ns, w0;
     const int nt = key_tiles<C::KT>(rblk * WROWS, min(rblk * WROWS + WROWS, len) - 1, len, a.left, a.right, a.sinks, ns, w0);
     const int qlast = min(q0 + 31, len - 1);
-    int t = ns > 0 ? 0 : w0;
-    const TileAt<C> at(a.ld, tid);
-    TileRegs<C> regs;
-    load_tile(regs, at, kb_, a.ld, t * C::KT, len);
-    store_tile(smem, regs, tid);
-    load_tile(regs, at, vb_, a.ld, t * C::KT, len);
-    store_tile(smem + C::TILE, regs, tid);
-    __syncthreads();
+    const Ring ring(base + (a.H + h / (a.H / a.KV)) * HD, a.ld, a.KV * HD, len, wave, lane);
+    const TrAt<C> tr(lane);
+    auto tile = [&](int it) { return it < ns ? it : w0 + it - ns; };
+    int fill = 0, use = 0;               // ring positions
+    for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), smem + fill * Ring::STAGE);
+    fill = Ring::STAGES - 1;
     for (int it = 0; it < nt; ++it) {
-        const unsigned char *kl = smem + (it & 1) * 2 * C::TILE, *vl = kl + C::TILE;
-        unsigned char* next = smem + (~it & 1) * 2 * C::TILE;
-        const int k0 = t * C::KT, k1 = k0 + C::KT - 1;
-        const bool more = it + 1 < nt;
-        t = it + 1 < ns ? it + 1 : w0 + it + 1 - ns;
-        if (more) load_tile(regs, at, kb_, a.ld, t * C::KT, len);
-        const bool mine = !(q0 >= len || k0 > qlast + a.right || (k1 < q0 - a.left && k0 >= a.sinks));      // this wave sees some of the tile
+        tile_ready<(Ring::STAGES - 2) * C::NI>(it + Ring::STAGES - 1 > nt);
+        if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), smem + fill * Ring::STAGE);
+        fill = fill + 1 == Ring::STAGES ? 0 : fill + 1;
+        const unsigned char *kl = smem + use * Ring::STAGE, *vl = kl + C::TILE;
+        use = use + 1 == Ring::STAGES ? 0 : use + 1;
+        const int k0 = tile(it) * C::KT, k1 = k0 + C::KT - 1;
+        if (q0 >= len || k0 > qlast + a.right || (k1 < q0 - a.left && k0 >= a.sinks)) continue;      // this wave sees nothing of the tile
         f32x16_t s[C::KB];
-        if (mine) {
 #pragma unroll
-            for (int kb = 0; kb < C::KB; ++kb) {
-                s[kb] = splat16(0.f);
+        for (int kb = 0; kb < C::KB; ++kb) {
+            s[kb] = splat16(0.f);
 #pragma unroll
-                for (int j = 0; j < C::FR; ++j)
-                    s[kb] = mma_frag<T>(*reinterpret_cast<const uint4*>(kl + img_off<T, HD>(kb * 32 + r, 2 * j + h2)), qf[j], s[kb]);
-            }
+            for (int j = 0; j < C::FR; ++j) s[kb] = mma_frag<T>(row_frag<C>(kl, kb * 32 + r, 2 * j + h2), qf[j], s[kb]);
         }
-        if (more) {
-            store_tile(next, regs, tid);
-            load_tile(regs, at, vb_, a.ld, t * C::KT, len);
-        }
-        if (mine) {
-            if (!(k1 < len && k1 <= q0 + a.right && (k0 >= qlast - a.left || k1 < a.sinks))) {      // a border runs through the tile
-#pragma unroll
-                for (int kb = 0; kb < C::KB; ++kb)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int key = k0 + kb * 32 + acc_row(e, h2);
-                        if (key >= len || !visible(q, key, a.left, a.right, a.sinks)) s[kb][e] = -INFINITY;
-                    }
-            }
-            float mx = s[0][0];
-#pragma unroll
-            for (int kb = 0; kb < C::KB; ++kb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) mx = __builtin_elementwise_maximum(mx, s[kb][e]);
-            mx = pair_max(mx);
-            if (__builtin_amdgcn_ballot_w64((mx - m) * c > RESCALE_TH) != 0) {
-                const float mn = fmaxf(m, mx);
-                const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);       // a row that saw nothing yet: m = mn = -inf
-                m = mn;
-                l *= alpha;
-#pragma unroll
-                for (int db = 0; db < C::DB; ++db)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
-            }
-            const float mc = m == -INFINITY ? 0.f : m * c;
-            float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!(k1 < len && k1 <= q0 + a.right && (k0 >= qlast - a.left || k1 < a.sinks))) {      // a border runs through the tile
 #pragma unroll
             for (int kb = 0; kb < C::KB; ++kb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    s[kb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e], c, -mc));
-                    ls[e & 3] += s[kb][e];
+                    const int key = k0 + kb * 32 + acc_row(e, h2);
+                    if (key >= len || !visible(q, key, a.left, a.right, a.sinks)) s[kb][e] = -INFINITY;
                 }
-            l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-#pragma unroll
-            for (int kb = 0; kb < C::KB; ++kb)
-#pragma unroll
-                for (int db = 0; db < C::DB; ++db) o[db] = mma_tr<T, HD>(vl, kb * 32, db, s[kb], o[db], lane);
         }
-        if (more) store_tile(next + C::TILE, regs, tid);
-        __syncthreads();
+        float mx = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < C::KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = __builtin_elementwise_maximum(mx, s[kb][e]);
+        mx = pair_max(mx);
+        if (__builtin_amdgcn_ballot_w64((mx - m) * c > RESCALE_TH) != 0) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);       // a row that saw nothing yet: m = mn = -inf
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < C::KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[kb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e], c, -mc));
+                ls[e & 3] += s[kb][e];
+            }
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        mma_tr<C, 0>(vl, tr, s[0], o, lane);
+        if constexpr (C::KB == 2) mma_tr<C, 32>(vl, tr, s[1], o, lane);
     }
     if (q < len) {
         l = pair_sum(l);
@@ -337,8 +374,9 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_fw
 
 // dQ, the query on the lane; also delta = rowsum(dO * O), which the dK/dV kernels launched behind this one read
 template <typename T, int HD>
-__global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : DQ_OCC)) void window_dq_kernel(WArgs a) {
+__global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_dq_kernel(WArgs a) {
     using C = WCfg<T, HD>;
+    using Ring = KvRing<C>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int nrb = (a.L + WROWS - 1) / WROWS;
     const int work = xcd_remap(blockIdx.x, gridDim.x);
@@ -348,22 +386,19 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : DQ_OCC)) void wind
     if (rblk * WROWS >= len) return;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h2 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = a.H + h / (a.H / a.KV);
     const T* base = (const T*)a.qkv + start * a.ld;
-    const T *kb_ = base + hk * HD, *vb_ = kb_ + a.KV * HD;
     const int q0 = rblk * WROWS + wave * 32, q = q0 + r;
     const float c = a.scale * LOG2E;
 
-    uint4 qf[C::FR], gf[C::FR];
+    typename Frag<T>::V qf[C::FR] = {}, gf[C::FR] = {};
     float dl = 0.f, ls = 0.f;
 #pragma unroll
-    for (int j = 0; j < C::FR; ++j) {
-        qf[j] = gf[j] = make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < C::FR; ++j)
         if (q < len) {
             const int col = h * HD + (2 * j + h2) * (16 / C::ES);
             const int64_t ro = (start + q) * a.H * HD + col;
-            qf[j] = *reinterpret_cast<const uint4*>(base + (int64_t)q * a.ld + col);
-            gf[j] = *reinterpret_cast<const uint4*>((const T*)a.dout + ro);
+            qf[j] = *reinterpret_cast<const typename Frag<T>::V*>(base + (int64_t)q * a.ld + col);
+            gf[j] = *reinterpret_cast<const typename Frag<T>::V*>((const T*)a.dout + ro);
             float x[4], y[4];
 #pragma unroll
             for (int u = 0; u < 16 / C::ES; u += 4) {
@@ -373,12 +408,17 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : DQ_OCC)) void wind
                 for (int k = 0; k < 4; ++k) dl = __builtin_fmaf(x[k], y[k], dl);
             }
         }
-    }
     dl = pair_sum(dl);
     if (q < len) {
         ls = a.lse[(int64_t)h * a.R + start + q];
         if (h2 == 0) a.delta[(int64_t)h * a.R + start + q] = dl;
     }
+#pragma unroll
+    for (int j = 0; j < C::FR; ++j) {
+        pin(qf[j]);
+        pin(gf[j]);
+    }
+    asm volatile("" : "+v"(ls), "+v"(dl));
     f32x16_t dq[C::DB];
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) dq[db] = splat16(0.f);
@@ -386,41 +426,28 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : DQ_OCC)) void wind
     int ns, w0;
     const int nt = key_tiles<C::KT>(rblk * WROWS, min(rblk * WROWS + WROWS, len) - 1, len, a.left, a.right, a.sinks, ns, w0);
     const int qlast = min(q0 + 31, len - 1);
-    int t = ns > 0 ? 0 : w0;
-    const TileAt<C> at(a.ld, tid);
-    TileRegs<C> regs;
-    load_tile(regs, at, kb_, a.ld, t * C::KT, len);
-    store_tile(smem, regs, tid);
-    load_tile(regs, at, vb_, a.ld, t * C::KT, len);
-    store_tile(smem + C::TILE, regs, tid);
-    __syncthreads();
+    const Ring ring(base + (a.H + h / (a.H / a.KV)) * HD, a.ld, a.KV * HD, len, wave, lane);
+    const TrAt<C> tr(lane);
+    auto tile = [&](int it) { return it < ns ? it : w0 + it - ns; };
+    int fill = 0, use = 0;
+    for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), smem + fill * Ring::STAGE);
+    fill = Ring::STAGES - 1;
     for (int it = 0; it < nt; ++it) {
-        const unsigned char *kl = smem + (it & 1) * 2 * C::TILE, *vl = kl + C::TILE;
-        unsigned char* next = smem + (~it & 1) * 2 * C::TILE;
-        const int k0 = t * C::KT, k1 = k0 + C::KT - 1;
-        const bool more = it + 1 < nt;
-        t = it + 1 < ns ? it + 1 : w0 + it + 1 - ns;
-        const bool mine = !(q0 >= len || k0 > qlast + a.right || (k1 < q0 - a.left && k0 >= a.sinks));
+        tile_ready<(Ring::STAGES - 2) * C::NI>(it + Ring::STAGES - 1 > nt);
+        if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), smem + fill * Ring::STAGE);
+        fill = fill + 1 == Ring::STAGES ? 0 : fill + 1;
+        const unsigned char *kl = smem + use * Ring::STAGE, *vl = kl + C::TILE;
+        use = use + 1 == Ring::STAGES ? 0 : use + 1;
+        const int k0 = tile(it) * C::KT, k1 = k0 + C::KT - 1;
+        if (q0 >= len || k0 > qlast + a.right || (k1 < q0 - a.left && k0 >= a.sinks)) continue;
         const bool whole = k1 < len && k1 <= q0 + a.right && (k0 >= qlast - a.left || k1 < a.sinks);
-#pragma unroll
-        for (int kb = 0; kb < C::KB; ++kb) {
-            if (more) {                            // K while the first half is worked on, V while the last is
-                if (kb == 0) load_tile(regs, at, kb_, a.ld, t * C::KT, len);
-                if (kb == C::KB - 1) {
-                    if (C::KB > 1 || !mine) store_tile(next, regs, tid);
-                    if (C::KB > 1 || !mine) load_tile(regs, at, vb_, a.ld, t * C::KT, len);
-                }
-            }
-            if (!mine) continue;
+        auto half = [&](auto kb_) {
+            constexpr int kb = decltype(kb_)::value;
             f32x16_t s = splat16(0.f), dp = splat16(-dl);
 #pragma unroll
             for (int j = 0; j < C::FR; ++j) {
-                s = mma_frag<T>(*reinterpret_cast<const uint4*>(kl + img_off<T, HD>(kb * 32 + r, 2 * j + h2)), qf[j], s);
-                dp = mma_frag<T>(*reinterpret_cast<const uint4*>(vl + img_off<T, HD>(kb * 32 + r, 2 * j + h2)), gf[j], dp);
-            }
-            if (C::KB == 1 && more) {
-                store_tile(next, regs, tid);
-                load_tile(regs, at, vb_, a.ld, t * C::KT, len);
+                s = mma_frag<T>(row_frag<C>(kl, kb * 32 + r, 2 * j + h2), qf[j], s);
+                dp = mma_frag<T>(row_frag<C>(vl, kb * 32 + r, 2 * j + h2), gf[j], dp);
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -ls)) * dp[e];
@@ -431,50 +458,56 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : DQ_OCC)) void wind
                     if (key >= len || !visible(q, key, a.left, a.right, a.sinks)) s[e] = 0.f;
                 }
             }
-#pragma unroll
-            for (int db = 0; db < C::DB; ++db) dq[db] = mma_tr<T, HD>(kl, kb * 32, db, s, dq[db], lane);
-        }
-        if (more) store_tile(next + C::TILE, regs, tid);
-        __syncthreads();
+            mma_tr<C, kb * 32>(kl, tr, s, dq, lane);
+        };
+        half(std::integral_constant<int, 0>{});
+        if constexpr (C::KB == 2) half(std::integral_constant<int, 1>{});
     }
     if (q < len) store_rows<T, HD>(dq, a.scale, (T*)a.dqkv + (start + q) * (a.H + 2 * a.KV) * HD + h * HD, h2);
 }
 
-// P and dS of 32 queries (rows of the images ql and gl at qb) x 32 keys (kf, vf), and their products into dV and dK
-template <class C, typename T, int HD, class VIS>
-__device__ __forceinline__ void dkv_block(const unsigned char* ql, const unsigned char* gl, const float* lsl, const float* dll, int qb, const uint4 (&kf)[C::FR],
-                                          const uint4 (&vf)[C::FR], float c, bool whole, VIS vis, f32x16_t (&dk)[C::DB], f32x16_t (&dv)[C::DB], int lane) {
+// P and dS of 32 queries (rows BLK .. of the images ql and gl) x 32 keys (kf, vf), and their products into dV and dK
+template <class C, int BLK, class VIS>
+__device__ __forceinline__ void dkv_block(const unsigned char* ql, const unsigned char* gl, const float* lsl, const float* dll, const typename Frag<typename C::Type>::V (&kf)[C::FR],
+                                          const typename Frag<typename C::Type>::V (&vf)[C::FR], float c, bool whole, VIS vis, const TrAt<C>& tr, f32x16_t (&dk)[C::DB],
+                                          f32x16_t (&dv)[C::DB], int lane) {
+    using T = typename C::Type;
     const int r = lane & 31, h2 = lane >> 5;
     f32x16_t s = splat16(0.f), dp = splat16(0.f);
 #pragma unroll
     for (int j = 0; j < C::FR; ++j) {
-        s = mma_frag<T>(*reinterpret_cast<const uint4*>(ql + img_off<T, HD>(qb + r, 2 * j + h2)), kf[j], s);
-        dp = mma_frag<T>(*reinterpret_cast<const uint4*>(gl + img_off<T, HD>(qb + r, 2 * j + h2)), vf[j], dp);
+        s = mma_frag<T>(row_frag<C>(ql, BLK + r, 2 * j + h2), kf[j], s);
+        dp = mma_frag<T>(row_frag<C>(gl, BLK + r, 2 * j + h2), vf[j], dp);
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const int i = qb + acc_row(e, h2);
-        s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -lsl[i]));
-        dp[e] = s[e] * (dp[e] - dll[i]);
+    for (int t = 0; t < 4; ++t) {
+        const f32x4_t lt = *reinterpret_cast<const f32x4_t*>(lsl + BLK + 8 * t + 4 * h2), dt = *reinterpret_cast<const f32x4_t*>(dll + BLK + 8 * t + 4 * h2);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int e = 4 * t + u;
+            s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -lt[u]));
+            dp[e] = s[e] * (dp[e] - dt[u]);
+        }
     }
     if (!whole) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-            if (!vis(qb + acc_row(e, h2))) s[e] = dp[e] = 0.f;
+            if (!vis(BLK + acc_row(e, h2))) s[e] = dp[e] = 0.f;
     }
-#pragma unroll
-    for (int db = 0; db < C::DB; ++db) {
-        dv[db] = mma_tr<T, HD>(gl, qb, db, s, dv[db], lane);
-        dk[db] = mma_tr<T, HD>(ql, qb, db, dp, dk[db], lane);
-    }
+    mma_tr<C, BLK>(gl, tr, s, dv, lane);
+    mma_tr<C, BLK>(ql, tr, dp, dk, lane);
 }
 
 // dK and dV, the key on the lane: sweeps the queries that see the block's keys, for every query head of the group.  far_parts > 0: the
 // queries that see a sink from beyond the window were done by window_far_kernel, and the sums start from its own.
-template <typename T, int HD>
-__global__ __launch_bounds__(WT, (sizeof(T) * HD >= 256 ? DKV_OCC : 2)) void window_dkv_kernel(WArgs a) {
+template <typename T, int HD> struct DkvCfg {
     using C = WCfg<T, HD, (sizeof(T) == 2 && HD < 128) ? 64 : 32>;
-    constexpr int STAGE = 2 * C::TILE + 2 * C::KT * 4;
+    static constexpr int STAGE = 2 * C::TILE + 512, STAGES = STAGE > 20480 ? 2 : 3;      // Q image | dO image | 64 log-sum-exps | 64 row dots
+};
+template <typename T, int HD>
+__global__ __launch_bounds__(WT, (sizeof(T) * HD >= 256 ? 1 : 2)) void window_dkv_kernel(WArgs a) {
+    using C = typename DkvCfg<T, HD>::C;
+    constexpr int STAGE = DkvCfg<T, HD>::STAGE, STAGES = DkvCfg<T, HD>::STAGES;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int nrb = (a.L + WROWS - 1) / WROWS;
     const int work = xcd_remap(blockIdx.x, gridDim.x);
@@ -491,14 +524,17 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 256 ? DKV_OCC : 2)) void win
     const int sinks = a.far_parts ? 0 : a.sinks;
     const float c = a.scale * LOG2E;
 
-    uint4 kf[C::FR], vf[C::FR];
+    typename Frag<T>::V kf[C::FR] = {}, vf[C::FR] = {};
+#pragma unroll
+    for (int j = 0; j < C::FR; ++j)
+        if (key < len) {
+            kf[j] = *reinterpret_cast<const typename Frag<T>::V*>(kb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
+            vf[j] = *reinterpret_cast<const typename Frag<T>::V*>(vb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
+        }
 #pragma unroll
     for (int j = 0; j < C::FR; ++j) {
-        kf[j] = vf[j] = make_uint4(0, 0, 0, 0);
-        if (key < len) {
-            kf[j] = *reinterpret_cast<const uint4*>(kb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
-            vf[j] = *reinterpret_cast<const uint4*>(vb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
-        }
+        pin(kf[j]);
+        pin(vf[j]);
     }
     f32x16_t dk[C::DB], dv[C::DB];
 #pragma unroll
@@ -513,52 +549,56 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 256 ? DKV_OCC : 2)) void win
                 dv[db][e] = w[((C::DB + db) * 16 + e) * 64];
             }
     }
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db) asm volatile("" : "+v"(dk[db]), "+v"(dv[db]));
 
     // queries that see a key of the block: from the first key minus right to the last key plus left, to the end where there are sinks
     const int qlo = max(0, kb0 - a.right), qhi = kb0 < sinks ? len - 1 : min(len - 1, min(kb0 + WROWS, len) - 1 + a.left);
     const int t0 = qlo / C::KT, nt = qhi / C::KT - t0 + 1, total = nt * rep;
     const int64_t gld = (int64_t)a.H * HD;
-    const TileAt<C> qat(a.ld, tid), gat(gld, tid);
     const T* gb = (const T*)a.dout + start * gld;
-    const float* cb = (tid < C::KT ? a.lse : a.delta) + start;        // the row constants: a thread of the first two groups of KT fetches one
-    TileRegs<C> qr, gr;
-    float cr = 0.f;
-    int ft = 0, fh = hk * rep;            // the tile and head to fetch next
-    auto fetch = [&]() {
-        const int row0 = (t0 + ft) * C::KT;
-        load_tile(qr, qat, base + fh * HD, a.ld, row0, len);
-        load_tile(gr, gat, gb + fh * HD, gld, row0, len);
-        const int row = row0 + tid % C::KT;
-        cr = tid < 2 * C::KT && row < len ? cb[(int64_t)fh * a.R + row] : 0.f;
+    const float* cb = ((wave & 1) ? a.delta : a.lse) + start;
+    unsigned src[C::NI];
+#pragma unroll
+    for (int j = 0; j < C::NI; ++j) {       // the waves alternate between the two images: an instruction knows its descriptor
+        const int p = j * 4 + wave;
+        src[j] = piece_src<C>(p >= C::NP ? p - C::NP : p, lane, p >= C::NP ? gld : a.ld);
+    }
+    int ft = 0, fh = hk * rep;              // the tile and head to fetch next
+    auto issue = [&](unsigned char* stage) {
+        const int64_t row0 = (int64_t)(t0 + ft) * C::KT, left = len - 1 - row0;
+        const __amdgpu_buffer_rsrc_t rq = rows_rsrc(base + fh * HD + row0 * a.ld, (left * a.ld + HD) * C::ES);
+        const __amdgpu_buffer_rsrc_t rg = rows_rsrc(gb + fh * HD + row0 * gld, (left * gld + HD) * C::ES);
+#pragma unroll
+        for (int j = 0; j < C::NI; ++j) {
+            const int p = j * 4 + wave;
+            if (p >= C::NP) dma16(rg, stage + p * 1024, src[j]);
+            else dma16(rq, stage + p * 1024, src[j]);
+        }
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rows_rsrc(cb + (int64_t)fh * a.R + row0, (left + 1) * 4), (lds_ptr_t)(stage + 2 * C::TILE + (wave & 1) * 256), 4, lane * 4, 0, 0, 0);
         if (++ft == nt) {
             ft = 0;
             ++fh;
         }
     };
-    auto put = [&](unsigned char* st) {
-        store_tile(st, qr, tid);
-        store_tile(st + C::TILE, gr, tid);
-        if (tid < 2 * C::KT) reinterpret_cast<float*>(st + 2 * C::TILE)[tid] = cr;
-    };
-    fetch();
-    put(smem);
-    __syncthreads();
-    int ct = 0;
+    const TrAt<C> tr(lane);
+    int fill = 0, use = 0, ct = 0;
+    for (; fill < STAGES - 1 && fill < total; ++fill) issue(smem + fill * STAGE);
+    fill = STAGES - 1;
     for (int it = 0; it < total; ++it) {
-        const unsigned char *ql = smem + (it & 1) * STAGE, *gl = ql + C::TILE;
-        const float *lsl = reinterpret_cast<const float*>(gl + C::TILE), *dll = lsl + C::KT;
+        tile_ready<(STAGES - 2) * (C::NI + 1)>(it + STAGES - 1 > total);
+        if (it + STAGES - 1 < total) issue(smem + fill * STAGE);
+        fill = fill + 1 == STAGES ? 0 : fill + 1;
+        const unsigned char *ql = smem + use * STAGE, *gl = ql + C::TILE;
+        use = use + 1 == STAGES ? 0 : use + 1;
+        const float *lsl = reinterpret_cast<const float*>(gl + C::TILE), *dll = lsl + 64;
         const int q0 = (t0 + ct) * C::KT, q1 = q0 + C::KT - 1;
         ct = ct + 1 == nt ? 0 : ct + 1;
-        if (it + 1 < total) fetch();
-        if (!(k0 >= len || q1 < k0 - a.right || (q0 > klast + a.left && k0 >= sinks))) {
-            const bool whole = q1 < len && q0 >= klast - a.right && (q1 <= k0 + a.left || klast < sinks);
-#pragma unroll
-            for (int qb = 0; qb < C::KB; ++qb)
-                dkv_block<C, T, HD>(ql, gl, lsl, dll, qb * 32, kf, vf, c, whole,
-                                    [&](int i) { return q0 + i < len && visible(q0 + i, key, a.left, a.right, sinks); }, dk, dv, lane);
-        }
-        if (it + 1 < total) put(smem + (~it & 1) * STAGE);
-        __syncthreads();
+        if (k0 >= len || q1 < k0 - a.right || (q0 > klast + a.left && k0 >= sinks)) continue;
+        const bool whole = q1 < len && q0 >= klast - a.right && (q1 <= k0 + a.left || klast < sinks);
+        auto vis = [&](int i) { return q0 + i < len && visible(q0 + i, key, a.left, a.right, sinks); };
+        dkv_block<C, 0>(ql, gl, lsl, dll, kf, vf, c, whole, vis, tr, dk, dv, lane);
+        if constexpr (C::KB == 2) dkv_block<C, 32>(ql, gl, lsl, dll, kf, vf, c, whole, vis, tr, dk, dv, lane);
     }
     if (key < len) {
         T* row = (T*)a.dqkv + (start + key) * (a.H + 2 * a.KV) * HD + (a.H + hk) * HD;
@@ -588,15 +628,15 @@ __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
     const T* base = (const T*)a.qkv + start * a.ld;
     const T *kb_ = base + (a.H + hk) * HD, *vb_ = kb_ + a.KV * HD;
     const float c = a.scale * LOG2E;
-    uint4 kf[C::FR], vf[C::FR];
+    typedef typename Frag<T>::V V;
+    V kf[C::FR] = {}, vf[C::FR] = {};
 #pragma unroll
-    for (int j = 0; j < C::FR; ++j) {
-        kf[j] = vf[j] = make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < C::FR; ++j)
         if (key < kend) {
-            kf[j] = *reinterpret_cast<const uint4*>(kb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
-            vf[j] = *reinterpret_cast<const uint4*>(vb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
+            kf[j] = *reinterpret_cast<const V*>(kb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
+            vf[j] = *reinterpret_cast<const V*>(vb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
         }
-    }
+    const TrAt<C> tr(lane);
     f32x16_t dk[C::DB], dv[C::DB];
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) dk[db] = dv[db] = splat16(0.f);
@@ -608,28 +648,28 @@ __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
     for (int it = i0; it < i1; ++it) {
         const int h = hk * rep + it / nt, q0 = (t0 + it % nt) * 32;
         const T *qs = base + h * HD, *gs = (const T*)a.dout + start * a.H * HD + h * HD;
-        uint4 qr[NL], gr[NL];
+        V qr[NL], gr[NL];
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int id = lane + i * 64, row = q0 + id / C::CH, col = (id % C::CH) * (16 / C::ES);
-            qr[i] = gr[i] = make_uint4(0, 0, 0, 0);
+            qr[i] = gr[i] = V{};
             if (row < len) {
-                qr[i] = *reinterpret_cast<const uint4*>(qs + (int64_t)row * a.ld + col);
-                gr[i] = *reinterpret_cast<const uint4*>(gs + (int64_t)row * a.H * HD + col);
+                qr[i] = *reinterpret_cast<const V*>(qs + (int64_t)row * a.ld + col);
+                gr[i] = *reinterpret_cast<const V*>(gs + (int64_t)row * a.H * HD + col);
             }
         }
         const float cr = q0 + r < len ? (h2 ? a.delta : a.lse)[(int64_t)h * a.R + start + q0 + r] : 0.f;
         wave_sync();                                        // the previous tile's reads are done
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int id = lane + i * 64, at = img_off<T, HD>(id / C::CH, id % C::CH);
-            *reinterpret_cast<uint4*>(ql + at) = qr[i];
-            *reinterpret_cast<uint4*>(gl + at) = gr[i];
+            const int id = lane + i * 64, at = C::at(id / C::CH, id % C::CH);
+            *reinterpret_cast<V*>(ql + at) = qr[i];
+            *reinterpret_cast<V*>(gl + at) = gr[i];
         }
         lsl[lane] = cr;
         wave_sync();
-        dkv_block<C, T, HD>(ql, gl, lsl, dll, 0, kf, vf, c, q0 > lim && q0 + 31 < len && kend >= k0 + 32,
-                            [&](int i) { return q0 + i < len && key < kend && q0 + i > key + a.left; }, dk, dv, lane);
+        dkv_block<C, 0>(ql, gl, lsl, dll, kf, vf, c, q0 > lim && q0 + 31 < len && kend >= k0 + 32,
+                            [&](int i) { return q0 + i < len && key < kend && q0 + i > key + a.left; }, tr, dk, dv, lane);
     }
     float* w = a.far_ws + (((int64_t)(b * a.KV + hk) * a.far_groups + grp) * a.far_parts + part) * (2 * C::DB * 1024) + lane;
 #pragma unroll
@@ -670,20 +710,19 @@ template <void (*KERNEL)(WArgs)> static int launch(const char* who, int64_t bloc
     return 0;
 }
 template <typename T, int HD> static int run_fwd(const WArgs& a, hipStream_t s) {
-    return launch<window_fwd_kernel<T, HD>>("star_attn_window_fwd", (int64_t)cdiv(a.L, WROWS) * a.H * a.NB, 4 * WCfg<T, HD>::TILE, a, s);
+    return launch<window_fwd_kernel<T, HD>>("star_attn_window_fwd", (int64_t)cdiv(a.L, WROWS) * a.H * a.NB, KvRing<WCfg<T, HD>>::STAGES * KvRing<WCfg<T, HD>>::STAGE, a, s);
 }
 template <typename T, int HD> static int run_bwd(const WArgs& a, hipStream_t s) {
     const char* who = "star_attn_window_bwd";
     const int64_t nrb = cdiv(a.L, WROWS);
-    if (int rc = launch<window_dq_kernel<T, HD>>(who, nrb * a.H * a.NB, 4 * WCfg<T, HD>::TILE, a, s)) return rc;
+    if (int rc = launch<window_dq_kernel<T, HD>>(who, nrb * a.H * a.NB, KvRing<WCfg<T, HD>>::STAGES * KvRing<WCfg<T, HD>>::STAGE, a, s)) return rc;
     if (a.far_parts) {
         const int lists = a.NB * a.KV * a.far_groups, size = 2 * WCfg<T, HD>::DB * 1024;
         if (int rc = launch<window_far_kernel<T, HD>>(who, (int64_t)lists * (a.far_parts / 4), 4 * (2 * WCfg<T, HD, 32>::TILE + 256), a, s)) return rc;
         hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, lists), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
         STAR_LAUNCH_CHECK(who);
     }
-    using C = WCfg<T, HD, (sizeof(T) == 2 && HD < 128) ? 64 : 32>;
-    return launch<window_dkv_kernel<T, HD>>(who, nrb * a.KV * a.NB, 2 * (2 * C::TILE + 2 * C::KT * 4), a, s);
+    return launch<window_dkv_kernel<T, HD>>(who, nrb * a.KV * a.NB, DkvCfg<T, HD>::STAGES * DkvCfg<T, HD>::STAGE, a, s);
 }
 
 // How the far queries of the sinks are cut: about eight waves per compute unit in all, no more than 64 parts to add up, and at least two
