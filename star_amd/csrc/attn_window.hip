@@ -25,6 +25,12 @@ typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 
 #define WT 256                    // threads of a block: four waves of 32 queries (backward of K and V: 32 keys)
 #define WROWS 128
+// Waves that the registers of a kernel have to leave room for on a SIMD, by row bytes (measured: of 2, 3 and 4 the fastest each): a tighter
+// budget makes the compiler give up the distance between its LDS reads and the products that use them.
+#define WAVES_FWD(B) ((B) >= 512 ? 1 : (B) >= 256 ? 2 : 4)
+#define WAVES_DQ(B) ((B) >= 512 ? 1 : (B) >= 256 ? 2 : (B) >= 128 ? 3 : 4)
+#define WAVES_DKV(B) ((B) >= 512 ? 1 : (B) >= 128 ? 2 : 3)
+#define WAVES_PER_SIMD(N) __attribute__((amdgpu_waves_per_eu(N, N)))
 #define LOG2E 1.4426950408889634f
 #define RESCALE_TH 8.0f           // log2 units: the reference maximum is raised only when a row exceeds it by 2^8 (float32 sums: no loss)
 
@@ -44,13 +50,14 @@ template <typename T, int HD, int ROWS = sizeof(T) == 2 ? 64 : 32> struct WCfg {
     static constexpr int NI = 2 * NP / 4;                   // pieces that each of the four waves brings per pair of images
     // The 16-byte chunks of a row are permuted by the row's number, so that neither 16 lanes reading one chunk of 16 successive rows nor
     // 32 lanes of a transposing read (4 rows x 4 chunks) hit one of the 64 banks twice.
-    static __device__ __forceinline__ int swizzle(int row) {
+    // (A bit permutation of the row: swizzle(a ^ b) = swizzle(a) ^ swizzle(b).)
+    static constexpr __device__ __forceinline__ int swizzle(int row) {
         if constexpr (CH == 2) return (row >> 3) & 1;
         else if constexpr (CH == 4) return (row >> 2) & 3;
         else if constexpr (CH == 8) return ES == 2 ? ((row >> 1 & 1) << 2) | (row >> 2 & 3) : (row >> 1) & 7;
         else return ES == 2 ? ((row & 3) << 2) | (row >> 2 & 3) : row & 15;
     }
-    static __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swizzle(row)) << 4); }
+    static constexpr __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swizzle(row)) << 4); }
 };
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
@@ -75,12 +82,24 @@ template <int N> __device__ __forceinline__ void tile_ready(bool last) {
     asm volatile("" ::: "memory");
 }
 
-// 16 bytes of a row.  (A compiler-visible read through another type, uint4 or a builtin, would be given a wait for every LDS-DMA in flight.)
+// 16 bytes of a row.  (Through a vector type: a read of uint4 would be given a wait for every LDS-DMA in flight.)
 template <typename T> struct Frag { typedef short8_t V; };
 template <> struct Frag<float> { typedef f32x4_t V; };
-template <class C> __device__ __forceinline__ typename Frag<typename C::Type>::V row_frag(const unsigned char* lds, int row, int chunk) {
-    return *reinterpret_cast<const typename Frag<typename C::Type>::V*>(lds + C::at(row, chunk));
-}
+// LDS is addressed by 32-bit offsets.  Images start at multiples of 512 bytes, so the chunk of an address can be changed by an XOR: KEEP = false
+// holds one offset per access pattern and forms the others by XORs, which the dK/dV kernel of 128-wide heads needs to fit two waves on a
+// SIMD (694 against 891 us at 2 x 8192 rows, 16 heads, window 2048); KEEP = true holds them all (dQ kernel, 64-wide heads: 77 against 88 us).
+template <typename V> __device__ __forceinline__ V lds_read(unsigned addr) { return *reinterpret_cast<const __attribute__((address_space(3))) V*>(addr); }
+// fragments of row (lane & 31) of an image
+template <class C, bool KEEP> struct RowAt {
+    unsigned off[KEEP ? C::FR : 1];
+    __device__ __forceinline__ RowAt(int lane) {
+#pragma unroll
+        for (int j = 0; j < (KEEP ? C::FR : 1); ++j) off[j] = C::at(lane & 31, 2 * j + (lane >> 5));
+    }
+    template <int BLK> __device__ __forceinline__ typename Frag<typename C::Type>::V read(unsigned img, int j) const {
+        return lds_read<typename Frag<typename C::Type>::V>((KEEP ? img + off[KEEP ? j : 0] : (img + off[0]) ^ (unsigned)(j << 5)) + BLK * C::RB);
+    }
+};
 // a global load consumed here: the compiler then has no wait of its own to put into the loop
 template <typename V> __device__ __forceinline__ void pin(V& v) {
     i32x4_t t = __builtin_bit_cast(i32x4_t, v);
@@ -100,37 +119,37 @@ template <typename T> __device__ __forceinline__ f32x16_t mma_frag(typename Frag
 }
 
 // Products with a transposed image: acc[db] += A_db B for rows blk .. blk+31 of the image, A_db = its columns 32 db .. 32 db + 31 as MFMA rows, B
-// = the 32 x 32 accumulator block s as it lies (its rows are the image's rows).
-// bf16: transposing LDS reads, in the row order in which an accumulator holds its registers.  They are issued in assembly, because the compiler
-// puts a wait for every LDS-DMA in flight before its own, and waited for in the same block.  float32: register e of the two lane halves is one
+// = the 32 x 32 accumulator block p as it lies (its rows are the image's rows).
+// bf16: transposing LDS reads, in the row order in which an accumulator holds its registers.  (The compiler puts a wait for every LDS-DMA in
+// flight before the first of them; the next tile's was issued a whole score product earlier.)  float32: register e of the two lane halves is one
 // product step, its operand an ordinary read.
-template <class C> struct TrAt {
-    unsigned lo[C::DB], hi[C::DB];          // bf16: byte offsets of rows (0 | 8) + 4 h2 + i / 4 in the image
+template <class C, bool KEEP_> struct TrAt {
+    static constexpr bool KEEP = KEEP_ && C::ES == 2;
+    unsigned lo_[KEEP ? C::DB : 1], hi_[KEEP ? C::DB : 1];            // bf16: byte offsets of rows (0 | 8) + 4 h2 + i / 4, first 32 columns; float32 (lo_): row 4 h2, column lane & 31
     __device__ __forceinline__ TrAt(int lane) {
-        const int g = lane >> 4, i = lane & 15;
+        if constexpr (C::ES == 2) {
+            const int g = lane >> 4, i = lane & 15, row = 4 * (g >> 1) + (i >> 2);
 #pragma unroll
-        for (int db = 0; db < C::DB; ++db) {
-            const int col = db * 64 + (C::HDIM >= 32 ? (g & 1) * 32 : 0) + (i & 3) * 8, row = 4 * (g >> 1) + (i >> 2);
-            lo[db] = C::at(row, col >> 4) + (col & 15);
-            hi[db] = C::at(row + 8, col >> 4) + (col & 15);
+            for (int db = 0; db < (KEEP ? C::DB : 1); ++db) {
+                const int col = db * 64 + (C::HDIM >= 32 ? (g & 1) * 32 : 0) + (i & 3) * 8;
+                lo_[db] = C::at(row, col >> 4) + (col & 15);
+                hi_[db] = C::at(row + 8, col >> 4) + (col & 15);
+            }
+        } else {
+            const int d = C::HDIM >= 32 ? (lane & 31) : (lane & 15);
+            lo_[0] = hi_[0] = C::at(4 * (lane >> 5), d >> 2) + (d & 3) * 4;
         }
     }
+    __device__ __forceinline__ unsigned lo(unsigned img, int db) const { return KEEP ? img + lo_[KEEP ? db : 0] : (img + lo_[0]) ^ (unsigned)(db << 6); }
+    __device__ __forceinline__ unsigned hi(unsigned img, int db) const { return KEEP ? img + hi_[KEEP ? db : 0] : (img + hi_[0]) ^ (unsigned)(db << 6); }
 };
+__device__ __forceinline__ short4_t tr1(unsigned a) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) short4_t*>(a)); }
 template <int OFF, int STEP> __device__ __forceinline__ void tr_read(unsigned lo, unsigned hi, short4_t (&r)[4]) {
-    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %5 offset:%6\n\t"
-                 "ds_read_b64_tr_b16 %2, %4 offset:%7\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
-                 : "v"(lo), "v"(hi), "n"(OFF), "n"(OFF + STEP)
-                 : "memory");
+    r[0] = tr1(lo + OFF); r[1] = tr1(hi + OFF); r[2] = tr1(lo + OFF + STEP); r[3] = tr1(hi + OFF + STEP);
 }
 template <int OFF, int STEP> __device__ __forceinline__ void tr_read2(unsigned lo, unsigned hi, unsigned lo2, unsigned hi2, short4_t (&r)[4], short4_t (&s)[4]) {
-    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
-                 "ds_read_b64_tr_b16 %2, %8 offset:%13\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %11 offset:%12\n\t"
-                 "ds_read_b64_tr_b16 %6, %10 offset:%13\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
-                 : "v"(lo), "v"(hi), "v"(lo2), "v"(hi2), "n"(OFF), "n"(OFF + STEP)
-                 : "memory");
+    tr_read<OFF, STEP>(lo, hi, r);
+    tr_read<OFF, STEP>(lo2, hi2, s);
 }
 __device__ __forceinline__ f32x16_t mma_tr16(const short4_t (&r)[4], bf16x8_t p0, bf16x8_t p1, f32x16_t acc) {
     const short8_t a = {r[0][0], r[0][1], r[0][2], r[0][3], r[1][0], r[1][1], r[1][2], r[1][3]};
@@ -138,39 +157,68 @@ __device__ __forceinline__ f32x16_t mma_tr16(const short4_t (&r)[4], bf16x8_t p0
     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), p0, acc, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, b), p1, acc, 0, 0, 0);
 }
-template <class C, int BLK> __device__ __forceinline__ void mma_tr(const unsigned char* img, const TrAt<C>& at, const f32x16_t& s, f32x16_t (&acc)[C::DB], int lane) {
-    if constexpr (C::ES == 2) {
-        const unsigned base = lds_u32(img);
-        bf16x8_t p0, p1;
+// an accumulator block as the B operand, rounded to the row type
+template <typename T> struct Block {
+    bf16x8_t lo, hi;
+    __device__ __forceinline__ Block(const f32x16_t& s) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            p0[j] = (__bf16)s[j];
-            p1[j] = (__bf16)s[8 + j];
+            lo[j] = (__bf16)s[j];
+            hi[j] = (__bf16)s[8 + j];
         }
+    }
+};
+template <> struct Block<float> {
+    f32x16_t v;
+    __device__ __forceinline__ Block(const f32x16_t& s) : v(s) {}
+};
+template <class C, int BLK, class TR> __device__ __forceinline__ void mma_tr(unsigned img, const TR& at, const Block<typename C::Type>& p, f32x16_t (&acc)[C::DB]) {
+    if constexpr (C::ES == 2) {
+        const bf16x8_t p0 = p.lo, p1 = p.hi;
         short4_t r[4], t[4];
         if constexpr (C::DB == 1) {
-            tr_read<BLK * C::RB, 16 * C::RB>(base + at.lo[0], base + at.hi[0], r);
+            tr_read<BLK * C::RB, 16 * C::RB>(at.lo(img, 0), at.hi(img, 0), r);
             acc[0] = mma_tr16(r, p0, p1, acc[0]);
         } else {
 #pragma unroll
             for (int db = 0; db < C::DB; db += 2) {
-                tr_read2<BLK * C::RB, 16 * C::RB>(base + at.lo[db], base + at.hi[db], base + at.lo[db + 1], base + at.hi[db + 1], r, t);
+                tr_read2<BLK * C::RB, 16 * C::RB>(at.lo(img, db), at.hi(img, db), at.lo(img, db + 1), at.hi(img, db + 1), r, t);
                 acc[db] = mma_tr16(r, p0, p1, acc[db]);
                 acc[db + 1] = mma_tr16(t, p0, p1, acc[db + 1]);
             }
         }
     } else {
-        const int h2 = lane >> 5;
 #pragma unroll
-        for (int db = 0; db < C::DB; ++db) {
-            const int d = db * 32 + (C::HDIM >= 32 ? (lane & 31) : (lane & 15));
+        for (int db = 0; db < C::DB; ++db)
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(
-                    *reinterpret_cast<const float*>(img + C::at(BLK + (e & 3) + 8 * (e >> 2) + 4 * h2, d >> 2) + (d & 3) * 4), s[e], acc[db], 0, 0, 0);
-        }
+            for (int e = 0; e < 16; ++e) {
+                const int row = (e & 3) + 8 * (e >> 2);
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(lds_read<float>((at.lo(img, 0) ^ (unsigned)((C::swizzle(row) ^ (db * 8)) << 4)) + (BLK + row) * C::RB), p.v[e], acc[db], 0, 0, 0);
+            }
     }
 }
+
+// Order of N fragment reads and their N products: six reads first, then one for every product (left alone the compiler keeps two or
+// three in flight; 128-wide heads 549 -> 522 us at 8192 rows, 32 heads, window 4096).
+template <int N> __device__ __forceinline__ void reads_ahead() {
+    constexpr int AHEAD = N < 6 ? N : 6;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int j = 0; j < N - AHEAD; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, AHEAD, 0);
+}
+
+// Masks of a 32-row accumulator block as one bit per row: rows first .. last are in, and the rows in front of `sinks`, if not behind last.  A
+// register takes two instructions then (bit field extract, bit field insert) instead of three comparisons and a select.
+__device__ __forceinline__ unsigned bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+__device__ __forceinline__ unsigned block_mask(int first, int last, int sinks, int h2) {
+    return (bits_below(last + 1) & (~bits_below(first) | bits_below(sinks))) >> (4 * h2);
+}
+__device__ __forceinline__ unsigned row_in(unsigned mask, int e) { return (unsigned)((int)(mask << (31 - ((e & 3) + 8 * (e >> 2)))) >> 31); }      // all ones, or zero
+__device__ __forceinline__ float keep_or(unsigned in, float v, unsigned other) { return __uint_as_float((in & __float_as_uint(v)) | (~in & other)); }
 
 // row index of accumulator register e on lane half h2
 __device__ __forceinline__ int acc_row(int e, int h2) { return (e & 3) + 8 * (e >> 2) + 4 * h2; }
@@ -221,7 +269,7 @@ struct WArgs {
     float* lse;
     const void* dout;
     void* dqkv;
-    float* delta;            // [H, R] row dots
+    float* ndelta;           // [H, R] negated row dots
     float* far_ws;           // [NB, KV, far_groups, far_parts] partial sums of 32 sink keys
     int64_t ld, R;
     int NB, L, H, KV, left, right, sinks;
@@ -243,8 +291,6 @@ __device__ __forceinline__ int seq_rows(const WArgs& a, int b, int64_t& start) {
     return (int)(e - s > a.L ? a.L : e - s);
 }
 
-__device__ __forceinline__ bool visible(int i, int j, int left, int right, int sinks) { return j <= i + right && (j >= i - left || j < sinks); }
-
 // the key tiles that queries [q0, q1] see: `ns` leading tiles (sinks in front of the window), then tiles w0 .. w0 + count - ns - 1
 template <int KT> __device__ __forceinline__ int key_tiles(int q0, int q1, int len, int left, int right, int sinks, int& ns, int& w0) {
     const int lo = max(0, q0 - left), hi = min(len - 1, q1 + right);
@@ -255,7 +301,7 @@ template <int KT> __device__ __forceinline__ int key_tiles(int q0, int q1, int l
 
 // A ring of STAGES (K image | V image) stages: while one tile is worked on the next STAGES - 1 are on their way, without registers.
 template <class C> struct KvRing {
-    static constexpr int STAGE = 2 * C::TILE, STAGES = STAGE > 16384 ? 2 : 3;
+    static constexpr int STAGE = 2 * C::TILE, STAGES = STAGE > 8192 ? 2 : 3;
     const typename C::Type* k;              // key 0 of the head; its value lies v columns further on
     int64_t ld;
     int v, len, wave;
@@ -276,7 +322,7 @@ template <class C> struct KvRing {
 };
 
 template <typename T, int HD>
-__global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_fwd_kernel(WArgs a) {
+__global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_FWD(sizeof(T) * HD)) void window_fwd_kernel(WArgs a) {
     using C = WCfg<T, HD>;
     using Ring = KvRing<C>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -307,7 +353,9 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_fw
     const int nt = key_tiles<C::KT>(rblk * WROWS, min(rblk * WROWS + WROWS, len) - 1, len, a.left, a.right, a.sinks, ns, w0);
     const int qlast = min(q0 + 31, len - 1);
     const Ring ring(base + (a.H + h / (a.H / a.KV)) * HD, a.ld, a.KV * HD, len, wave, lane);
-    const TrAt<C> tr(lane);
+    const TrAt<C, (C::RB < 256)> tr(lane);
+    const RowAt<C, (C::RB < 256)> row(lane);
+    const unsigned lds = lds_u32(smem);
     auto tile = [&](int it) { return it < ns ? it : w0 + it - ns; };
     int fill = 0, use = 0;               // ring positions
     for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), smem + fill * Ring::STAGE);
@@ -316,7 +364,7 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_fw
         tile_ready<(Ring::STAGES - 2) * C::NI>(it + Ring::STAGES - 1 > nt);
         if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), smem + fill * Ring::STAGE);
         fill = fill + 1 == Ring::STAGES ? 0 : fill + 1;
-        const unsigned char *kl = smem + use * Ring::STAGE, *vl = kl + C::TILE;
+        const unsigned kl = lds + use * Ring::STAGE, vl = kl + C::TILE;
         use = use + 1 == Ring::STAGES ? 0 : use + 1;
         const int k0 = tile(it) * C::KT, k1 = k0 + C::KT - 1;
         if (q0 >= len || k0 > qlast + a.right || (k1 < q0 - a.left && k0 >= a.sinks)) continue;      // this wave sees nothing of the tile
@@ -325,16 +373,17 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_fw
         for (int kb = 0; kb < C::KB; ++kb) {
             s[kb] = splat16(0.f);
 #pragma unroll
-            for (int j = 0; j < C::FR; ++j) s[kb] = mma_frag<T>(row_frag<C>(kl, kb * 32 + r, 2 * j + h2), qf[j], s[kb]);
+            for (int j = 0; j < C::FR; ++j) s[kb] = mma_frag<T>(kb ? row.template read<32>(kl, j) : row.template read<0>(kl, j), qf[j], s[kb]);
         }
+        if constexpr (C::ES == 2) reads_ahead<C::KB * C::FR>();
         if (!(k1 < len && k1 <= q0 + a.right && (k0 >= qlast - a.left || k1 < a.sinks))) {      // a border runs through the tile
 #pragma unroll
-            for (int kb = 0; kb < C::KB; ++kb)
+            for (int kb = 0; kb < C::KB; ++kb) {
+                const int kk = k0 + kb * 32;
+                const unsigned in = block_mask(q - a.left - kk, min(q + a.right, len - 1) - kk, a.sinks - kk, h2);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = k0 + kb * 32 + acc_row(e, h2);
-                    if (key >= len || !visible(q, key, a.left, a.right, a.sinks)) s[kb][e] = -INFINITY;
-                }
+                for (int e = 0; e < 16; ++e) s[kb][e] = keep_or(row_in(in, e), s[kb][e], 0xff800000u);
+            }
         }
         float mx = s[0][0];
 #pragma unroll
@@ -353,17 +402,19 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_fw
                 for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
         }
         const float mc = m == -INFINITY ? 0.f : m * c;
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kb = 0; kb < C::KB; ++kb)
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};       // of the unrounded weights: the log-sum-exp that the backward pass reads is a float32 one
+        auto half = [&](auto kb_) {
+            constexpr int kb = decltype(kb_)::value;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 s[kb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e], c, -mc));
                 ls[e & 3] += s[kb][e];
             }
+            mma_tr<C, kb * 32>(vl, tr, Block<T>(s[kb]), o);
+        };
+        half(std::integral_constant<int, 0>{});
+        if constexpr (C::KB == 2) half(std::integral_constant<int, 1>{});
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-        mma_tr<C, 0>(vl, tr, s[0], o, lane);
-        if constexpr (C::KB == 2) mma_tr<C, 32>(vl, tr, s[1], o, lane);
     }
     if (q < len) {
         l = pair_sum(l);
@@ -372,9 +423,9 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_fw
     }
 }
 
-// dQ, the query on the lane; also delta = rowsum(dO * O), which the dK/dV kernels launched behind this one read
+// dQ, the query on the lane; also -delta = -rowsum(dO * O), which the dK/dV kernels launched behind this one read
 template <typename T, int HD>
-__global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_dq_kernel(WArgs a) {
+__global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DQ(sizeof(T) * HD)) void window_dq_kernel(WArgs a) {
     using C = WCfg<T, HD>;
     using Ring = KvRing<C>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -411,7 +462,7 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_dq
     dl = pair_sum(dl);
     if (q < len) {
         ls = a.lse[(int64_t)h * a.R + start + q];
-        if (h2 == 0) a.delta[(int64_t)h * a.R + start + q] = dl;
+        if (h2 == 0) a.ndelta[(int64_t)h * a.R + start + q] = -dl;
     }
 #pragma unroll
     for (int j = 0; j < C::FR; ++j) {
@@ -427,7 +478,9 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_dq
     const int nt = key_tiles<C::KT>(rblk * WROWS, min(rblk * WROWS + WROWS, len) - 1, len, a.left, a.right, a.sinks, ns, w0);
     const int qlast = min(q0 + 31, len - 1);
     const Ring ring(base + (a.H + h / (a.H / a.KV)) * HD, a.ld, a.KV * HD, len, wave, lane);
-    const TrAt<C> tr(lane);
+    const TrAt<C, (C::RB < 256)> tr(lane);
+    const RowAt<C, (C::RB < 256)> row(lane);
+    const unsigned lds = lds_u32(smem);
     auto tile = [&](int it) { return it < ns ? it : w0 + it - ns; };
     int fill = 0, use = 0;
     for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), smem + fill * Ring::STAGE);
@@ -436,7 +489,7 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_dq
         tile_ready<(Ring::STAGES - 2) * C::NI>(it + Ring::STAGES - 1 > nt);
         if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), smem + fill * Ring::STAGE);
         fill = fill + 1 == Ring::STAGES ? 0 : fill + 1;
-        const unsigned char *kl = smem + use * Ring::STAGE, *vl = kl + C::TILE;
+        const unsigned kl = lds + use * Ring::STAGE, vl = kl + C::TILE;
         use = use + 1 == Ring::STAGES ? 0 : use + 1;
         const int k0 = tile(it) * C::KT, k1 = k0 + C::KT - 1;
         if (q0 >= len || k0 > qlast + a.right || (k1 < q0 - a.left && k0 >= a.sinks)) continue;
@@ -446,19 +499,18 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_dq
             f32x16_t s = splat16(0.f), dp = splat16(-dl);
 #pragma unroll
             for (int j = 0; j < C::FR; ++j) {
-                s = mma_frag<T>(row_frag<C>(kl, kb * 32 + r, 2 * j + h2), qf[j], s);
-                dp = mma_frag<T>(row_frag<C>(vl, kb * 32 + r, 2 * j + h2), gf[j], dp);
+                s = mma_frag<T>(row.template read<kb * 32>(kl, j), qf[j], s);
+                dp = mma_frag<T>(row.template read<kb * 32>(vl, j), gf[j], dp);
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -ls)) * dp[e];
             if (!whole) {
+                const int kk = k0 + kb * 32;
+                const unsigned in = block_mask(q - a.left - kk, min(q + a.right, len - 1) - kk, a.sinks - kk, h2);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = k0 + kb * 32 + acc_row(e, h2);
-                    if (key >= len || !visible(q, key, a.left, a.right, a.sinks)) s[e] = 0.f;
-                }
+                for (int e = 0; e < 16; ++e) s[e] = keep_or(row_in(in, e), s[e], 0u);
             }
-            mma_tr<C, kb * 32>(kl, tr, s, dq, lane);
+            mma_tr<C, kb * 32>(kl, tr, Block<T>(s), dq);
         };
         half(std::integral_constant<int, 0>{});
         if constexpr (C::KB == 2) half(std::integral_constant<int, 1>{});
@@ -466,36 +518,47 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 512 ? 1 : 2)) void window_dq
     if (q < len) store_rows<T, HD>(dq, a.scale, (T*)a.dqkv + (start + q) * (a.H + 2 * a.KV) * HD + h * HD, h2);
 }
 
-// P and dS of 32 queries (rows BLK .. of the images ql and gl) x 32 keys (kf, vf), and their products into dV and dK
-template <class C, int BLK, class VIS>
-__device__ __forceinline__ void dkv_block(const unsigned char* ql, const unsigned char* gl, const float* lsl, const float* dll, const typename Frag<typename C::Type>::V (&kf)[C::FR],
-                                          const typename Frag<typename C::Type>::V (&vf)[C::FR], float c, bool whole, VIS vis, const TrAt<C>& tr, f32x16_t (&dk)[C::DB],
-                                          f32x16_t (&dv)[C::DB], int lane) {
+// P and dS of 32 queries (rows BLK .. of the images at ql and gl, their log-sum-exps and negated row dots at cst and cst + 256) x 32 keys (kf,
+// vf), and their products into dV and dK.  The dP accumulator starts from -delta.  Not `whole`: the lane's key is seen by the image's
+// rows first .. last alone.
+template <class C, int BLK, class ROW, class TR>
+__device__ __forceinline__ void dkv_block(unsigned ql, unsigned gl, unsigned cst, const ROW& row, const typename Frag<typename C::Type>::V (&kf)[C::FR],
+                                          const typename Frag<typename C::Type>::V (&vf)[C::FR], float c, bool whole, int first, int last, const TR& tr, f32x16_t (&dk)[C::DB],
+                                          f32x16_t (&dv)[C::DB], int h2) {
     using T = typename C::Type;
-    const int r = lane & 31, h2 = lane >> 5;
-    f32x16_t s = splat16(0.f), dp = splat16(0.f);
+    f32x16_t s = splat16(0.f), dp;
+    cst += BLK * 4 + 16 * h2;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const f32x4_t d = lds_read<f32x4_t>(cst + 256 + 32 * t);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) dp[4 * t + u] = d[u];
+    }
 #pragma unroll
     for (int j = 0; j < C::FR; ++j) {
-        s = mma_frag<T>(row_frag<C>(ql, BLK + r, 2 * j + h2), kf[j], s);
-        dp = mma_frag<T>(row_frag<C>(gl, BLK + r, 2 * j + h2), vf[j], dp);
+        s = mma_frag<T>(row.template read<BLK>(ql, j), kf[j], s);
+        dp = mma_frag<T>(row.template read<BLK>(gl, j), vf[j], dp);
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        const f32x4_t lt = *reinterpret_cast<const f32x4_t*>(lsl + BLK + 8 * t + 4 * h2), dt = *reinterpret_cast<const f32x4_t*>(dll + BLK + 8 * t + 4 * h2);
+        const f32x4_t lt = lds_read<f32x4_t>(cst + 32 * t);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int e = 4 * t + u;
             s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -lt[u]));
-            dp[e] = s[e] * (dp[e] - dt[u]);
+            dp[e] *= s[e];
         }
     }
     if (!whole) {
+        const unsigned in = block_mask(first - BLK, last - BLK, 0, h2);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            if (!vis(BLK + acc_row(e, h2))) s[e] = dp[e] = 0.f;
+        for (int e = 0; e < 16; ++e) {
+            s[e] = keep_or(row_in(in, e), s[e], 0u);
+            dp[e] = keep_or(row_in(in, e), dp[e], 0u);
+        }
     }
-    mma_tr<C, BLK>(gl, tr, s, dv, lane);
-    mma_tr<C, BLK>(ql, tr, dp, dk, lane);
+    mma_tr<C, BLK>(gl, tr, Block<T>(s), dv);
+    mma_tr<C, BLK>(ql, tr, Block<T>(dp), dk);
 }
 
 // dK and dV, the key on the lane: sweeps the queries that see the block's keys, for every query head of the group.  far_parts > 0: the
@@ -505,7 +568,7 @@ template <typename T, int HD> struct DkvCfg {
     static constexpr int STAGE = 2 * C::TILE + 512, STAGES = STAGE > 20480 ? 2 : 3;      // Q image | dO image | 64 log-sum-exps | 64 row dots
 };
 template <typename T, int HD>
-__global__ __launch_bounds__(WT, (sizeof(T) * HD >= 256 ? 1 : 2)) void window_dkv_kernel(WArgs a) {
+__global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DKV(sizeof(T) * HD)) void window_dkv_kernel(WArgs a) {
     using C = typename DkvCfg<T, HD>::C;
     constexpr int STAGE = DkvCfg<T, HD>::STAGE, STAGES = DkvCfg<T, HD>::STAGES;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -557,7 +620,7 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 256 ? 1 : 2)) void window_dk
     const int t0 = qlo / C::KT, nt = qhi / C::KT - t0 + 1, total = nt * rep;
     const int64_t gld = (int64_t)a.H * HD;
     const T* gb = (const T*)a.dout + start * gld;
-    const float* cb = ((wave & 1) ? a.delta : a.lse) + start;
+    const float* cb = ((wave & 1) ? a.ndelta : a.lse) + start;
     unsigned src[C::NI];
 #pragma unroll
     for (int j = 0; j < C::NI; ++j) {       // the waves alternate between the two images: an instruction knows its descriptor
@@ -581,7 +644,9 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 256 ? 1 : 2)) void window_dk
             ++fh;
         }
     };
-    const TrAt<C> tr(lane);
+    const TrAt<C, (C::RB < 256)> tr(lane);
+    const RowAt<C, (C::RB < 256)> rows(lane);
+    const unsigned lds = lds_u32(smem);
     int fill = 0, use = 0, ct = 0;
     for (; fill < STAGES - 1 && fill < total; ++fill) issue(smem + fill * STAGE);
     fill = STAGES - 1;
@@ -589,16 +654,15 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 256 ? 1 : 2)) void window_dk
         tile_ready<(STAGES - 2) * (C::NI + 1)>(it + STAGES - 1 > total);
         if (it + STAGES - 1 < total) issue(smem + fill * STAGE);
         fill = fill + 1 == STAGES ? 0 : fill + 1;
-        const unsigned char *ql = smem + use * STAGE, *gl = ql + C::TILE;
+        const unsigned ql = lds + use * STAGE, gl = ql + C::TILE;
         use = use + 1 == STAGES ? 0 : use + 1;
-        const float *lsl = reinterpret_cast<const float*>(gl + C::TILE), *dll = lsl + 64;
         const int q0 = (t0 + ct) * C::KT, q1 = q0 + C::KT - 1;
         ct = ct + 1 == nt ? 0 : ct + 1;
         if (k0 >= len || q1 < k0 - a.right || (q0 > klast + a.left && k0 >= sinks)) continue;
         const bool whole = q1 < len && q0 >= klast - a.right && (q1 <= k0 + a.left || klast < sinks);
-        auto vis = [&](int i) { return q0 + i < len && visible(q0 + i, key, a.left, a.right, sinks); };
-        dkv_block<C, 0>(ql, gl, lsl, dll, kf, vf, c, whole, vis, tr, dk, dv, lane);
-        if constexpr (C::KB == 2) dkv_block<C, 32>(ql, gl, lsl, dll, kf, vf, c, whole, vis, tr, dk, dv, lane);
+        const int first = key - a.right - q0, last = (key < sinks ? len - 1 : min(len - 1, key + a.left)) - q0;
+        dkv_block<C, 0>(ql, gl, gl + C::TILE, rows, kf, vf, c, whole, first, last, tr, dk, dv, h2);
+        if constexpr (C::KB == 2) dkv_block<C, 32>(ql, gl, gl + C::TILE, rows, kf, vf, c, whole, first, last, tr, dk, dv, h2);
     }
     if (key < len) {
         T* row = (T*)a.dqkv + (start + key) * (a.H + 2 * a.KV) * HD + (a.H + hk) * HD;
@@ -613,7 +677,7 @@ __global__ __launch_bounds__(WT, (sizeof(T) * HD >= 256 ? 1 : 2)) void window_dk
 template <typename T, int HD>
 __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
     using C = WCfg<T, HD, 32>;
-    constexpr int STAGE = 2 * C::TILE + 256, NL = C::CH / 2;
+    constexpr int STAGE = 2 * C::TILE + 512, NL = C::CH / 2;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, r = lane & 31, h2 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -636,14 +700,16 @@ __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
             kf[j] = *reinterpret_cast<const V*>(kb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
             vf[j] = *reinterpret_cast<const V*>(vb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
         }
-    const TrAt<C> tr(lane);
+    const TrAt<C, false> tr(lane);
+    const RowAt<C, false> rows(lane);
     f32x16_t dk[C::DB], dv[C::DB];
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) dk[db] = dv[db] = splat16(0.f);
     const int t0 = (k0 + a.left + 1) / 32, nt = max(0, (len - 1) / 32 - t0 + 1);         // empty where the window reaches the end
     const int total = nt * rep, per = (total + a.far_parts - 1) / a.far_parts, i0 = part * per, i1 = min(total, i0 + per);
     unsigned char *ql = smem + wave * STAGE, *gl = ql + C::TILE;
-    float *lsl = reinterpret_cast<float*>(gl + C::TILE), *dll = lsl + 32;
+    float* cst = reinterpret_cast<float*>(gl + C::TILE) + h2 * 64 + r;
+    const unsigned la = lds_u32(ql);
     const int lim = min(kend - 1, k0 + 31) + a.left;        // queries past this see every key of the group
     for (int it = i0; it < i1; ++it) {
         const int h = hk * rep + it / nt, q0 = (t0 + it % nt) * 32;
@@ -658,7 +724,7 @@ __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
                 gr[i] = *reinterpret_cast<const V*>(gs + (int64_t)row * a.H * HD + col);
             }
         }
-        const float cr = q0 + r < len ? (h2 ? a.delta : a.lse)[(int64_t)h * a.R + start + q0 + r] : 0.f;
+        const float cr = q0 + r < len ? (h2 ? a.ndelta : a.lse)[(int64_t)h * a.R + start + q0 + r] : 0.f;
         wave_sync();                                        // the previous tile's reads are done
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
@@ -666,10 +732,10 @@ __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
             *reinterpret_cast<V*>(ql + at) = qr[i];
             *reinterpret_cast<V*>(gl + at) = gr[i];
         }
-        lsl[lane] = cr;
+        *cst = cr;
         wave_sync();
-        dkv_block<C, 0>(ql, gl, lsl, dll, kf, vf, c, q0 > lim && q0 + 31 < len && kend >= k0 + 32,
-                            [&](int i) { return q0 + i < len && key < kend && q0 + i > key + a.left; }, tr, dk, dv, lane);
+        dkv_block<C, 0>(la, la + C::TILE, la + 2 * C::TILE, rows, kf, vf, c, q0 > lim && q0 + 31 < len && kend >= k0 + 32,
+                            key + a.left + 1 - q0, key < kend ? len - 1 - q0 : -1, tr, dk, dv, h2);
     }
     float* w = a.far_ws + (((int64_t)(b * a.KV + hk) * a.far_groups + grp) * a.far_parts + part) * (2 * C::DB * 1024) + lane;
 #pragma unroll
@@ -718,7 +784,7 @@ template <typename T, int HD> static int run_bwd(const WArgs& a, hipStream_t s) 
     if (int rc = launch<window_dq_kernel<T, HD>>(who, nrb * a.H * a.NB, KvRing<WCfg<T, HD>>::STAGES * KvRing<WCfg<T, HD>>::STAGE, a, s)) return rc;
     if (a.far_parts) {
         const int lists = a.NB * a.KV * a.far_groups, size = 2 * WCfg<T, HD>::DB * 1024;
-        if (int rc = launch<window_far_kernel<T, HD>>(who, (int64_t)lists * (a.far_parts / 4), 4 * (2 * WCfg<T, HD, 32>::TILE + 256), a, s)) return rc;
+        if (int rc = launch<window_far_kernel<T, HD>>(who, (int64_t)lists * (a.far_parts / 4), 4 * (2 * WCfg<T, HD, 32>::TILE + 512), a, s)) return rc;
         hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, lists), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
         STAR_LAUNCH_CHECK(who);
     }
@@ -785,7 +851,7 @@ extern "C" int star_attn_window_bwd(const StarAttnWindow* g, void* stream) {
     STAR_CHECK((uintptr_t)g->dout % 16 == 0 && (uintptr_t)g->dqkv % 16 == 0, "star_attn_window_bwd: dout and dqkv must be 16-byte aligned");
     a.dout = g->dout;
     a.dqkv = g->dqkv;
-    a.delta = g->ws;
+    a.ndelta = g->ws;
     far_plan(g->NB, g->L, g->H, g->KV, g->left, g->sinks, a.far_groups, a.far_parts);
     a.far_ws = g->ws + (g->H * g->R + 63) / 64 * 64;
     hipStream_t s = (hipStream_t)stream;

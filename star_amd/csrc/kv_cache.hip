@@ -274,22 +274,22 @@ __global__ __launch_bounds__(KT_) void step_kernel(StepArgs a) {
     }
 }
 
-// the splits of one (sequence, query head), in their order
+// The splits (at most 64) of one (sequence, query head), in their order: a wave per row, a split's weight on a lane.
 template <typename T>
 __global__ __launch_bounds__(KT_) void step_join_kernel(const float* __restrict__ ws, T* __restrict__ out, int rows, int hd, int splits) {
-    const int i = blockIdx.x * KT_ + threadIdx.x, row = i / hd, d = i % hd;
+    const int lane = threadIdx.x & 63, row = blockIdx.x * (KT_ / 64) + (threadIdx.x >> 6);
     if (row >= rows) return;
     const float* w = ws + (int64_t)row * splits * (hd + 2);
-    float mn = -INFINITY;
-    for (int s = 0; s < splits; ++s) mn = fmaxf(mn, w[s * (hd + 2) + hd]);
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    float l = 0.f, t = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        const float f = __builtin_amdgcn_exp2f(w[s * (hd + 2) + hd] - ref);
-        l += w[s * (hd + 2) + hd + 1] * f;
-        t += w[s * (hd + 2) + d] * f;
+    const float m = lane < splits ? w[lane * (hd + 2) + hd] : -INFINITY, l = lane < splits ? w[lane * (hd + 2) + hd + 1] : 0.f;
+    const float mn = wave_max(m);
+    const float f = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn), sum = wave_sum(l * f);
+    const float inv = mn == -INFINITY ? 0.f : 1.0f / sum;         // an idle entry saw nothing: zeros
+    for (int d = lane; d < hd; d += 64) {
+        float t = 0.f;
+#pragma unroll 8
+        for (int s = 0; s < splits; ++s) t = __builtin_fmaf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s)), w[s * (hd + 2) + d], t);
+        Act<T>::st(out + (int64_t)row * hd + d, t * inv);
     }
-    Act<T>::st(out + i, mn == -INFINITY ? 0.f : t / l);          // an idle entry saw nothing: zeros
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -326,7 +326,7 @@ static int step_splits(int NB, int H, int KV, int cap, int left, int sinks) {
     const int64_t vis = (int64_t)left + 1 + sinks < cap ? (int64_t)left + 1 + sinks : cap;
     int64_t s = (4 * (int64_t)star_num_cus() + blocks - 1) / blocks;
     if (s > vis / 64) s = vis / 64;
-    return s < 1 ? 1 : (int)s;
+    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
 extern "C" int64_t star_attn_window_step_ws(int NB, int H, int KV, int hd, int cap, int left, int sinks) {
@@ -347,7 +347,7 @@ template <typename T> static void step_run(const StepArgs& a, int hd, int G, dim
     else if (hd == 64) step_launch<T, 64>(a, G, grid, s);
     else step_launch<T, 128>(a, G, grid, s);
     if (a.splits > 1)
-        hipLaunchKernelGGL(step_join_kernel<T>, dim3(cdiv((int64_t)a.NB * a.H * hd, KT_)), dim3(KT_), 0, s, a.ws, (T*)a.out, a.NB * a.H, hd, a.splits);
+        hipLaunchKernelGGL(step_join_kernel<T>, dim3(cdiv((int64_t)a.NB * a.H, KT_ / 64)), dim3(KT_), 0, s, a.ws, (T*)a.out, a.NB * a.H, hd, a.splits);
 }
 
 extern "C" int star_attn_window_step(const StarAttnStep* g, void* stream) {
