@@ -284,10 +284,17 @@ __global__ __launch_bounds__(KT_) void step_join_kernel(const float* __restrict_
     const float mn = wave_max(m);
     const float f = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn), sum = wave_sum(l * f);
     const float inv = mn == -INFINITY ? 0.f : 1.0f / sum;         // an idle entry saw nothing: zeros
+    // eight splits' rows on their way at a time; lanes past the last split have weight 0 and read its row
     for (int d = lane; d < hd; d += 64) {
         float t = 0.f;
-#pragma unroll 8
-        for (int s = 0; s < splits; ++s) t = __builtin_fmaf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s)), w[s * (hd + 2) + d], t);
+        for (int s0 = 0; s0 < splits; s0 += 8) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = w[min(s0 + k, splits - 1) * (hd + 2) + d];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (s0 + k < splits) t = __builtin_fmaf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + k)), v[k], t);
+        }
         Act<T>::st(out + (int64_t)row * hd + d, t * inv);
     }
 }

@@ -1,6 +1,5 @@
 """Tensor-level wrappers over the C ABI (one per kernel group).  PyTorch only allocates and hands over
 device pointers here; all arithmetic happens in libstar_hip.so."""
-import contextlib
 import ctypes as C
 import functools
 import math
@@ -373,19 +372,50 @@ def attn_bwd(qkv, out, dout, lse, nb, l, h, hd):
 
 
 # ---- rotary positions, sliding-window attention with sinks, rolling key/value cache ------------------------------------
-def _on(first, *rest):
-    """The device that a call runs on: the operands' own, which need not be the current one.  -> a context to launch in."""
-    _cuda(first, *rest)
+# These calls are short (a decoding step is a few microseconds of GPU time), so their host side is kept lean: no context managers and no
+# keyword calls on the usual path.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _home(first, *rest):
+    """index of the operands' device, which every operand has to be on"""
+    if not first.is_cuda:
+        raise RuntimeError("star_amd ops need device tensors (got a CPU tensor)")
     dev = first.device
-    if any(t is not None and t.device != dev for t in rest):
-        raise RuntimeError("star_amd ops need all tensors on one device (got %s)" % ", ".join(sorted({str(t.device) for t in (first,) + rest if t is not None})))
-    return torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext()
+    for t in rest:
+        if t is not None and t.device != dev:
+            _cuda(t)
+            raise RuntimeError("star_amd ops need all tensors on one device (got %s and %s)" % (dev, t.device))
+    return dev.index
 
 
-def _rows2d(t, name):
-    """A matrix whose rows are dense and may lie apart: what the kernels take of packed qkv rows."""
-    assert t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1), "%s must be a matrix with dense rows" % name
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _at_home(fn):
+    """fn(home, tensors ..., ...) launches on the current device: where the operands live on another one, that is made current for the call."""
+    @functools.wraps(fn)
+    def call(first, *args, **kw):
+        home = _home(first)
+        if home == torch.cuda.current_device():
+            return fn(home, first, *args, **kw)
+        with torch.cuda.device(home):
+            return fn(home, first, *args, **kw)
+    return call
+
+
+def _call(tag, nbytes, fn, *args):
+    if PROFILER is None:
+        rc = fn(*args)
+    else:
+        with _timed(tag, 0.0, float(nbytes)):
+            rc = fn(*args)
+    if rc:
+        L.check(rc)
+
+
+def _rows2d(t, shape, name):
+    """row stride of a matrix whose rows are dense and may lie apart: what the kernels take of packed qkv rows"""
+    st = t.stride()
+    assert len(shape) == 2 and (st[1] == 1 or shape[1] <= 1), "%s must be a matrix with dense rows" % name
+    return st[0] if shape[0] > 1 else max(st[0], shape[1])
 
 
 @functools.lru_cache(maxsize=256)
@@ -407,27 +437,31 @@ def rope_plan(sections, base=10000.0, per_axis=False, interleaved=False):
     return f
 
 
-def _positions(pos, plan, r):
+def _positions(pos, axes, r):
     if pos.dim() == 1:
         pos = pos.unsqueeze(0)
-    assert pos.dtype == torch.int32 and pos.dim() == 2 and pos.shape == (plan.axes, r), "positions must be int32 [%d, %d]" % (plan.axes, r)
-    assert pos.stride(1) == 1 or r <= 1, "positions of one axis must be dense"
-    return pos, (pos.stride(0) if plan.axes > 1 else max(pos.stride(0), r))
+    assert pos.dtype == torch.int32 and pos.shape == (axes, r), "positions must be int32 [%d, %d]" % (axes, r)
+    st = pos.stride()
+    assert st[1] == 1 or r <= 1, "positions of one axis must be dense"
+    return pos, (st[0] if axes > 1 else max(st[0], r))
 
 
-def _rope(x, pos, rot_heads, hd, sections, base, per_axis, interleaved, out, inverse):
-    with _on(x, pos, out):
-        ld = _rows2d(x, "x")
-        r, w = x.shape
-        plan = rope_plan(tuple(sections), float(base), bool(per_axis), bool(interleaved))
-        pos, pos_ld = _positions(pos, plan, r)
-        if out is None:
-            out = torch.empty(r, w, dtype=x.dtype, device=x.device)
-        assert out.shape == x.shape and out.dtype == x.dtype
-        out_ld = _rows2d(out, "out")
-        if r:
-            with _timed("rope", 0.0, 2.0 * r * w * x.element_size()):
-                L.check(L.lib().star_rope(p(x), ld, p(out), out_ld, p(pos), pos_ld, C.byref(plan), r, w, rot_heads, hd, inverse, L.dt_of(x), L.stream()))
+@_at_home
+def _rope(home, x, pos, rot_heads, hd, sections, base, per_axis, interleaved, out, inverse):
+    _home(x, pos, out)
+    shape = x.shape
+    ld = _rows2d(x, shape, "x")
+    r, w = shape
+    plan = rope_plan(tuple(sections), base, per_axis, interleaved)
+    pos, pos_ld = _positions(pos, plan.axes, r)
+    if out is None:
+        out, out_ld = x.new_empty(shape), w
+    else:
+        assert out.shape == shape and out.dtype == x.dtype
+        out_ld = _rows2d(out, shape, "out")
+    if r:
+        _call("rope", 2 * r * w * x.element_size(), L.lib().star_rope, x.data_ptr(), ld, out.data_ptr(), out_ld, pos.data_ptr(), pos_ld, plan, r, w,
+              rot_heads, hd, inverse, L.dt_of(x), _raw_stream(home))
     return out
 
 
@@ -444,22 +478,38 @@ def rope_bwd(dy, pos, rot_heads, hd, sections, base=10000.0, per_axis=False, int
     return _rope(dy, pos, rot_heads, hd, sections, base, per_axis, interleaved, out, 1)
 
 
-def _window(qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale):
-    ld = _rows2d(qkv, "qkv")
-    kv = h if kv_heads is None else kv_heads
-    r, w = qkv.shape
+def _offsets(offsets, nb):
+    assert offsets.dtype == torch.int64 and offsets.shape == (nb + 1,) and offsets.stride(0) == 1, "offsets must be int64 [nb + 1]"
+    return offsets.data_ptr()
+
+
+def _window(qkv, nb, l, h, hd, kv, left, right, sinks, offsets, scale):
+    """the StarAttnWindow of a call, without its outputs; checks what the C entry cannot see"""
+    shape = qkv.shape
+    ld = _rows2d(qkv, shape, "qkv")
+    r, w = shape
     assert w == (h + 2 * kv) * hd, "qkv rows of %d columns are not %d + 2 * %d heads of %d" % (w, h, kv, hd)
-    if offsets is not None:
-        assert offsets.dtype == torch.int64 and offsets.is_contiguous() and offsets.shape == (nb + 1,), "offsets must be int64 [nb + 1]"
+    assert offsets is not None or r == nb * l, "%d rows for %d sequences of %d" % (r, nb, l)
+    return L.StarAttnWindow(qkv.data_ptr(), None if offsets is None else _offsets(offsets, nb), None, None, None, None, None, ld, r, nb, l, h, kv, hd,
+                            l if left is None else left, l if right is None else right, sinks, hd ** -0.5 if scale is None else scale, L.dt_of(qkv))
+
+
+@_at_home
+def _window_fwd(home, qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale, want_lse, out):
+    _home(qkv, offsets, out)
+    g = _window(qkv, nb, l, h, hd, h if kv_heads is None else kv_heads, left, right, sinks, offsets, scale)
+    r = g.R
+    if out is None:
+        out = (qkv.new_empty if offsets is None else qkv.new_zeros)((r, h * hd))     # rows of no sequence stay as they are: zeros here
     else:
-        assert r == nb * l, "%d rows for %d sequences of %d" % (r, nb, l)
-    return L.StarAttnWindow(qkv=p(qkv), offsets=p(offsets), ld=ld, R=r, NB=nb, L=l, H=h, KV=kv, hd=hd, left=l if left is None else left,
-                            right=l if right is None else right, sinks=sinks, scale=hd ** -0.5 if scale is None else scale, dt=L.dt_of(qkv))
-
-
-def _fresh(r, w, like, offsets):
-    """an output of r rows: with offsets, rows of no sequence are left as they were -- zeros in a new tensor"""
-    return (torch.empty if offsets is None else torch.zeros)(r, w, dtype=like.dtype, device=like.device)
+        assert out.shape == (r, h * hd) and out.dtype == qkv.dtype and out.is_contiguous()
+    lse = qkv.new_empty((h, r), dtype=torch.float32) if want_lse else None
+    if r:
+        g.out = out.data_ptr()
+        if want_lse:
+            g.lse = lse.data_ptr()
+        _call("attn_window_fwd", r * (qkv.shape[1] + h * hd) * qkv.element_size(), L.lib().star_attn_window_fwd, g, _raw_stream(home))
+    return out, lse
 
 
 def attn_window_fwd(qkv, nb, l, h, hd, kv_heads=None, left=None, right=0, sinks=0, offsets=None, scale=None, want_lse=True, out=None):
@@ -468,46 +518,56 @@ def attn_window_fwd(qkv, nb, l, h, hd, kv_heads=None, left=None, right=0, sinks=
     bound (right=0: causal; left=right=None: everything).  nb sequences of l rows, or ragged: offsets int64 [nb + 1] on the device, l >= the
     longest sequence (of a longer one only the first l rows take part).  Rows outside every sequence are neither read nor written.
     -> (out [R, h*hd], lse float32 [h, R] or None)"""
-    with _on(qkv, offsets, out):
-        g = _window(qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale)
-        r = qkv.shape[0]
-        if out is None:
-            out = _fresh(r, h * hd, qkv, offsets)
-        assert out.shape == (r, h * hd) and out.dtype == qkv.dtype and out.is_contiguous()
-        lse = torch.empty(h, r, dtype=torch.float32, device=qkv.device) if want_lse else None
-        if r:
-            g.out, g.lse = p(out), p(lse)
-            with _timed("attn_window_fwd", 0.0, float(r) * (qkv.shape[1] + h * hd) * qkv.element_size()):
-                L.check(L.lib().star_attn_window_fwd(C.byref(g), L.stream()))
-    return out, lse
+    return _window_fwd(qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale, want_lse, out)
 
 
-def attn_window_bwd(qkv, out, dout, lse, nb, l, h, hd, kv_heads=None, left=None, right=0, sinks=0, offsets=None, scale=None, dqkv=None):
-    """Gradient of attn_window_fwd (the same arguments): dout [R, h*hd] -> dqkv [R, (h + 2 kv_heads) hd].  Two launches, each recomputing the scores
-    from the stored row log-sum-exp; no atomics, bitwise reproducible."""
-    with _on(qkv, out, dout, lse, offsets, dqkv):
-        g = _window(qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale)
-        r, w = qkv.shape
-        for t in (out, dout):
-            assert t.shape == (r, h * hd) and t.dtype == qkv.dtype and t.is_contiguous()
-        assert lse.shape == (h, r) and lse.dtype == torch.float32 and lse.is_contiguous()
-        if dqkv is None:
-            dqkv = _fresh(r, w, qkv, offsets)
-        assert dqkv.shape == (r, w) and dqkv.dtype == qkv.dtype and dqkv.is_contiguous()
-        if r:
-            ws = torch.empty(L.lib().star_attn_window_bwd_ws(r, nb, l, h, g.KV, hd, g.left, sinks), dtype=torch.float32, device=qkv.device)
-            g.out, g.lse, g.dout, g.dqkv, g.ws = p(out), p(lse), p(dout), p(dqkv), p(ws)
-            with _timed("attn_window_bwd", 0.0, float(r) * 2 * (w + h * hd) * qkv.element_size()):
-                L.check(L.lib().star_attn_window_bwd(C.byref(g), L.stream()))
+@_at_home
+def _window_bwd(home, qkv, out, dout, lse, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale, dqkv):
+    _home(qkv, out, dout, lse, offsets, dqkv)
+    g = _window(qkv, nb, l, h, hd, h if kv_heads is None else kv_heads, left, right, sinks, offsets, scale)
+    r = g.R
+    for t in (out, dout):
+        assert t.shape == (r, h * hd) and t.dtype == qkv.dtype and t.is_contiguous()
+    assert lse.shape == (h, r) and lse.dtype == torch.float32 and lse.is_contiguous()
+    if dqkv is None:
+        dqkv = (qkv.new_empty if offsets is None else qkv.new_zeros)(qkv.shape)
+    else:
+        assert dqkv.shape == qkv.shape and dqkv.dtype == qkv.dtype and dqkv.is_contiguous()
+    if r:
+        lib = L.lib()
+        ws = qkv.new_empty(lib.star_attn_window_bwd_ws(r, nb, l, h, g.KV, hd, g.left, sinks), dtype=torch.float32)
+        g.out, g.lse, g.dout, g.dqkv, g.ws = out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dqkv.data_ptr(), ws.data_ptr()
+        _call("attn_window_bwd", 2 * r * (qkv.shape[1] + h * hd) * qkv.element_size(), lib.star_attn_window_bwd, g, _raw_stream(home))
     return dqkv
 
 
-def _cache_dims(cache, qkv, nb, hd_heads, h, lengths):
-    assert cache.dim() == 5 and cache.shape[0] == 2 and cache.shape[1] == nb and cache.is_contiguous(), "cache must be a dense [2, nb, kv_heads, capacity, hd]"
-    kv, cap, hd = cache.shape[2:]
-    assert cache.dtype == qkv.dtype and hd_heads == (h + 2 * kv) * hd, "qkv rows of %d columns are not %d + 2 * %d heads of %d" % (hd_heads, h, kv, hd)
-    assert lengths.dtype == torch.int32 and lengths.is_contiguous() and lengths.shape == (nb,), "lengths must be int32 [nb]"
-    return kv, cap, hd
+def attn_window_bwd(qkv, out, dout, lse, nb, l, h, hd, kv_heads=None, left=None, right=0, sinks=0, offsets=None, scale=None, dqkv=None):
+    """Gradient of attn_window_fwd (the same arguments): dout [R, h*hd] -> dqkv [R, (h + 2 kv_heads) hd].  The scores are recomputed from the stored
+    row log-sum-exp; no atomics, bitwise reproducible."""
+    return _window_bwd(qkv, out, dout, lse, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale, dqkv)
+
+
+def _cache_dims(cache, qkv, w, h, lengths):
+    shape = cache.shape
+    assert len(shape) == 5 and shape[0] == 2 and cache.is_contiguous(), "cache must be a dense [2, nb, kv_heads, capacity, hd]"
+    _, nb, kv, cap, hd = shape
+    assert cache.dtype == qkv.dtype and w == (h + 2 * kv) * hd, "qkv rows of %d columns are not %d + 2 * %d heads of %d" % (w, h, kv, hd)
+    assert lengths.dtype == torch.int32 and lengths.shape == (nb,) and (nb <= 1 or lengths.stride(0) == 1), "lengths must be int32 [nb]"
+    return nb, kv, cap, hd
+
+
+@_at_home
+def _kv_append(home, qkv, cache, lengths, l, h, sinks, offsets):
+    _home(qkv, cache, lengths, offsets)
+    shape = qkv.shape
+    ld = _rows2d(qkv, shape, "qkv")
+    r = shape[0]
+    nb, kv, cap, hd = _cache_dims(cache, qkv, shape[1], h, lengths)
+    assert offsets is not None or r == nb * l, "%d rows for %d sequences of %d" % (r, nb, l)
+    if r and nb:
+        _call("kv_append", 4 * r * kv * hd * qkv.element_size(), L.lib().star_kv_append, qkv.data_ptr(), ld, None if offsets is None else _offsets(offsets, nb),
+              cache.data_ptr(), lengths.data_ptr(), r, nb, l, h, kv, hd, cap, sinks, L.dt_of(qkv), _raw_stream(home))
+    return cache
 
 
 def kv_append(qkv, cache, lengths, l, h, sinks=0, offsets=None):
@@ -515,19 +575,34 @@ def kv_append(qkv, cache, lengths, l, h, sinks=0, offsets=None):
     lies in slot p for p < sinks, else in slot sinks + (p - sinks) % (capacity - sinks): the sinks stay, the ring behind them holds the newest
     tokens (capacity >= the longest sequence: an ordinary cache).  lengths int32 [nb]: a sequence's tokens with the new ones, which are
     its last: l rows of each (qkv [nb*l, ...]) or rows offsets[b] .. offsets[b+1], at most l.  -> cache"""
-    nb = cache.shape[1]
-    with _on(qkv, cache, lengths, offsets):
-        ld = _rows2d(qkv, "qkv")
-        r = qkv.shape[0]
-        kv, cap, hd = _cache_dims(cache, qkv, nb, qkv.shape[1], h, lengths)
-        if offsets is not None:
-            assert offsets.dtype == torch.int64 and offsets.is_contiguous() and offsets.shape == (nb + 1,), "offsets must be int64 [nb + 1]"
-        else:
-            assert r == nb * l, "%d rows for %d sequences of %d" % (r, nb, l)
-        if r and nb:
-            with _timed("kv_append", 0.0, float(r) * 4 * kv * hd * qkv.element_size()):
-                L.check(L.lib().star_kv_append(p(qkv), ld, p(offsets), p(cache), p(lengths), r, nb, l, h, kv, hd, cap, sinks, L.dt_of(qkv), L.stream()))
-    return cache
+    return _kv_append(qkv, cache, lengths, l, h, sinks, offsets)
+
+
+@_at_home
+def _window_step(home, qkv, cache, lengths, h, left, sinks, pos, sections, base, per_axis, interleaved, scale, out):
+    _home(qkv, cache, lengths, pos, out)
+    shape = qkv.shape
+    ld = _rows2d(qkv, shape, "qkv")
+    nb, kv, cap, hd = _cache_dims(cache, qkv, shape[1], h, lengths)
+    assert shape[0] == nb, "%d rows for %d cache entries" % (shape[0], nb)
+    if out is None:
+        out = qkv.new_empty((nb, h * hd))
+    else:
+        assert out.shape == (nb, h * hd) and out.dtype == qkv.dtype and out.is_contiguous()
+    if nb:
+        lib = L.lib()
+        if left is None:
+            left = cap - sinks - 1
+        need = lib.star_attn_window_step_ws(nb, h, kv, hd, cap, left, sinks)
+        ws = qkv.new_empty(need, dtype=torch.float32) if need else None
+        g = L.StarAttnStep(qkv.data_ptr(), cache.data_ptr(), lengths.data_ptr(), None, None, out.data_ptr(), None if ws is None else ws.data_ptr(), ld, 0, nb, h, kv,
+                           hd, cap, left, sinks, hd ** -0.5 if scale is None else scale, L.dt_of(qkv))
+        if sections is not None:
+            plan = rope_plan(tuple(sections), base, per_axis, interleaved)
+            pos, g.pos_ld = _positions(pos, plan.axes, nb)
+            g.pos, g.h_rope = pos.data_ptr(), C.pointer(plan)
+        _call("attn_window_step", nb * min(cap, left + 1 + sinks) * 2 * kv * hd * qkv.element_size(), lib.star_attn_window_step, g, _raw_stream(home))
+    return out
 
 
 def attn_window_step(qkv, cache, lengths, h, left=None, sinks=0, pos=None, sections=None, base=10000.0, per_axis=False, interleaved=False,
@@ -537,29 +612,7 @@ def attn_window_step(qkv, cache, lengths, h, left=None, sinks=0, pos=None, secti
     [axes, nb] first (rope_fwd's arguments).  The key (turned) and the value go into the cache, then the token attends to itself, to the
     `left` tokens before it and to the first `sinks`; None: to all that the ring holds.  left + sinks < capacity.  lengths[b] = 0: an idle
     entry, its row of the result is zeros and its cache stays as it is.  -> out [nb, h*hd]"""
-    nb = cache.shape[1]
-    with _on(qkv, cache, lengths, pos, out):
-        ld = _rows2d(qkv, "qkv")
-        assert qkv.shape[0] == nb, "%d rows for %d cache entries" % (qkv.shape[0], nb)
-        kv, cap, hd = _cache_dims(cache, qkv, nb, qkv.shape[1], h, lengths)
-        plan, pos_ld = None, 0
-        if sections is not None:
-            plan = rope_plan(tuple(sections), float(base), bool(per_axis), bool(interleaved))
-            pos, pos_ld = _positions(pos, plan, nb)
-        if left is None:
-            left = cap - sinks - 1
-        if out is None:
-            out = torch.empty(nb, h * hd, dtype=qkv.dtype, device=qkv.device)
-        assert out.shape == (nb, h * hd) and out.dtype == qkv.dtype and out.is_contiguous()
-        if nb:
-            need = L.lib().star_attn_window_step_ws(nb, h, kv, hd, cap, left, sinks)
-            ws = torch.empty(need, dtype=torch.float32, device=qkv.device) if need else None
-            g = L.StarAttnStep(qkv=p(qkv), cache=p(cache), lengths=p(lengths), pos=p(pos) if plan is not None else None,
-                               h_rope=C.pointer(plan) if plan is not None else None, out=p(out), ws=p(ws), ld=ld, pos_ld=pos_ld, NB=nb, H=h, KV=kv,
-                               hd=hd, cap=cap, left=left, sinks=sinks, scale=hd ** -0.5 if scale is None else scale, dt=L.dt_of(qkv))
-            with _timed("attn_window_step", 0.0, float(nb) * min(cap, left + 1 + sinks) * 2 * kv * hd * qkv.element_size()):
-                L.check(L.lib().star_attn_window_step(C.byref(g), L.stream()))
-    return out
+    return _window_step(qkv, cache, lengths, h, left, sinks, pos, sections, base, per_axis, interleaved, scale, out)
 
 
 # ---------------------------------------------------------------------------------------------------
