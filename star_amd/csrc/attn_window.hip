@@ -270,7 +270,7 @@ struct WArgs {
     const void* dout;
     void* dqkv;
     float* ndelta;           // [H, R] negated row dots
-    float* far_ws;           // [NB, KV, far_groups, far_parts] partial sums of 32 sink keys
+    float* far_ws;           // [NB, KV, far_groups, far_parts] partial sums of 32 sink keys (the parts are blocks)
     int64_t ld, R;
     int NB, L, H, KV, left, right, sinks;
     float scale;
@@ -289,6 +289,25 @@ __device__ __forceinline__ int seq_rows(const WArgs& a, int b, int64_t& start) {
     e = e < s ? s : (e > a.R ? a.R : e);
     start = s;
     return (int)(e - s > a.L ? a.L : e - s);
+}
+
+// Block -> (stream = one head of one sequence, row block).  The row blocks of a stream stay on one XCD and share its L2.  Sequences of one
+// length: every XCD walks a contiguous range of streams, which balances at any count.  Ragged with enough streams: they are dealt to the
+// XCDs in turn, or the XCD that got the long sequences would finish alone (7 sequences of 0 .. 2043 rows, 16 heads, window 128 + 128:
+// forward 42 -> 27 us, dQ 65 -> 43, dK/dV 63 -> 57); their grid is rounded up to whole rounds of 8.
+static __host__ __device__ __forceinline__ bool dealt(const int64_t* offsets, int streams) { return offsets && streams >= 16; }
+__device__ __forceinline__ bool place(const WArgs& a, int streams, int& stream, int& rblk) {
+    const int nrb = (a.L + WROWS - 1) / WROWS;
+    if (dealt(a.offsets, streams)) {
+        const int i = blockIdx.x >> 3;
+        stream = (blockIdx.x & 7) + 8 * (i / nrb);
+        rblk = i % nrb;
+        return stream < streams;
+    }
+    const int work = xcd_remap(blockIdx.x, gridDim.x);
+    stream = work / nrb;
+    rblk = work % nrb;
+    return true;
 }
 
 // the key tiles that queries [q0, q1] see: `ns` leading tiles (sinks in front of the window), then tiles w0 .. w0 + count - ns - 1
@@ -326,9 +345,10 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_FWD(sizeof(T) * HD)) void 
     using C = WCfg<T, HD>;
     using Ring = KvRing<C>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int nrb = (a.L + WROWS - 1) / WROWS;
-    const int work = xcd_remap(blockIdx.x, gridDim.x);      // the row blocks of one head run on one XCD and share its L2
-    const int rblk = nrb - 1 - work % nrb, h = (work / nrb) % a.H, b = work / (nrb * a.H);
+    int stream, rblk;
+    if (!place(a, a.NB * a.H, stream, rblk)) return;
+    const int h = stream % a.H, b = stream / a.H;
+    rblk = (a.L + WROWS - 1) / WROWS - 1 - rblk;             // the last rows see most: they go first
     int64_t start;
     const int len = seq_rows(a, b, start);
     if (rblk * WROWS >= len) return;
@@ -429,9 +449,10 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DQ(sizeof(T) * HD)) void w
     using C = WCfg<T, HD>;
     using Ring = KvRing<C>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int nrb = (a.L + WROWS - 1) / WROWS;
-    const int work = xcd_remap(blockIdx.x, gridDim.x);
-    const int rblk = nrb - 1 - work % nrb, h = (work / nrb) % a.H, b = work / (nrb * a.H);
+    int stream, rblk;
+    if (!place(a, a.NB * a.H, stream, rblk)) return;
+    const int h = stream % a.H, b = stream / a.H;
+    rblk = (a.L + WROWS - 1) / WROWS - 1 - rblk;             // the last rows see most: they go first
     int64_t start;
     const int len = seq_rows(a, b, start);
     if (rblk * WROWS >= len) return;
@@ -572,9 +593,9 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DKV(sizeof(T) * HD)) void 
     using C = typename DkvCfg<T, HD>::C;
     constexpr int STAGE = DkvCfg<T, HD>::STAGE, STAGES = DkvCfg<T, HD>::STAGES;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int nrb = (a.L + WROWS - 1) / WROWS;
-    const int work = xcd_remap(blockIdx.x, gridDim.x);
-    const int rblk = work % nrb, hk = (work / nrb) % a.KV, b = work / (nrb * a.KV);
+    int stream, rblk;
+    if (!place(a, a.NB * a.KV, stream, rblk)) return;
+    const int hk = stream % a.KV, b = stream / a.KV;
     int64_t start;
     const int len = seq_rows(a, b, start);
     if (rblk * WROWS >= len) return;
@@ -673,7 +694,7 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DKV(sizeof(T) * HD)) void 
 
 // The part of dK and dV that reaches the sinks from queries beyond the window (i > j + left): few keys, all queries of the sequence.  Left to
 // the kernel above, the block with the sinks would sweep the whole sequence while the others are long done.  A wave takes one group of 32
-// keys and one of `far_parts` slices of the (query head, 32-query tile) list, with its own images in LDS, and leaves its sums in far_ws.
+// keys and one of 4 far_parts slices of the (query head, 32-query tile) list, with its own images in LDS; a block leaves its waves' sum in far_ws.
 template <typename T, int HD>
 __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
     using C = WCfg<T, HD, 32>;
@@ -681,7 +702,7 @@ __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, r = lane & 31, h2 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nblk = a.far_parts / 4;
+    const int nblk = a.far_parts;
     const int part = (blockIdx.x % nblk) * 4 + wave, grp = (blockIdx.x / nblk) % a.far_groups;
     const int hk = (blockIdx.x / (nblk * a.far_groups)) % a.KV, b = blockIdx.x / (nblk * a.far_groups * a.KV);
     int64_t start;
@@ -706,15 +727,16 @@ __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) dk[db] = dv[db] = splat16(0.f);
     const int t0 = (k0 + a.left + 1) / 32, nt = max(0, (len - 1) / 32 - t0 + 1);         // empty where the window reaches the end
-    const int total = nt * rep, per = (total + a.far_parts - 1) / a.far_parts, i0 = part * per, i1 = min(total, i0 + per);
+    const int total = nt * rep, per = (total + 4 * nblk - 1) / (4 * nblk), i0 = part * per, i1 = min(total, i0 + per);
     unsigned char *ql = smem + wave * STAGE, *gl = ql + C::TILE;
     float* cst = reinterpret_cast<float*>(gl + C::TILE) + h2 * 64 + r;
     const unsigned la = lds_u32(ql);
     const int lim = min(kend - 1, k0 + 31) + a.left;        // queries past this see every key of the group
-    for (int it = i0; it < i1; ++it) {
+    V qr[NL], gr[NL];
+    float cr = 0.f;
+    auto fetch = [&](int it) {
         const int h = hk * rep + it / nt, q0 = (t0 + it % nt) * 32;
         const T *qs = base + h * HD, *gs = (const T*)a.dout + start * a.H * HD + h * HD;
-        V qr[NL], gr[NL];
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int id = lane + i * 64, row = q0 + id / C::CH, col = (id % C::CH) * (16 / C::ES);
@@ -724,7 +746,11 @@ __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
                 gr[i] = *reinterpret_cast<const V*>(gs + (int64_t)row * a.H * HD + col);
             }
         }
-        const float cr = q0 + r < len ? (h2 ? a.ndelta : a.lse)[(int64_t)h * a.R + start + q0 + r] : 0.f;
+        cr = q0 + r < len ? (h2 ? a.ndelta : a.lse)[(int64_t)h * a.R + start + q0 + r] : 0.f;
+    };
+    if (i0 < i1) fetch(i0);
+    for (int it = i0; it < i1; ++it) {
+        const int q0 = (t0 + it % nt) * 32;
         wave_sync();                                        // the previous tile's reads are done
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
@@ -734,17 +760,25 @@ __global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
         }
         *cst = cr;
         wave_sync();
+        if (it + 1 < i1) fetch(it + 1);
         dkv_block<C, 0>(la, la + C::TILE, la + 2 * C::TILE, rows, kf, vf, c, q0 > lim && q0 + 31 < len && kend >= k0 + 32,
-                            key + a.left + 1 - q0, key < kend ? len - 1 - q0 : -1, tr, dk, dv, h2);
+                        key + a.left + 1 - q0, key < kend ? len - 1 - q0 : -1, tr, dk, dv, h2);
     }
-    float* w = a.far_ws + (((int64_t)(b * a.KV + hk) * a.far_groups + grp) * a.far_parts + part) * (2 * C::DB * 1024) + lane;
+    // the block's four parts become one, added in their order: every wave adds four of an accumulator's sixteen registers
+    float* w = a.far_ws + (((int64_t)(b * a.KV + hk) * a.far_groups + grp) * nblk + blockIdx.x % nblk) * (2 * C::DB * 1024);
+    float* sum = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int db = 0; db < C::DB; ++db)
+    for (int i = 0; i < 2 * C::DB; ++i) {
+        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            w[(db * 16 + e) * 64] = dk[db][e];
-            w[((C::DB + db) * 16 + e) * 64] = dv[db][e];
+        for (int e = 0; e < 16; ++e) sum[(wave * 16 + e) * 64 + lane] = i < C::DB ? dk[i % C::DB][e] : dv[i % C::DB][e];
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int at = (wave * 4 + e) * 64 + lane;
+            w[i * 1024 + at] = (sum[at] + sum[1024 + at]) + (sum[2048 + at] + sum[3072 + at]);
         }
+    }
 }
 
 // the parts of a group of sinks, added in their order into the first
@@ -753,7 +787,7 @@ __global__ __launch_bounds__(WT) void window_far_fold_kernel(float* __restrict__
     float* w = ws + (int64_t)blockIdx.y * parts * size;
     if (i >= size) return;
     float t = 0.f;
-#pragma unroll 8
+#pragma unroll 4
     for (int p = 0; p < parts; ++p) t += w[(int64_t)p * size + i];
     w[i] = t;
 }
@@ -775,24 +809,28 @@ template <void (*KERNEL)(WArgs)> static int launch(const char* who, int64_t bloc
     STAR_LAUNCH_CHECK(who);
     return 0;
 }
+static int64_t grid_of(const WArgs& a, int heads) {
+    const int64_t streams = (int64_t)a.NB * heads;
+    return (dealt(a.offsets, (int)streams) ? cdiv(streams, 8) * 8 : streams) * cdiv(a.L, WROWS);
+}
 template <typename T, int HD> static int run_fwd(const WArgs& a, hipStream_t s) {
-    return launch<window_fwd_kernel<T, HD>>("star_attn_window_fwd", (int64_t)cdiv(a.L, WROWS) * a.H * a.NB, KvRing<WCfg<T, HD>>::STAGES * KvRing<WCfg<T, HD>>::STAGE, a, s);
+    return launch<window_fwd_kernel<T, HD>>("star_attn_window_fwd", grid_of(a, a.H), KvRing<WCfg<T, HD>>::STAGES * KvRing<WCfg<T, HD>>::STAGE, a, s);
 }
 template <typename T, int HD> static int run_bwd(const WArgs& a, hipStream_t s) {
     const char* who = "star_attn_window_bwd";
-    const int64_t nrb = cdiv(a.L, WROWS);
-    if (int rc = launch<window_dq_kernel<T, HD>>(who, nrb * a.H * a.NB, KvRing<WCfg<T, HD>>::STAGES * KvRing<WCfg<T, HD>>::STAGE, a, s)) return rc;
+    if (int rc = launch<window_dq_kernel<T, HD>>(who, grid_of(a, a.H), KvRing<WCfg<T, HD>>::STAGES * KvRing<WCfg<T, HD>>::STAGE, a, s)) return rc;
     if (a.far_parts) {
+        constexpr int FAR_LDS = 4 * (2 * WCfg<T, HD, 32>::TILE + 512);
         const int lists = a.NB * a.KV * a.far_groups, size = 2 * WCfg<T, HD>::DB * 1024;
-        if (int rc = launch<window_far_kernel<T, HD>>(who, (int64_t)lists * (a.far_parts / 4), 4 * (2 * WCfg<T, HD, 32>::TILE + 512), a, s)) return rc;
+        if (int rc = launch<window_far_kernel<T, HD>>(who, (int64_t)lists * a.far_parts, FAR_LDS < 16384 ? 16384 : FAR_LDS, a, s)) return rc;
         hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, lists), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
         STAR_LAUNCH_CHECK(who);
     }
-    return launch<window_dkv_kernel<T, HD>>(who, nrb * a.KV * a.NB, DkvCfg<T, HD>::STAGES * DkvCfg<T, HD>::STAGE, a, s);
+    return launch<window_dkv_kernel<T, HD>>(who, grid_of(a, a.KV), DkvCfg<T, HD>::STAGES * DkvCfg<T, HD>::STAGE, a, s);
 }
 
-// How the far queries of the sinks are cut: about eight waves per compute unit in all, no more than 64 parts to add up, and at least two
-// 32-query tiles in a part.  With over 256 sinks, or very many heads, there are enough key blocks with a long sweep to fill the chip: no parts.
+// How the far queries of the sinks are cut: about two blocks of four waves per compute unit in all, no more than 16 parts to add up, and at least
+// two 32-query tiles for a wave.  With over 256 sinks, or very many heads, there are enough key blocks with a long sweep to fill the chip: no parts.
 static void far_plan(int NB, int L, int H, int KV, int left, int sinks, int& groups, int& parts) {
     groups = parts = 0;
     sinks = sinks < L ? sinks : L;
@@ -800,9 +838,9 @@ static void far_plan(int NB, int L, int H, int KV, int left, int sinks, int& gro
     const int64_t lists = (int64_t)NB * KV * cdiv(sinks, 32), tiles = (int64_t)(H / KV) * cdiv(L - left - 1, 32);
     if (lists > 65535) return;
     groups = cdiv(sinks, 32);
-    int64_t p = cdiv(8 * (int64_t)star_num_cus(), lists);
-    if (p > tiles / 2) p = tiles / 2;
-    parts = p < 4 ? 4 : p > 64 ? 64 : (int)(p / 4 * 4);
+    int64_t p = cdiv(2 * (int64_t)star_num_cus(), lists);
+    if (p > tiles / 8) p = tiles / 8;
+    parts = p < 1 ? 1 : p > 16 ? 16 : (int)p;
 }
 
 static int window_args(const char* who, const StarAttnWindow* g, WArgs& a) {
@@ -820,7 +858,7 @@ static int window_args(const char* who, const StarAttnWindow* g, WArgs& a) {
                "%s: qkv rows of %lld elements must hold all heads and be 16-byte aligned", who, (long long)g->ld);
     STAR_CHECK(g->ld * es < (1 << 24), "%s: qkv rows %lld elements apart", who, (long long)g->ld);       // a tile's offsets are 32 bits
     STAR_CHECK((uintptr_t)g->out % 16 == 0, "%s: out must be 16-byte aligned", who);
-    STAR_CHECK((int64_t)cdiv(g->L, WROWS) * g->H * g->NB < (1ll << 31), "%s: NB, H, L too large for the grid", who);
+    STAR_CHECK((int64_t)cdiv(g->L, WROWS) * ((int64_t)g->H * g->NB + 7) < (1ll << 31), "%s: NB, H, L too large for the grid", who);
     // a bound over L says the same as L: what is left cannot overflow in i + right and i - left
     a = WArgs{g->qkv, g->offsets, g->out, g->lse, nullptr, nullptr, nullptr, nullptr, g->ld, g->R, g->NB, g->L, g->H, g->KV,
               g->left < g->L ? g->left : g->L, g->right < g->L ? g->right : g->L, g->sinks < g->L ? g->sinks : g->L, g->scale, 0, 0};
