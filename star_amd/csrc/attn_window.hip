@@ -34,7 +34,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 #define LOG2E 1.4426950408889634f
 #define RESCALE_TH 8.0f           // log2 units: the reference maximum is raised only when a row exceeds it by 2^8 (float32 sums: no loss)
 
-template <typename T, int HD, int ROWS = sizeof(T) == 2 ? 64 : 32> struct WCfg {
+template <typename T, int HD, int ROWS = sizeof(T) == 2 ? 64 : 32, int NW_ = 4> struct WCfg {
     using Type = T;
     static constexpr int HDIM = HD;
     static constexpr int ES = sizeof(T);
@@ -47,7 +47,8 @@ template <typename T, int HD, int ROWS = sizeof(T) == 2 ? 64 : 32> struct WCfg {
     static constexpr int TILE = KT * RB;
     static constexpr int RPP = 1024 / RB;                   // rows of a 1-KiB piece: what one wave's LDS-DMA instruction fills
     static constexpr int NP = TILE / 1024;                  // pieces of an image
-    static constexpr int NI = 2 * NP / 4;                   // pieces that each of the four waves brings per pair of images
+    static constexpr int NW = NW_;
+    static constexpr int NI = 2 * NP / NW;                  // pieces that each of the NW waves that share a tile brings per pair of images
     // The 16-byte chunks of a row are permuted by the row's number, so that neither 16 lanes reading one chunk of 16 successive rows nor
     // 32 lanes of a transposing read (4 rows x 4 chunks) hit one of the 64 banks twice.
     // (A bit permutation of the row: swizzle(a ^ b) = swizzle(a) ^ swizzle(b).)
@@ -73,12 +74,16 @@ template <class C> __device__ __forceinline__ unsigned piece_src(int p, int lane
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned char* lds, unsigned off) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 16, off, 0, 0, 0);
 }
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, unsigned char* lds, unsigned off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 4, off, 0, 0, 0);
+}
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // every wave's DMA of the tile has landed, and every wave is done with the stage that is filled next
-template <int N> __device__ __forceinline__ void tile_ready(bool last) {
+// (a wave with a ring of its own needs no barrier: its reads of a stage have returned when it fills it again)
+template <int N, bool OWN> __device__ __forceinline__ void tile_ready(bool last) {
     if (last) wait_vm<0>();
     else wait_vm<N>();
-    __builtin_amdgcn_s_barrier();
+    if constexpr (!OWN) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
 
@@ -297,8 +302,8 @@ __device__ __forceinline__ int seq_rows(const WArgs& a, int b, int64_t& start) {
 // XCDs in turn, or the XCD that got the long sequences would finish alone (7 sequences of 0 .. 2043 rows, 16 heads, window 128 + 128:
 // forward 42 -> 27 us, dQ 65 -> 43, dK/dV 63 -> 57); their grid is rounded up to whole rounds of 8.
 static __host__ __device__ __forceinline__ bool dealt(const int64_t* offsets, int streams) { return offsets && streams >= 16; }
-__device__ __forceinline__ bool place(const WArgs& a, int streams, int side, int& stream, int& rblk) {
-    const int nrb = (a.L + WROWS - 1) / WROWS;
+__device__ __forceinline__ bool place(const WArgs& a, int rows, int streams, int side, int& stream, int& rblk) {
+    const int nrb = (a.L + rows - 1) / rows;
     if (dealt(a.offsets, streams)) {
         const int i = blockIdx.x >> 3;
         stream = (blockIdx.x & 7) + 8 * (i / nrb);
@@ -319,9 +324,12 @@ template <int KT> __device__ __forceinline__ int key_tiles(int q0, int q1, int l
     return ns + hi / KT - w0 + 1;
 }
 
+// the tiles of a launch form (see the split form below): shared by four waves, or a wave's own
+template <typename T, int HD, bool SPLIT> using RowCfg = std::conditional_t<SPLIT, WCfg<T, HD, 32, 1>, WCfg<T, HD>>;
+
 // A ring of STAGES (K image | V image) stages: while one tile is worked on the next STAGES - 1 are on their way, without registers.
 template <class C> struct KvRing {
-    static constexpr int STAGE = 2 * C::TILE, STAGES = STAGE > 8192 ? 2 : 3;
+    static constexpr int STAGE = 2 * C::TILE, STAGES = C::NW == 1 || STAGE > 8192 ? 2 : 3, BYTES = STAGES * STAGE;
     const typename C::Type* k;              // key 0 of the head; its value lies v columns further on
     int64_t ld;
     int v, len, wave;
@@ -341,22 +349,45 @@ template <class C> struct KvRing {
     }
 };
 
-template <typename T, int HD>
+// Split form: the four waves of a block work on the same 32 rows (dK/dV: keys), each on every fourth tile with a ring of its own, and are added up
+// through LDS, in their order, when all are done.  For launches whose row form (a wave per 32 rows, four sharing the tiles) leaves most of the
+// chip idle (SplitUpTo).
+// mul * sum of the waves' accumulators -> the lane's row: a wave adds and stores four of the sixteen registers of every block.
+template <class C> __device__ __forceinline__ void join_rows(const f32x16_t (&acc)[C::DB], float mul, float* sum, bool valid, typename C::Type* row, int wave, int lane) {
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum[(wave * 16 + e) * 64 + lane] = acc[db][e] * mul;
+        __syncthreads();
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int at = (wave * 4 + e) * 64 + lane;
+            v[e] = (sum[at] + sum[1024 + at]) + (sum[2048 + at] + sum[3072 + at]);
+        }
+        const int d = db * 32 + 8 * wave + 4 * (lane >> 5);
+        if (valid && d < C::HDIM) st4(row + d, v);
+    }
+}
+
+template <typename T, int HD, bool SPLIT>
 __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_FWD(sizeof(T) * HD)) void window_fwd_kernel(WArgs a) {
-    using C = WCfg<T, HD>;
+    using C = RowCfg<T, HD, SPLIT>;
+    constexpr int ROWS = SPLIT ? 32 : WROWS, STEP = SPLIT ? 4 : 1;
     using Ring = KvRing<C>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     int stream, rblk;
-    if (!place(a, a.NB * a.H, a.H / a.KV, stream, rblk)) return;
+    if (!place(a, ROWS, a.NB * a.H, a.H / a.KV, stream, rblk)) return;
     const int h = stream % a.H, b = stream / a.H;
-    rblk = (a.L + WROWS - 1) / WROWS - 1 - rblk;             // the last rows see most: they go first
+    rblk = (a.L + ROWS - 1) / ROWS - 1 - rblk;             // the last rows see most: they go first
     int64_t start;
     const int len = seq_rows(a, b, start);
-    if (rblk * WROWS >= len) return;
+    if (rblk * ROWS >= len) return;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h2 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const T* base = (const T*)a.qkv + start * a.ld;
-    const int q0 = rblk * WROWS + wave * 32, q = q0 + r;
+    const int q0 = rblk * ROWS + (SPLIT ? 0 : wave * 32), q = q0 + r;
     const float c = a.scale * LOG2E;
 
     typename Frag<T>::V qf[C::FR] = {};
@@ -371,19 +402,24 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_FWD(sizeof(T) * HD)) void 
     float m = -INFINITY, l = 0.f;       // the lane pair holds one row's statistics: m in both, l as two partial sums
 
     int ns, w0;
-    const int nt = key_tiles<C::KT>(rblk * WROWS, min(rblk * WROWS + WROWS, len) - 1, len, a.left, a.right, a.sinks, ns, w0);
+    const int all = key_tiles<C::KT>(rblk * ROWS, min(rblk * ROWS + ROWS, len) - 1, len, a.left, a.right, a.sinks, ns, w0);
+    const int first = SPLIT ? wave : 0, nt = (all - first + STEP - 1) / STEP;              // this wave's tiles: first, first + STEP, ...
     const int qlast = min(q0 + 31, len - 1);
-    const Ring ring(base + (a.H + h / (a.H / a.KV)) * HD, a.ld, a.KV * HD, len, wave, lane);
+    const Ring ring(base + (a.H + h / (a.H / a.KV)) * HD, a.ld, a.KV * HD, len, SPLIT ? 0 : wave, lane);
     const TrAt<C, (C::RB < 256)> tr(lane);
     const RowAt<C, (C::RB < 256)> row(lane);
-    const unsigned lds = lds_u32(smem);
-    auto tile = [&](int it) { return it < ns ? it : w0 + it - ns; };
+    unsigned char* own = smem + (SPLIT ? wave * Ring::BYTES : 0);
+    const unsigned lds = lds_u32(own);
+    auto tile = [&](int i) {
+        const int it = first + i * STEP;
+        return it < ns ? it : w0 + it - ns;
+    };
     int fill = 0, use = 0;               // ring positions
-    for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), smem + fill * Ring::STAGE);
+    for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), own + fill * Ring::STAGE);
     fill = Ring::STAGES - 1;
     for (int it = 0; it < nt; ++it) {
-        tile_ready<(Ring::STAGES - 2) * C::NI>(it + Ring::STAGES - 1 > nt);
-        if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), smem + fill * Ring::STAGE);
+        tile_ready<(Ring::STAGES - 2) * C::NI, SPLIT>(it + Ring::STAGES - 1 > nt);
+        if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), own + fill * Ring::STAGE);
         fill = fill + 1 == Ring::STAGES ? 0 : fill + 1;
         const unsigned kl = lds + use * Ring::STAGE, vl = kl + C::TILE;
         use = use + 1 == Ring::STAGES ? 0 : use + 1;
@@ -437,30 +473,50 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_FWD(sizeof(T) * HD)) void 
         if constexpr (C::KB == 2) half(std::integral_constant<int, 1>{});
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
     }
+    l = pair_sum(l);
+    if constexpr (SPLIT) {
+        float* st = reinterpret_cast<float*>(smem);          // [wave][maximum, sum][lane], then join_rows' 16 KiB
+        __syncthreads();
+        st[wave * 128 + lane] = m;
+        st[wave * 128 + 64 + lane] = l;
+        __syncthreads();
+        const float own_m = m;
+        m = fmaxf(fmaxf(st[lane], st[128 + lane]), fmaxf(st[256 + lane], st[384 + lane]));
+        l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float mw = st[w * 128 + lane];
+            l += mw == -INFINITY ? 0.f : st[w * 128 + 64 + lane] * __builtin_amdgcn_exp2f((mw - m) * c);
+        }
+        const float f = own_m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((own_m - m) * c) / l;
+        join_rows<C>(o, f, st + 512, q < len, (T*)a.out + (start + q) * a.H * HD + h * HD, wave, lane);
+        if (q < len && a.lse && h2 == 0 && wave == 0) a.lse[(int64_t)h * a.R + start + q] = m * c + log2f(l);
+        return;
+    }
     if (q < len) {
-        l = pair_sum(l);
         store_rows<T, HD>(o, 1.0f / l, (T*)a.out + (start + q) * a.H * HD + h * HD, h2);
         if (a.lse && h2 == 0) a.lse[(int64_t)h * a.R + start + q] = m * c + log2f(l);
     }
 }
 
 // dQ, the query on the lane; also -delta = -rowsum(dO * O), which the dK/dV kernels launched behind this one read
-template <typename T, int HD>
+template <typename T, int HD, bool SPLIT>
 __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DQ(sizeof(T) * HD)) void window_dq_kernel(WArgs a) {
-    using C = WCfg<T, HD>;
+    using C = RowCfg<T, HD, SPLIT>;
+    constexpr int ROWS = SPLIT ? 32 : WROWS, STEP = SPLIT ? 4 : 1;
     using Ring = KvRing<C>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     int stream, rblk;
-    if (!place(a, a.NB * a.H, a.H / a.KV, stream, rblk)) return;
+    if (!place(a, ROWS, a.NB * a.H, a.H / a.KV, stream, rblk)) return;
     const int h = stream % a.H, b = stream / a.H;
-    rblk = (a.L + WROWS - 1) / WROWS - 1 - rblk;             // the last rows see most: they go first
+    rblk = (a.L + ROWS - 1) / ROWS - 1 - rblk;             // the last rows see most: they go first
     int64_t start;
     const int len = seq_rows(a, b, start);
-    if (rblk * WROWS >= len) return;
+    if (rblk * ROWS >= len) return;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h2 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const T* base = (const T*)a.qkv + start * a.ld;
-    const int q0 = rblk * WROWS + wave * 32, q = q0 + r;
+    const int q0 = rblk * ROWS + (SPLIT ? 0 : wave * 32), q = q0 + r;
     const float c = a.scale * LOG2E;
 
     typename Frag<T>::V qf[C::FR] = {}, gf[C::FR] = {};
@@ -484,7 +540,7 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DQ(sizeof(T) * HD)) void w
     dl = pair_sum(dl);
     if (q < len) {
         ls = a.lse[(int64_t)h * a.R + start + q];
-        if (h2 == 0) a.ndelta[(int64_t)h * a.R + start + q] = -dl;
+        if (h2 == 0 && (!SPLIT || wave == 0)) a.ndelta[(int64_t)h * a.R + start + q] = -dl;
     }
 #pragma unroll
     for (int j = 0; j < C::FR; ++j) {
@@ -497,19 +553,24 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DQ(sizeof(T) * HD)) void w
     for (int db = 0; db < C::DB; ++db) dq[db] = splat16(0.f);
 
     int ns, w0;
-    const int nt = key_tiles<C::KT>(rblk * WROWS, min(rblk * WROWS + WROWS, len) - 1, len, a.left, a.right, a.sinks, ns, w0);
+    const int all = key_tiles<C::KT>(rblk * ROWS, min(rblk * ROWS + ROWS, len) - 1, len, a.left, a.right, a.sinks, ns, w0);
+    const int first = SPLIT ? wave : 0, nt = (all - first + STEP - 1) / STEP;              // this wave's tiles: first, first + STEP, ...
     const int qlast = min(q0 + 31, len - 1);
-    const Ring ring(base + (a.H + h / (a.H / a.KV)) * HD, a.ld, a.KV * HD, len, wave, lane);
+    const Ring ring(base + (a.H + h / (a.H / a.KV)) * HD, a.ld, a.KV * HD, len, SPLIT ? 0 : wave, lane);
     const TrAt<C, (C::RB < 256)> tr(lane);
     const RowAt<C, (C::RB < 256)> row(lane);
-    const unsigned lds = lds_u32(smem);
-    auto tile = [&](int it) { return it < ns ? it : w0 + it - ns; };
+    unsigned char* own = smem + (SPLIT ? wave * Ring::BYTES : 0);
+    const unsigned lds = lds_u32(own);
+    auto tile = [&](int i) {
+        const int it = first + i * STEP;
+        return it < ns ? it : w0 + it - ns;
+    };
     int fill = 0, use = 0;
-    for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), smem + fill * Ring::STAGE);
+    for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), own + fill * Ring::STAGE);
     fill = Ring::STAGES - 1;
     for (int it = 0; it < nt; ++it) {
-        tile_ready<(Ring::STAGES - 2) * C::NI>(it + Ring::STAGES - 1 > nt);
-        if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), smem + fill * Ring::STAGE);
+        tile_ready<(Ring::STAGES - 2) * C::NI, SPLIT>(it + Ring::STAGES - 1 > nt);
+        if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), own + fill * Ring::STAGE);
         fill = fill + 1 == Ring::STAGES ? 0 : fill + 1;
         const unsigned kl = lds + use * Ring::STAGE, vl = kl + C::TILE;
         use = use + 1 == Ring::STAGES ? 0 : use + 1;
@@ -536,6 +597,10 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DQ(sizeof(T) * HD)) void w
         };
         half(std::integral_constant<int, 0>{});
         if constexpr (C::KB == 2) half(std::integral_constant<int, 1>{});
+    }
+    if constexpr (SPLIT) {
+        join_rows<C>(dq, a.scale, reinterpret_cast<float*>(smem), q < len, (T*)a.dqkv + (start + q) * (a.H + 2 * a.KV) * HD + h * HD, wave, lane);
+        return;
     }
     if (q < len) store_rows<T, HD>(dq, a.scale, (T*)a.dqkv + (start + q) * (a.H + 2 * a.KV) * HD + h * HD, h2);
 }
@@ -585,27 +650,28 @@ __device__ __forceinline__ void dkv_block(unsigned ql, unsigned gl, unsigned cst
 
 // dK and dV, the key on the lane: sweeps the queries that see the block's keys, for every query head of the group.  far_parts > 0: the
 // queries that see a sink from beyond the window were done by window_far_kernel, and the sums start from its own.
-template <typename T, int HD> struct DkvCfg {
-    using C = WCfg<T, HD, (sizeof(T) == 2 && HD < 128) ? 64 : 32>;
-    static constexpr int STAGE = 2 * C::TILE + 512, STAGES = STAGE > 20480 ? 2 : 3;      // Q image | dO image | 64 log-sum-exps | 64 row dots
+template <typename T, int HD, bool SPLIT> struct DkvCfg {
+    using C = std::conditional_t<SPLIT, WCfg<T, HD, 32, 1>, WCfg<T, HD, (sizeof(T) == 2 && HD < 128) ? 64 : 32>>;
+    static constexpr int STAGE = 2 * C::TILE + 512, STAGES = SPLIT || STAGE > 20480 ? 2 : 3, BYTES = STAGES * STAGE;      // Q image | dO image | 64 log-sum-exps | 64 row dots
 };
-template <typename T, int HD>
+template <typename T, int HD, bool SPLIT>
 __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DKV(sizeof(T) * HD)) void window_dkv_kernel(WArgs a) {
-    using C = typename DkvCfg<T, HD>::C;
-    constexpr int STAGE = DkvCfg<T, HD>::STAGE, STAGES = DkvCfg<T, HD>::STAGES;
+    using D = DkvCfg<T, HD, SPLIT>;
+    using C = typename D::C;
+    constexpr int STAGE = D::STAGE, STAGES = D::STAGES, ROWS = SPLIT ? 32 : WROWS, STEP = SPLIT ? 4 : 1, NC = SPLIT ? 2 : 1;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     int stream, rblk;
-    if (!place(a, a.NB * a.KV, 1, stream, rblk)) return;
+    if (!place(a, ROWS, a.NB * a.KV, 1, stream, rblk)) return;
     const int hk = stream % a.KV, b = stream / a.KV;
     int64_t start;
     const int len = seq_rows(a, b, start);
-    if (rblk * WROWS >= len) return;
+    if (rblk * ROWS >= len) return;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h2 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rep = a.H / a.KV;
     const T* base = (const T*)a.qkv + start * a.ld;
     const T *kb_ = base + (a.H + hk) * HD, *vb_ = kb_ + a.KV * HD;
-    const int kb0 = rblk * WROWS, k0 = kb0 + wave * 32, key = k0 + r, klast = min(k0 + 31, len - 1);
+    const int kb0 = rblk * ROWS, k0 = kb0 + (SPLIT ? 0 : wave * 32), key = k0 + r, klast = min(k0 + 31, len - 1);
     const int sinks = a.far_parts ? 0 : a.sinks;
     const float c = a.scale * LOG2E;
 
@@ -624,7 +690,7 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DKV(sizeof(T) * HD)) void 
     f32x16_t dk[C::DB], dv[C::DB];
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) dk[db] = dv[db] = splat16(0.f);
-    if (a.far_parts && k0 < min(a.sinks, len)) {
+    if (a.far_parts && k0 < min(a.sinks, len) && (!SPLIT || wave == 0)) {
         const float* w = a.far_ws + ((int64_t)(b * a.KV + hk) * a.far_groups + k0 / 32) * a.far_parts * (2 * C::DB * 1024) + lane;
 #pragma unroll
         for (int db = 0; db < C::DB; ++db)
@@ -638,56 +704,65 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DKV(sizeof(T) * HD)) void 
     for (int db = 0; db < C::DB; ++db) asm volatile("" : "+v"(dk[db]), "+v"(dv[db]));
 
     // queries that see a key of the block: from the first key minus right to the last key plus left, to the end where there are sinks
-    const int qlo = max(0, kb0 - a.right), qhi = kb0 < sinks ? len - 1 : min(len - 1, min(kb0 + WROWS, len) - 1 + a.left);
-    const int t0 = qlo / C::KT, nt = qhi / C::KT - t0 + 1, total = nt * rep;
+    const int qlo = max(0, kb0 - a.right), qhi = kb0 < sinks ? len - 1 : min(len - 1, min(kb0 + ROWS, len) - 1 + a.left);
+    const int t0 = qlo / C::KT, nt = qhi / C::KT - t0 + 1, total = (nt * rep - (SPLIT ? wave : 0) + STEP - 1) / STEP;      // (head, tile) pairs of this wave
     const int64_t gld = (int64_t)a.H * HD;
     const T* gb = (const T*)a.dout + start * gld;
-    const float* cb = ((wave & 1) ? a.ndelta : a.lse) + start;
+    const float* cb = ((wave & 1) ? a.ndelta : a.lse) + start;         // a shared tile's row constants: the waves alternate, too
     unsigned src[C::NI];
 #pragma unroll
     for (int j = 0; j < C::NI; ++j) {       // the waves alternate between the two images: an instruction knows its descriptor
-        const int p = j * 4 + wave;
+        const int p = SPLIT ? j : j * 4 + wave;
         src[j] = piece_src<C>(p >= C::NP ? p - C::NP : p, lane, p >= C::NP ? gld : a.ld);
     }
-    int ft = 0, fh = hk * rep;              // the tile and head to fetch next
+    int ft = SPLIT ? wave % nt : 0, fh = hk * rep + (SPLIT ? wave / nt : 0);              // the tile and head to fetch next
     auto issue = [&](unsigned char* stage) {
         const int64_t row0 = (int64_t)(t0 + ft) * C::KT, left = len - 1 - row0;
         const __amdgpu_buffer_rsrc_t rq = rows_rsrc(base + fh * HD + row0 * a.ld, (left * a.ld + HD) * C::ES);
         const __amdgpu_buffer_rsrc_t rg = rows_rsrc(gb + fh * HD + row0 * gld, (left * gld + HD) * C::ES);
 #pragma unroll
         for (int j = 0; j < C::NI; ++j) {
-            const int p = j * 4 + wave;
+            const int p = SPLIT ? j : j * 4 + wave;
             if (p >= C::NP) dma16(rg, stage + p * 1024, src[j]);
             else dma16(rq, stage + p * 1024, src[j]);
         }
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rows_rsrc(cb + (int64_t)fh * a.R + row0, (left + 1) * 4), (lds_ptr_t)(stage + 2 * C::TILE + (wave & 1) * 256), 4, lane * 4, 0, 0, 0);
-        if (++ft == nt) {
-            ft = 0;
-            ++fh;
+        const int64_t crow = (int64_t)fh * a.R + row0;
+        if constexpr (SPLIT) {
+            dma4(rows_rsrc(a.lse + start + crow, (left + 1) * 4), stage + 2 * C::TILE, lane * 4);
+            dma4(rows_rsrc(a.ndelta + start + crow, (left + 1) * 4), stage + 2 * C::TILE + 256, lane * 4);
+        } else {
+            dma4(rows_rsrc(cb + crow, (left + 1) * 4), stage + 2 * C::TILE + (wave & 1) * 256, lane * 4);
         }
+        for (ft += STEP; ft >= nt; ft -= nt) ++fh;
     };
     const TrAt<C, (C::RB < 256)> tr(lane);
     const RowAt<C, (C::RB < 256)> rows(lane);
-    const unsigned lds = lds_u32(smem);
-    int fill = 0, use = 0, ct = 0;
-    for (; fill < STAGES - 1 && fill < total; ++fill) issue(smem + fill * STAGE);
+    unsigned char* own = smem + (SPLIT ? wave * D::BYTES : 0);
+    const unsigned lds = lds_u32(own);
+    int fill = 0, use = 0, ct = SPLIT ? wave % nt : 0;
+    for (; fill < STAGES - 1 && fill < total; ++fill) issue(own + fill * STAGE);
     fill = STAGES - 1;
     for (int it = 0; it < total; ++it) {
-        tile_ready<(STAGES - 2) * (C::NI + 1)>(it + STAGES - 1 > total);
-        if (it + STAGES - 1 < total) issue(smem + fill * STAGE);
+        tile_ready<(STAGES - 2) * (C::NI + NC), SPLIT>(it + STAGES - 1 > total);
+        if (it + STAGES - 1 < total) issue(own + fill * STAGE);
         fill = fill + 1 == STAGES ? 0 : fill + 1;
         const unsigned ql = lds + use * STAGE, gl = ql + C::TILE;
         use = use + 1 == STAGES ? 0 : use + 1;
         const int q0 = (t0 + ct) * C::KT, q1 = q0 + C::KT - 1;
-        ct = ct + 1 == nt ? 0 : ct + 1;
+        for (ct += STEP; ct >= nt;) ct -= nt;
         if (k0 >= len || q1 < k0 - a.right || (q0 > klast + a.left && k0 >= sinks)) continue;
         const bool whole = q1 < len && q0 >= klast - a.right && (q1 <= k0 + a.left || klast < sinks);
         const int first = key - a.right - q0, last = (key < sinks ? len - 1 : min(len - 1, key + a.left)) - q0;
         dkv_block<C, 0>(ql, gl, gl + C::TILE, rows, kf, vf, c, whole, first, last, tr, dk, dv, h2);
         if constexpr (C::KB == 2) dkv_block<C, 32>(ql, gl, gl + C::TILE, rows, kf, vf, c, whole, first, last, tr, dk, dv, h2);
     }
+    T* row = (T*)a.dqkv + (start + key) * (a.H + 2 * a.KV) * HD + (a.H + hk) * HD;
+    if constexpr (SPLIT) {
+        join_rows<C>(dk, a.scale, reinterpret_cast<float*>(smem), key < len, row, wave, lane);
+        join_rows<C>(dv, 1.0f, reinterpret_cast<float*>(smem), key < len, row + a.KV * HD, wave, lane);
+        return;
+    }
     if (key < len) {
-        T* row = (T*)a.dqkv + (start + key) * (a.H + 2 * a.KV) * HD + (a.H + hk) * HD;
         store_rows<T, HD>(dk, a.scale, row, h2);
         store_rows<T, HD>(dv, 1.0f, row + a.KV * HD, h2);
     }
@@ -810,24 +885,72 @@ template <void (*KERNEL)(WArgs)> static int launch(const char* who, int64_t bloc
     STAR_LAUNCH_CHECK(who);
     return 0;
 }
-static int64_t grid_of(const WArgs& a, int heads) {
+static int64_t grid_of(const WArgs& a, int rows, int heads) {
     const int64_t streams = (int64_t)a.NB * heads;
-    return (dealt(a.offsets, (int)streams) ? cdiv(streams, 8) * 8 : streams) * cdiv(a.L, WROWS);
+    return (dealt(a.offsets, (int)streams) ? cdiv(streams, 8) * 8 : streams) * cdiv(a.L, rows);
+}
+// Split form or row form, by the 128-row blocks that the row form would have, in eighths of the compute units.  Below the limits the split form
+// was faster, above them the row form (1024 rows, 8 .. 80 heads, windows 64 and 512, forward in us, split / row: hd 32 10.5 / 12.0 at 256 blocks
+// and 15.4 / 15.7 at 448; hd 64 9.2 / 13.8 at 128, 13.8 / 14.2 at 192, 26.1 / 19.2 at 448; hd 128 10.1 / 17.1 at 64, 18.2 / 18.0 at 128; float32 hd 32
+// 29.5 / 35.5 at 256, hd 64 34.8 / 57.2 at 128, 61.3 / 58.4 at 256).  dK/dV has a longer sweep per block, over every head of a group: its limits lie
+// higher (dK/dV + dQ, 4 heads a group, window 256: hd 128 44.6 / 95.7 at 64 blocks, 120 / 131 at 160; hd 64 55 / 69 at 160).
+template <typename T, int HD> struct SplitUpTo {
+    static constexpr int RB = HD * sizeof(T);
+    static constexpr bool EVER = RB <= 256;                  // wider rows: four rings do not fit into LDS
+    static constexpr int ROWS = sizeof(T) == 2 ? (RB <= 64 ? 10 : RB <= 128 ? 4 : 3) : (RB <= 128 ? 10 : 5);
+    static constexpr int KEYS = sizeof(T) == 2 ? (RB <= 64 ? 12 : RB <= 128 ? 8 : 5) : (RB <= 128 ? 20 : 12);
+};
+static bool few_blocks(const WArgs& a, int heads, int eighths) {
+    const int64_t blocks = (a.offsets ? cdiv(a.R, WROWS) : (int64_t)a.NB * cdiv(a.L, WROWS)) * (int64_t)heads;
+    return blocks * 8 <= (int64_t)eighths * star_num_cus();
+}
+template <typename T, int HD, bool SPLIT> static int launch_fwd(const WArgs& a, hipStream_t s) {
+    using Ring = KvRing<RowCfg<T, HD, SPLIT>>;
+    constexpr int LDS = SPLIT ? 4 * Ring::BYTES : Ring::BYTES;
+    return launch<window_fwd_kernel<T, HD, SPLIT>>("star_attn_window_fwd", grid_of(a, SPLIT ? 32 : WROWS, a.H), SPLIT && LDS < 18432 ? 18432 : LDS, a, s);
+}
+template <typename T, int HD, bool SPLIT> static int launch_dq(const WArgs& a, hipStream_t s) {
+    using Ring = KvRing<RowCfg<T, HD, SPLIT>>;
+    constexpr int LDS = SPLIT ? 4 * Ring::BYTES : Ring::BYTES;
+    return launch<window_dq_kernel<T, HD, SPLIT>>("star_attn_window_bwd", grid_of(a, SPLIT ? 32 : WROWS, a.H), SPLIT && LDS < 16384 ? 16384 : LDS, a, s);
+}
+template <typename T, int HD, bool SPLIT> static int launch_dkv(const WArgs& a, hipStream_t s) {
+    using D = DkvCfg<T, HD, SPLIT>;
+    constexpr int LDS = SPLIT ? 4 * D::BYTES : D::BYTES;
+    return launch<window_dkv_kernel<T, HD, SPLIT>>("star_attn_window_bwd", grid_of(a, SPLIT ? 32 : WROWS, a.KV), SPLIT && LDS < 16384 ? 16384 : LDS, a, s);
 }
 template <typename T, int HD> static int run_fwd(const WArgs& a, hipStream_t s) {
-    return launch<window_fwd_kernel<T, HD>>("star_attn_window_fwd", grid_of(a, a.H), KvRing<WCfg<T, HD>>::STAGES * KvRing<WCfg<T, HD>>::STAGE, a, s);
+    using S = SplitUpTo<T, HD>;
+    if constexpr (S::EVER)
+        if (few_blocks(a, a.H, S::ROWS)) return launch_fwd<T, HD, true>(a, s);
+    return launch_fwd<T, HD, false>(a, s);
+}
+template <typename T, int HD> static int run_dq(const WArgs& a, hipStream_t s) {
+    using S = SplitUpTo<T, HD>;
+    if constexpr (S::EVER)
+        if (few_blocks(a, a.H, S::ROWS)) return launch_dq<T, HD, true>(a, s);
+    return launch_dq<T, HD, false>(a, s);
+}
+template <typename T, int HD> static int run_dkv(const WArgs& a, hipStream_t s) {
+    using S = SplitUpTo<T, HD>;
+    if constexpr (S::EVER)
+        if (few_blocks(a, a.KV, S::KEYS)) return launch_dkv<T, HD, true>(a, s);
+    return launch_dkv<T, HD, false>(a, s);
 }
 template <typename T, int HD> static int run_bwd(const WArgs& a, hipStream_t s) {
     const char* who = "star_attn_window_bwd";
-    if (int rc = launch<window_dq_kernel<T, HD>>(who, grid_of(a, a.H), KvRing<WCfg<T, HD>>::STAGES * KvRing<WCfg<T, HD>>::STAGE, a, s)) return rc;
+    int rc = run_dq<T, HD>(a, s);
+    if (rc) return rc;
     if (a.far_parts) {
         constexpr int FAR_LDS = 4 * (2 * WCfg<T, HD, 32>::TILE + 512);
         const int lists = a.NB * a.KV * a.far_groups, size = 2 * WCfg<T, HD>::DB * 1024;
-        if (int rc = launch<window_far_kernel<T, HD>>(who, (int64_t)lists * a.far_parts, FAR_LDS < 16384 ? 16384 : FAR_LDS, a, s)) return rc;
-        hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, lists), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
-        STAR_LAUNCH_CHECK(who);
+        if ((rc = launch<window_far_kernel<T, HD>>(who, (int64_t)lists * a.far_parts, FAR_LDS < 16384 ? 16384 : FAR_LDS, a, s))) return rc;
+        if (a.far_parts > 1) {
+            hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, lists), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
+            STAR_LAUNCH_CHECK(who);
+        }
     }
-    return launch<window_dkv_kernel<T, HD>>(who, grid_of(a, a.KV), DkvCfg<T, HD>::STAGES * DkvCfg<T, HD>::STAGE, a, s);
+    return run_dkv<T, HD>(a, s);
 }
 
 // How the far queries of the sinks are cut: about two blocks of four waves per compute unit in all, no more than 16 parts to add up, and at least
@@ -859,7 +982,7 @@ static int window_args(const char* who, const StarAttnWindow* g, WArgs& a) {
                "%s: qkv rows of %lld elements must hold all heads and be 16-byte aligned", who, (long long)g->ld);
     STAR_CHECK(g->ld * es < (1 << 24), "%s: qkv rows %lld elements apart", who, (long long)g->ld);       // a tile's offsets are 32 bits
     STAR_CHECK((uintptr_t)g->out % 16 == 0, "%s: out must be 16-byte aligned", who);
-    STAR_CHECK((int64_t)cdiv(g->L, WROWS) * ((int64_t)g->H * g->NB + 7) < (1ll << 31), "%s: NB, H, L too large for the grid", who);
+    STAR_CHECK((int64_t)cdiv(g->L, 32) * ((int64_t)g->H * g->NB + 7) < (1ll << 31), "%s: NB, H, L too large for the grid", who);
     // a bound over L says the same as L: what is left cannot overflow in i + right and i - left
     a = WArgs{g->qkv, g->offsets, g->out, g->lse, nullptr, nullptr, nullptr, nullptr, g->ld, g->R, g->NB, g->L, g->H, g->KV,
               g->left < g->L ? g->left : g->L, g->right < g->L ? g->right : g->L, g->sinks < g->L ? g->sinks : g->L, g->scale, 0, 0};

@@ -56,6 +56,47 @@ def test_window_attention_against_float64(dtype, hd, window):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("window", WINDOWS)
+def test_many_sequences(dtype, hd, window):
+    """enough heads and sequences that four waves share a block's tiles (fewer: each wave sweeps its own part): three of them against float64"""
+    left, right, sinks = window
+    g = _gen(hd + sinks + 1)
+    n, h, nb = 161, 12, 40
+    qkv, dout = _rand(g, nb * n, 3 * h * hd, dtype=dtype, mul=1.3), _rand(g, nb * n, h * hd, dtype=dtype)
+    kw = dict(left=left, right=right, sinks=sinks)
+    out, lse = ops.attn_window_fwd(qkv, nb, n, h, hd, **kw)
+    dqkv = ops.attn_window_bwd(qkv, out, dout, lse, nb, n, h, hd, **kw)
+    for b in (0, 17, nb - 1):
+        rows = slice(b * n, (b + 1) * n)
+        q, k, v = unpack(qkv[rows], h, h, hd)
+        want = reference(q, k, v, left, right, sinks, None, heads(dout[rows], hd), dtype)
+        assert_within(heads(out[rows], hd), want["out"], want["tol_out"], "out %d" % b)
+        assert_within(lse[:, rows].cpu().double(), want["lse"], want["tol_lse"], "lse %d" % b)
+        assert_within(heads(dqkv[rows], hd), want["dqkv"], want["tol_dqkv"], "dqkv %d" % b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,rep", [(32, 2), (64, 4), (128, 3)])
+def test_many_ragged_sequences_with_shared_heads(dtype, hd, rep):
+    g = _gen(hd * rep)
+    lens = [0, 300, 1, 64, 129, 31, 257, 500, 128, 2] * 6
+    kv = 8
+    h = kv * rep
+    qkv, dout = _rand(g, sum(lens) + 3, (h + 2 * kv) * hd, dtype=dtype), _rand(g, sum(lens) + 3, h * hd, dtype=dtype)
+    offsets = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], device=DEV)
+    kw = dict(kv_heads=kv, left=70, right=9, sinks=5, offsets=offsets)
+    out, lse = ops.attn_window_fwd(qkv, len(lens), 500, h, hd, **kw)
+    dqkv = ops.attn_window_bwd(qkv, out, dout, lse, len(lens), 500, h, hd, **kw)
+    for b in (1, 3, 6, 57, 58, 59):
+        rows = slice(sum(lens[:b]), sum(lens[:b + 1]))
+        q, k, v = unpack(qkv[rows], h, kv, hd)
+        want = reference(q, k, v, 70, 9, 5, None, heads(dout[rows], hd), dtype)
+        assert_within(heads(out[rows], hd), want["out"], want["tol_out"], "out %d" % b)
+        assert_within(heads(dqkv[rows], hd), want["dqkv"], want["tol_dqkv"], "dqkv %d" % b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n", [2, 31, 32, 63, 64, 65, 127, 128, 257, 512])
 def test_every_tile_border(dtype, n):
     g = _gen(n)
