@@ -280,7 +280,7 @@ typedef struct StarAttnStep {
     float scale;
     int32_t dt;
 } StarAttnStep;
-int64_t star_attn_window_step_ws(int NB, int H, int KV, int hd, int cap, int left, int sinks);
+int64_t star_attn_window_step_ws(int NB, int H, int KV, int hd, int cap, int left, int sinks, int dt);
 int star_attn_window_step(const StarAttnStep* g, void* stream);
 
 /* ---- K1: voxel -> patch gather ------------------------------------------------------------------------

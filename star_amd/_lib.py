@@ -81,7 +81,7 @@ _SIGS = {
     "star_attn_window_bwd_ws": (C.c_int64, [_L, _I, _I, _I, _I, _I, _I, _I]),
     "star_attn_window_bwd": (C.c_int, [C.POINTER(StarAttnWindow), _P]),
     "star_kv_append": (C.c_int, [_P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
-    "star_attn_window_step_ws": (C.c_int64, [_I, _I, _I, _I, _I, _I, _I]),
+    "star_attn_window_step_ws": (C.c_int64, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "star_attn_window_step": (C.c_int, [C.POINTER(StarAttnStep), _P]),
     "star_gemm_res_ln_supported": (C.c_int, [_I, _I, _I]),
     "star_gemm_res_ln_prefers": (C.c_int, [_I, _I, _I, _I]),

@@ -109,9 +109,9 @@ struct Seen {
 // One block: G query heads of one key head of one sequence over one split of the visible tokens.  A row's 16-byte chunks lie on LPR lanes;
 // every group of LPR lanes walks its own rows, U at a time, with its own running maximum and sum (no exchange but the dot products'); the
 // groups are joined once at the end.  The split that owns the newest token puts it into the cache first, and reads it from there.
-template <typename T, int HD, int G>
-__global__ __launch_bounds__(KT_) void step_kernel(StepArgs a) {
-    constexpr int ES = sizeof(T), E = 16 / ES, LPR = HD / E, RPB = KT_ / LPR, U = 4, NW = KT_ / 64;
+template <typename T, int HD, int G, int NT>
+__global__ __launch_bounds__(NT) void step_kernel(StepArgs a) {
+    constexpr int ES = sizeof(T), E = 16 / ES, LPR = HD / E, RPB = NT / LPR, U = 4, NW = NT / 64;
     __shared__ float sq[G][HD];
     __shared__ float so[NW][G][HD];
     __shared__ float sm[NW][G], sl[NW][G];
@@ -121,7 +121,10 @@ __global__ __launch_bounds__(KT_) void step_kernel(StepArgs a) {
     const int rep = a.H / a.KV, h0 = hk * rep + gc * G, ng = min(G, rep - gc * G);
     const int len = max(0, a.lengths[b]);
     const Seen seen(len, a.left, a.sinks, a.cap);
-    const int per = (seen.vis + a.splits - 1) / a.splits, v0 = split * per, v1 = min(seen.vis, v0 + per);
+    constexpr int ROUND = RPB * U;
+    const int per = ((seen.vis + a.splits - 1) / a.splits + ROUND - 1) / ROUND * ROUND;          // whole rounds
+    const int64_t begin = (int64_t)split * per;
+    const int v0 = (int)(begin < seen.vis ? begin : seen.vis), v1 = min(seen.vis, v0 + per);
     const bool owner = v1 == seen.vis && v0 < v1;
     const T* row = (const T*)a.qkv + b * a.ld;
     T* kc = (T*)a.cache + ((int64_t)b * a.KV + hk) * a.cap * HD;
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(KT_) void step_kernel(StepArgs a) {
     // rotate the query heads (and, in the owner, the key) once: items = pairs of the rotated part, then single elements of the rest
     const int n = a.f.pairs, rest = HD - 2 * n, items = n + rest;
     const int newest = owner ? seen.slot(seen.vis - 1) : 0;
-    for (int i = tid; i < (ng + (owner ? 1 : 0)) * items; i += KT_) {
+    for (int i = tid; i < (ng + (owner ? 1 : 0)) * items; i += NT) {
         const int g = i / items, k = i % items;
         const T* src = row + (g < ng ? h0 + g : a.H + hk) * HD;
         T* kd = kc + (int64_t)newest * HD;
@@ -155,7 +158,7 @@ __global__ __launch_bounds__(KT_) void step_kernel(StepArgs a) {
         }
     }
     if (owner)
-        for (int d = tid; d < HD; d += KT_) vc[(int64_t)newest * HD + d] = row[(a.H + a.KV + hk) * HD + d];
+        for (int d = tid; d < HD; d += NT) vc[(int64_t)newest * HD + d] = row[(a.H + a.KV + hk) * HD + d];
     __syncthreads();
 
     const int grp = tid / LPR, ch = tid % LPR;
@@ -170,7 +173,7 @@ __global__ __launch_bounds__(KT_) void step_kernel(StepArgs a) {
             o[g][e] = 0.f;
         }
     }
-    for (int vb = v0; vb < v1; vb += RPB * U) {
+    for (int vb = v0; vb < v1; vb += ROUND) {
         uint4 kw[U], vw[U];
         bool ok[U];
 #pragma unroll
@@ -248,7 +251,7 @@ __global__ __launch_bounds__(KT_) void step_kernel(StepArgs a) {
         }
     }
     __syncthreads();
-    for (int i = tid; i < ng * HD; i += KT_) {
+    for (int i = tid; i < ng * HD; i += NT) {
         const int g = i / HD, d = i % HD;
         float mn = sm[0][g];
 #pragma unroll
@@ -323,36 +326,55 @@ extern "C" int star_kv_append(const void* qkv, int64_t ld, const int64_t* offset
     return 0;
 }
 
-// query heads of a key head that one block serves (they share every row it reads)
-static int step_group(int rep) { return rep > 4 ? 8 : rep > 2 ? 4 : rep; }
-// few (sequence, key head) pairs leave the chip idle and one block's loads cannot fill it: the visible tokens are split until there are
-// about four blocks per compute unit, but no split gets under 64 tokens
-static int step_splits(int NB, int H, int KV, int cap, int left, int sinks) {
+// Query heads of a key head that one block serves: they share every row it reads, but its one or two rounds of rows cost the more arithmetic.  More
+// than two only where the key heads alone fill the chip (1 sequence, 32 heads of 128 on 8, 1000 tokens: 14.4 us with four, 11.8 with two; 16 x 8 heads of
+// 64 on 1, 2000 tokens: 19.8 with eight, 14.3 with four, 13.4 with two; 8 x 32 on 8, 4096 tokens: 37.1 with four, 33.6 with two, 83.6 with one).
+static int step_group(int NB, int H, int KV) {
     const int rep = H / KV;
-    const int64_t blocks = (int64_t)NB * KV * cdiv(rep, step_group(rep));
+    if ((int64_t)NB * KV < star_num_cus()) return rep > 1 ? 2 : 1;
+    return rep > 4 ? 8 : rep > 2 ? 4 : rep;
+}
+// Threads of a block and splits.  Where there is a block per compute unit, or two rounds of a wide block take all rows, a wide block takes the
+// whole sequence: one launch (5 sequences, 12 heads of 64, 300 visible tokens 6.9 us against 8.2 with narrow blocks, splits and their join; 32 x 8 heads of 128, 500
+// tokens 21 against 25).  Else few (sequence, key head) pairs would leave the chip idle: narrow blocks, the tokens split until there are about
+// four of them per compute unit (8 heads of 128, 4096 tokens 25 us against 70).
+struct StepPlan {
+    int threads, splits;
+};
+static StepPlan step_plan(int NB, int H, int KV, int hd, int es, int cap, int left, int sinks) {
+    const int rep = H / KV, G = step_group(NB, H, KV), wide = G == 8 ? 512 : 1024;
+    const int64_t blocks = (int64_t)NB * KV * cdiv(rep, G);
     const int64_t vis = (int64_t)left + 1 + sinks < cap ? (int64_t)left + 1 + sinks : cap;
+    const int per = 4 * 64 / (hd * es / 16);              // rows of a wave's round
+    if (blocks >= star_num_cus() || vis <= 2 * per * (wide / 64)) return {wide, 1};
+    const int64_t rounds = (vis + per * 4 - 1) / (per * 4);
     int64_t s = (4 * (int64_t)star_num_cus() + blocks - 1) / blocks;
-    if (s > vis / 64) s = vis / 64;
-    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+    if (s > rounds) s = rounds;
+    return {KT_, (int)(s < 1 ? 1 : s > 64 ? 64 : s)};
 }
 
-extern "C" int64_t star_attn_window_step_ws(int NB, int H, int KV, int hd, int cap, int left, int sinks) {
-    if (NB <= 0 || H <= 0 || KV <= 0 || H % KV || hd <= 0 || cap <= 0 || left < 0 || sinks < 0) return 0;
-    const int s = step_splits(NB, H, KV, cap, left, sinks);
+extern "C" int64_t star_attn_window_step_ws(int NB, int H, int KV, int hd, int cap, int left, int sinks, int dt) {
+    if (NB <= 0 || H <= 0 || KV <= 0 || H % KV || hd < 16 || hd > 128 || cap <= 0 || left < 0 || sinks < 0) return 0;
+    const int s = step_plan(NB, H, KV, hd, dt == STAR_BF16 ? 2 : 4, cap, left, sinks).splits;
     return s == 1 ? 0 : (int64_t)NB * H * s * (hd + 2);
 }
 
-template <typename T, int HD> static void step_launch(const StepArgs& a, int G, dim3 grid, hipStream_t s) {
-    if (G == 1) hipLaunchKernelGGL((step_kernel<T, HD, 1>), grid, dim3(KT_), 0, s, a);
-    else if (G == 2) hipLaunchKernelGGL((step_kernel<T, HD, 2>), grid, dim3(KT_), 0, s, a);
-    else if (G == 4) hipLaunchKernelGGL((step_kernel<T, HD, 4>), grid, dim3(KT_), 0, s, a);
-    else hipLaunchKernelGGL((step_kernel<T, HD, 8>), grid, dim3(KT_), 0, s, a);
+template <typename T, int HD, int G> static void step_launch(const StepArgs& a, int threads, dim3 grid, hipStream_t s) {
+    constexpr int WIDE = G == 8 ? 512 : 1024;
+    if (threads == WIDE) hipLaunchKernelGGL((step_kernel<T, HD, G, WIDE>), grid, dim3(WIDE), 0, s, a);
+    else hipLaunchKernelGGL((step_kernel<T, HD, G, KT_>), grid, dim3(KT_), 0, s, a);
 }
-template <typename T> static void step_run(const StepArgs& a, int hd, int G, dim3 grid, hipStream_t s) {
-    if (hd == 16) step_launch<T, 16>(a, G, grid, s);
-    else if (hd == 32) step_launch<T, 32>(a, G, grid, s);
-    else if (hd == 64) step_launch<T, 64>(a, G, grid, s);
-    else step_launch<T, 128>(a, G, grid, s);
+template <typename T, int HD> static void step_heads(const StepArgs& a, int G, int threads, dim3 grid, hipStream_t s) {
+    if (G == 1) step_launch<T, HD, 1>(a, threads, grid, s);
+    else if (G == 2) step_launch<T, HD, 2>(a, threads, grid, s);
+    else if (G == 4) step_launch<T, HD, 4>(a, threads, grid, s);
+    else step_launch<T, HD, 8>(a, threads, grid, s);
+}
+template <typename T> static void step_run(const StepArgs& a, int hd, int G, int threads, dim3 grid, hipStream_t s) {
+    if (hd == 16) step_heads<T, 16>(a, G, threads, grid, s);
+    else if (hd == 32) step_heads<T, 32>(a, G, threads, grid, s);
+    else if (hd == 64) step_heads<T, 64>(a, G, threads, grid, s);
+    else step_heads<T, 128>(a, G, threads, grid, s);
     if (a.splits > 1)
         hipLaunchKernelGGL(step_join_kernel<T>, dim3(cdiv((int64_t)a.NB * a.H, KT_ / 64)), dim3(KT_), 0, s, a.ws, (T*)a.out, a.NB * a.H, hd, a.splits);
 }
@@ -378,15 +400,16 @@ extern "C" int star_attn_window_step(const StarAttnStep* g, void* stream) {
             STAR_CHECK(g->h_rope->axis[i] < g->h_rope->axes, "star_attn_window_step: pair %d turns by axis %d of %d", i, g->h_rope->axis[i], g->h_rope->axes);
         a.f = *g->h_rope;
     }
-    const int rep = g->H / g->KV, G = step_group(rep);
+    const int rep = g->H / g->KV, G = step_group(g->NB, g->H, g->KV);
     a.chunks = cdiv(rep, G);
-    a.splits = step_splits(g->NB, g->H, g->KV, g->cap, g->left, g->sinks);
+    const StepPlan plan = step_plan(g->NB, g->H, g->KV, g->hd, es, g->cap, g->left, g->sinks);
+    a.splits = plan.splits;
     STAR_CHECK(a.splits == 1 || g->ws, "star_attn_window_step: null workspace (star_attn_window_step_ws)");
     const int64_t blocks = (int64_t)g->NB * g->KV * a.chunks * a.splits;
     STAR_CHECK(blocks < (1ll << 31), "star_attn_window_step: NB, KV too large for the grid");
     hipStream_t s = (hipStream_t)stream;
-    if (g->dt == STAR_BF16) step_run<bf16_t>(a, g->hd, G, dim3((unsigned)blocks), s);
-    else step_run<float>(a, g->hd, G, dim3((unsigned)blocks), s);
+    if (g->dt == STAR_BF16) step_run<bf16_t>(a, g->hd, G, plan.threads, dim3((unsigned)blocks), s);
+    else step_run<float>(a, g->hd, G, plan.threads, dim3((unsigned)blocks), s);
     STAR_LAUNCH_CHECK("star_attn_window_step");
     return 0;
 }

@@ -593,10 +593,11 @@ def _window_step(home, qkv, cache, lengths, h, left, sinks, pos, sections, base,
         lib = L.lib()
         if left is None:
             left = cap - sinks - 1
-        need = lib.star_attn_window_step_ws(nb, h, kv, hd, cap, left, sinks)
+        dt = L.dt_of(qkv)
+        need = lib.star_attn_window_step_ws(nb, h, kv, hd, cap, left, sinks, dt)
         ws = qkv.new_empty(need, dtype=torch.float32) if need else None
         g = L.StarAttnStep(qkv.data_ptr(), cache.data_ptr(), lengths.data_ptr(), None, None, out.data_ptr(), None if ws is None else ws.data_ptr(), ld, 0, nb, h, kv,
-                           hd, cap, left, sinks, hd ** -0.5 if scale is None else scale, L.dt_of(qkv))
+                           hd, cap, left, sinks, hd ** -0.5 if scale is None else scale, dt)
         if sections is not None:
             plan = rope_plan(tuple(sections), base, per_axis, interleaved)
             pos, g.pos_ld = _positions(pos, plan.axes, nb)
