@@ -255,7 +255,7 @@ typedef struct StarAttnWindow {
     int32_t dt;
 } StarAttnWindow;
 int star_attn_window_fwd(const StarAttnWindow* g, void* stream);
-int64_t star_attn_window_bwd_ws(int64_t R, int NB, int L, int H, int KV, int hd, int left, int sinks);
+int64_t star_attn_window_bwd_ws(int64_t R, int NB, int L, int H, int KV, int hd, int left, int sinks, int dt);
 int star_attn_window_bwd(const StarAttnWindow* g, void* stream);
 /* Rolling cache dt [2 (keys, values), NB, KV, cap, hd]: the token at position p lies in slot p for p < sinks, else in slot
  * sinks + (p - sinks) % (cap - sinks).  lengths int32 [NB]: the sequence's tokens INCLUDING the new ones.

@@ -78,7 +78,7 @@ _SIGS = {
     "star_attn_bwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "star_rope": (C.c_int, [_P, _L, _P, _L, _P, _L, C.POINTER(StarRope), _I, _I, _I, _I, _I, _I, _P]),
     "star_attn_window_fwd": (C.c_int, [C.POINTER(StarAttnWindow), _P]),
-    "star_attn_window_bwd_ws": (C.c_int64, [_L, _I, _I, _I, _I, _I, _I, _I]),
+    "star_attn_window_bwd_ws": (C.c_int64, [_L, _I, _I, _I, _I, _I, _I, _I, _I]),
     "star_attn_window_bwd": (C.c_int, [C.POINTER(StarAttnWindow), _P]),
     "star_kv_append": (C.c_int, [_P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "star_attn_window_step_ws": (C.c_int64, [_I, _I, _I, _I, _I, _I, _I, _I]),

@@ -30,6 +30,9 @@ typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 #define WAVES_FWD(B) ((B) >= 512 ? 1 : (B) >= 256 ? 2 : 4)
 #define WAVES_DQ(B) ((B) >= 512 ? 1 : (B) >= 256 ? 2 : (B) >= 128 ? 3 : 4)
 #define WAVES_DKV(B) ((B) >= 512 ? 1 : (B) >= 128 ? 2 : 3)
+// (Waves with rings of their own take up the LDS of a compute unit from row bytes of 256 on: one block of them, one wave on a SIMD.  float32 split
+// forms are 3 to 5 % faster within half of its registers all the same.)
+#define WAVES_OWN(N, B, OWN) ((OWN) && (B) >= 256 ? 1 : (N))
 #define WAVES_PER_SIMD(N) __attribute__((amdgpu_waves_per_eu(N, N)))
 #define LOG2E 1.4426950408889634f
 #define RESCALE_TH 8.0f           // log2 units: the reference maximum is raised only when a row exceeds it by 2^8 (float32 sums: no loss)
@@ -246,13 +249,6 @@ __device__ __forceinline__ float pair_sum(float v) {
     const u2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(x[0]) + __uint_as_float(x[1]);
 }
-// orders a wave's own LDS writes and reads (its lanes exchange data without a block barrier)
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // [d][32 lanes' rows] accumulator -> a row of T per lane (both halves of a lane pair hold parts of the same row)
 template <typename T, int HD> __device__ __forceinline__ void store_rows(const f32x16_t (&acc)[WCfg<T, HD>::DB], float mul, T* __restrict__ row, int h2) {
 #pragma unroll
@@ -352,27 +348,31 @@ template <class C> struct KvRing {
 // Split form: the four waves of a block work on the same 32 rows (dK/dV: keys), each on every fourth tile with a ring of its own, and are added up
 // through LDS, in their order, when all are done.  For launches whose row form (a wave per 32 rows, four sharing the tiles) leaves most of the
 // chip idle (SplitUpTo).
-// mul * sum of the waves' accumulators -> the lane's row: a wave adds and stores four of the sixteen registers of every block.
+// Sum of the waves' accumulator block, in their order: a wave gets four of the sixteen registers, 4 wave .. 4 wave + 3.
+__device__ __forceinline__ void join_block(const f32x16_t& acc, float mul, float* sum, float (&v)[4], int wave, int lane) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum[(wave * 16 + e) * 64 + lane] = acc[e] * mul;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int at = (wave * 4 + e) * 64 + lane;
+        v[e] = (sum[at] + sum[1024 + at]) + (sum[2048 + at] + sum[3072 + at]);
+    }
+}
+// mul * sum of the waves' accumulators -> the lane's row
 template <class C> __device__ __forceinline__ void join_rows(const f32x16_t (&acc)[C::DB], float mul, float* sum, bool valid, typename C::Type* row, int wave, int lane) {
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) {
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sum[(wave * 16 + e) * 64 + lane] = acc[db][e] * mul;
-        __syncthreads();
         float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int at = (wave * 4 + e) * 64 + lane;
-            v[e] = (sum[at] + sum[1024 + at]) + (sum[2048 + at] + sum[3072 + at]);
-        }
+        join_block(acc[db], mul, sum, v, wave, lane);
         const int d = db * 32 + 8 * wave + 4 * (lane >> 5);
         if (valid && d < C::HDIM) st4(row + d, v);
     }
 }
 
 template <typename T, int HD, bool SPLIT>
-__global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_FWD(sizeof(T) * HD)) void window_fwd_kernel(WArgs a) {
+__global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_FWD(sizeof(T) * HD), sizeof(T) * HD, SPLIT && sizeof(T) == 2)) void window_fwd_kernel(WArgs a) {
     using C = RowCfg<T, HD, SPLIT>;
     constexpr int ROWS = SPLIT ? 32 : WROWS, STEP = SPLIT ? 4 : 1;
     using Ring = KvRing<C>;
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_FWD(sizeof(T) * HD)) void 
 
 // dQ, the query on the lane; also -delta = -rowsum(dO * O), which the dK/dV kernels launched behind this one read
 template <typename T, int HD, bool SPLIT>
-__global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DQ(sizeof(T) * HD)) void window_dq_kernel(WArgs a) {
+__global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DQ(sizeof(T) * HD), sizeof(T) * HD, SPLIT && sizeof(T) == 2)) void window_dq_kernel(WArgs a) {
     using C = RowCfg<T, HD, SPLIT>;
     constexpr int ROWS = SPLIT ? 32 : WROWS, STEP = SPLIT ? 4 : 1;
     using Ring = KvRing<C>;
@@ -648,37 +648,48 @@ __device__ __forceinline__ void dkv_block(unsigned ql, unsigned gl, unsigned cst
     mma_tr<C, BLK>(ql, tr, Block<T>(dp), dk);
 }
 
-// dK and dV, the key on the lane: sweeps the queries that see the block's keys, for every query head of the group.  far_parts > 0: the
-// queries that see a sink from beyond the window were done by window_far_kernel, and the sums start from its own.
-template <typename T, int HD, bool SPLIT> struct DkvCfg {
-    using C = std::conditional_t<SPLIT, WCfg<T, HD, 32, 1>, WCfg<T, HD, (sizeof(T) == 2 && HD < 128) ? 64 : 32>>;
-    static constexpr int STAGE = 2 * C::TILE + 512, STAGES = SPLIT || STAGE > 20480 ? 2 : 3, BYTES = STAGES * STAGE;      // Q image | dO image | 64 log-sum-exps | 64 row dots
+// dK and dV, the key on the lane: sweeps the queries that see the block's keys, for every query head of the group.
+// FAR_FORM: the part that reaches the sinks from queries beyond the window (i > j + left): few keys, all queries of the sequence.  Left to the
+// other forms, the block with the sinks would sweep the whole sequence while the rest is long done (backward of 7 sequences of 0 .. 2043 rows,
+// one sink: 540 us with, 180 without).  A block takes 32 sinks and every far_parts-th four (head, tile) pairs, and leaves its waves' sum in
+// far_ws; with far_parts > 0 the other forms' sums start from there and leave those queries out.
+enum { ROW_FORM, SPLIT_FORM, FAR_FORM };
+template <typename T, int HD, bool OWN> struct DkvCfg {
+    using C = std::conditional_t<OWN, WCfg<T, HD, 32, 1>, WCfg<T, HD, (sizeof(T) == 2 && HD < 128) ? 64 : 32>>;
+    static constexpr int STAGE = 2 * C::TILE + 512, STAGES = OWN || STAGE > 20480 ? 2 : 3, BYTES = STAGES * STAGE;      // Q image | dO image | 64 log-sum-exps | 64 row dots
 };
-template <typename T, int HD, bool SPLIT>
-__global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DKV(sizeof(T) * HD)) void window_dkv_kernel(WArgs a) {
-    using D = DkvCfg<T, HD, SPLIT>;
+template <typename T, int HD, int FORM>
+__global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DKV(sizeof(T) * HD), sizeof(T) * HD, FORM == FAR_FORM || (FORM == SPLIT_FORM && sizeof(T) == 2))) void window_dkv_kernel(WArgs a) {
+    constexpr bool OWN = FORM != ROW_FORM, FAR = FORM == FAR_FORM;          // OWN: a wave with tiles of its own
+    using D = DkvCfg<T, HD, OWN>;
     using C = typename D::C;
-    constexpr int STAGE = D::STAGE, STAGES = D::STAGES, ROWS = SPLIT ? 32 : WROWS, STEP = SPLIT ? 4 : 1, NC = SPLIT ? 2 : 1;
+    constexpr int STAGE = D::STAGE, STAGES = D::STAGES, ROWS = OWN ? 32 : WROWS, NC = OWN ? 2 : 1;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    int stream, rblk;
-    if (!place(a, ROWS, a.NB * a.KV, 1, stream, rblk)) return;
+    int stream, rblk, part = 0;
+    if constexpr (FAR) {
+        part = blockIdx.x % a.far_parts;
+        rblk = blockIdx.x / a.far_parts % a.far_groups;
+        stream = blockIdx.x / (a.far_parts * a.far_groups);
+    } else if (!place(a, ROWS, a.NB * a.KV, 1, stream, rblk)) {
+        return;
+    }
     const int hk = stream % a.KV, b = stream / a.KV;
     int64_t start;
-    const int len = seq_rows(a, b, start);
-    if (rblk * ROWS >= len) return;
+    const int len = seq_rows(a, b, start), kend = FAR ? min(a.sinks, len) : len;        // keys from kend on take no part
+    if (rblk * ROWS >= kend) return;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h2 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rep = a.H / a.KV;
     const T* base = (const T*)a.qkv + start * a.ld;
     const T *kb_ = base + (a.H + hk) * HD, *vb_ = kb_ + a.KV * HD;
-    const int kb0 = rblk * ROWS, k0 = kb0 + (SPLIT ? 0 : wave * 32), key = k0 + r, klast = min(k0 + 31, len - 1);
+    const int kb0 = rblk * ROWS, k0 = kb0 + (OWN ? 0 : wave * 32), key = k0 + r, klast = min(k0 + 31, kend - 1);
     const int sinks = a.far_parts ? 0 : a.sinks;
     const float c = a.scale * LOG2E;
 
     typename Frag<T>::V kf[C::FR] = {}, vf[C::FR] = {};
 #pragma unroll
     for (int j = 0; j < C::FR; ++j)
-        if (key < len) {
+        if (key < kend) {
             kf[j] = *reinterpret_cast<const typename Frag<T>::V*>(kb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
             vf[j] = *reinterpret_cast<const typename Frag<T>::V*>(vb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
         }
@@ -690,7 +701,7 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DKV(sizeof(T) * HD)) void 
     f32x16_t dk[C::DB], dv[C::DB];
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) dk[db] = dv[db] = splat16(0.f);
-    if (a.far_parts && k0 < min(a.sinks, len) && (!SPLIT || wave == 0)) {
+    if (!FAR && a.far_parts && k0 < min(a.sinks, len) && (!OWN || wave == 0)) {
         const float* w = a.far_ws + ((int64_t)(b * a.KV + hk) * a.far_groups + k0 / 32) * a.far_parts * (2 * C::DB * 1024) + lane;
 #pragma unroll
         for (int db = 0; db < C::DB; ++db)
@@ -704,60 +715,74 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DKV(sizeof(T) * HD)) void 
     for (int db = 0; db < C::DB; ++db) asm volatile("" : "+v"(dk[db]), "+v"(dv[db]));
 
     // queries that see a key of the block: from the first key minus right to the last key plus left, to the end where there are sinks
-    const int qlo = max(0, kb0 - a.right), qhi = kb0 < sinks ? len - 1 : min(len - 1, min(kb0 + ROWS, len) - 1 + a.left);
-    const int t0 = qlo / C::KT, nt = qhi / C::KT - t0 + 1, total = (nt * rep - (SPLIT ? wave : 0) + STEP - 1) / STEP;      // (head, tile) pairs of this wave
+    const int qlo = FAR ? k0 + a.left + 1 : max(0, kb0 - a.right), qhi = FAR || kb0 < sinks ? len - 1 : min(len - 1, min(kb0 + ROWS, len) - 1 + a.left);
+    const int t0 = qlo / C::KT, nt = max(0, qhi / C::KT - t0 + 1);
+    // this wave's (head, tile) pairs: w0, w0 + step, ...
+    const int step = FAR ? 4 * a.far_parts : OWN ? 4 : 1, w0 = FAR ? part * 4 + wave : OWN ? wave : 0, total = (nt * rep - w0 + step - 1) / step;
     const int64_t gld = (int64_t)a.H * HD;
     const T* gb = (const T*)a.dout + start * gld;
     const float* cb = ((wave & 1) ? a.ndelta : a.lse) + start;         // a shared tile's row constants: the waves alternate, too
     unsigned src[C::NI];
 #pragma unroll
     for (int j = 0; j < C::NI; ++j) {       // the waves alternate between the two images: an instruction knows its descriptor
-        const int p = SPLIT ? j : j * 4 + wave;
+        const int p = OWN ? j : j * 4 + wave;
         src[j] = piece_src<C>(p >= C::NP ? p - C::NP : p, lane, p >= C::NP ? gld : a.ld);
     }
-    int ft = SPLIT ? wave % nt : 0, fh = hk * rep + (SPLIT ? wave / nt : 0);              // the tile and head to fetch next
+    int ft = OWN && nt ? w0 % nt : 0, fh = hk * rep + (OWN && nt ? w0 / nt : 0);              // the tile and head to fetch next
     auto issue = [&](unsigned char* stage) {
         const int64_t row0 = (int64_t)(t0 + ft) * C::KT, left = len - 1 - row0;
         const __amdgpu_buffer_rsrc_t rq = rows_rsrc(base + fh * HD + row0 * a.ld, (left * a.ld + HD) * C::ES);
         const __amdgpu_buffer_rsrc_t rg = rows_rsrc(gb + fh * HD + row0 * gld, (left * gld + HD) * C::ES);
 #pragma unroll
         for (int j = 0; j < C::NI; ++j) {
-            const int p = SPLIT ? j : j * 4 + wave;
+            const int p = OWN ? j : j * 4 + wave;
             if (p >= C::NP) dma16(rg, stage + p * 1024, src[j]);
             else dma16(rq, stage + p * 1024, src[j]);
         }
         const int64_t crow = (int64_t)fh * a.R + row0;
-        if constexpr (SPLIT) {
+        if constexpr (OWN) {
             dma4(rows_rsrc(a.lse + start + crow, (left + 1) * 4), stage + 2 * C::TILE, lane * 4);
             dma4(rows_rsrc(a.ndelta + start + crow, (left + 1) * 4), stage + 2 * C::TILE + 256, lane * 4);
         } else {
             dma4(rows_rsrc(cb + crow, (left + 1) * 4), stage + 2 * C::TILE + (wave & 1) * 256, lane * 4);
         }
-        for (ft += STEP; ft >= nt; ft -= nt) ++fh;
+        for (ft += step; ft >= nt; ft -= nt) ++fh;
     };
     const TrAt<C, (C::RB < 256)> tr(lane);
     const RowAt<C, (C::RB < 256)> rows(lane);
-    unsigned char* own = smem + (SPLIT ? wave * D::BYTES : 0);
+    unsigned char* own = smem + (OWN ? wave * D::BYTES : 0);
     const unsigned lds = lds_u32(own);
-    int fill = 0, use = 0, ct = SPLIT ? wave % nt : 0;
+    int fill = 0, use = 0, ct = ft;
     for (; fill < STAGES - 1 && fill < total; ++fill) issue(own + fill * STAGE);
     fill = STAGES - 1;
     for (int it = 0; it < total; ++it) {
-        tile_ready<(STAGES - 2) * (C::NI + NC), SPLIT>(it + STAGES - 1 > total);
+        tile_ready<(STAGES - 2) * (C::NI + NC), OWN>(it + STAGES - 1 > total);
         if (it + STAGES - 1 < total) issue(own + fill * STAGE);
         fill = fill + 1 == STAGES ? 0 : fill + 1;
         const unsigned ql = lds + use * STAGE, gl = ql + C::TILE;
         use = use + 1 == STAGES ? 0 : use + 1;
         const int q0 = (t0 + ct) * C::KT, q1 = q0 + C::KT - 1;
-        for (ct += STEP; ct >= nt;) ct -= nt;
-        if (k0 >= len || q1 < k0 - a.right || (q0 > klast + a.left && k0 >= sinks)) continue;
-        const bool whole = q1 < len && q0 >= klast - a.right && (q1 <= k0 + a.left || klast < sinks);
-        const int first = key - a.right - q0, last = (key < sinks ? len - 1 : min(len - 1, key + a.left)) - q0;
+        for (ct += step; ct >= nt;) ct -= nt;
+        if (!FAR && (k0 >= len || q1 < k0 - a.right || (q0 > klast + a.left && k0 >= sinks))) continue;
+        const bool whole = FAR ? q1 < len && q0 > klast + a.left && k0 + 31 < kend : q1 < len && q0 >= klast - a.right && (q1 <= k0 + a.left || klast < sinks);
+        const int first = FAR ? key + a.left + 1 - q0 : key - a.right - q0;
+        const int last = FAR ? (key < kend ? len - 1 - q0 : -1) : (key < sinks ? len - 1 : min(len - 1, key + a.left)) - q0;
         dkv_block<C, 0>(ql, gl, gl + C::TILE, rows, kf, vf, c, whole, first, last, tr, dk, dv, h2);
         if constexpr (C::KB == 2) dkv_block<C, 32>(ql, gl, gl + C::TILE, rows, kf, vf, c, whole, first, last, tr, dk, dv, h2);
     }
+    if constexpr (FAR) {
+        float* w = a.far_ws + (((int64_t)stream * a.far_groups + rblk) * a.far_parts + part) * (2 * C::DB * 1024) + wave * 256 + lane;
+#pragma unroll
+        for (int i = 0; i < 2 * C::DB; ++i) {
+            float v[4];
+            join_block(i < C::DB ? dk[i % C::DB] : dv[i % C::DB], 1.0f, reinterpret_cast<float*>(smem), v, wave, lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[i * 1024 + e * 64] = v[e];
+        }
+        return;
+    }
     T* row = (T*)a.dqkv + (start + key) * (a.H + 2 * a.KV) * HD + (a.H + hk) * HD;
-    if constexpr (SPLIT) {
+    if constexpr (OWN) {
         join_rows<C>(dk, a.scale, reinterpret_cast<float*>(smem), key < len, row, wave, lane);
         join_rows<C>(dv, 1.0f, reinterpret_cast<float*>(smem), key < len, row + a.KV * HD, wave, lane);
         return;
@@ -765,95 +790,6 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_DKV(sizeof(T) * HD)) void 
     if (key < len) {
         store_rows<T, HD>(dk, a.scale, row, h2);
         store_rows<T, HD>(dv, 1.0f, row + a.KV * HD, h2);
-    }
-}
-
-// The part of dK and dV that reaches the sinks from queries beyond the window (i > j + left): few keys, all queries of the sequence.  Left to
-// the kernel above, the block with the sinks would sweep the whole sequence while the others are long done.  A wave takes one group of 32
-// keys and one of 4 far_parts slices of the (query head, 32-query tile) list, with its own images in LDS; a block leaves its waves' sum in far_ws.
-template <typename T, int HD>
-__global__ __launch_bounds__(WT) void window_far_kernel(WArgs a) {
-    using C = WCfg<T, HD, 32>;
-    constexpr int STAGE = 2 * C::TILE + 512, NL = C::CH / 2;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int lane = threadIdx.x & 63, r = lane & 31, h2 = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nblk = a.far_parts;
-    const int part = (blockIdx.x % nblk) * 4 + wave, grp = (blockIdx.x / nblk) % a.far_groups;
-    const int hk = (blockIdx.x / (nblk * a.far_groups)) % a.KV, b = blockIdx.x / (nblk * a.far_groups * a.KV);
-    int64_t start;
-    const int len = seq_rows(a, b, start);
-    const int k0 = grp * 32, key = k0 + r, kend = min(a.sinks, len);
-    if (k0 >= kend) return;
-    const int rep = a.H / a.KV;
-    const T* base = (const T*)a.qkv + start * a.ld;
-    const T *kb_ = base + (a.H + hk) * HD, *vb_ = kb_ + a.KV * HD;
-    const float c = a.scale * LOG2E;
-    typedef typename Frag<T>::V V;
-    V kf[C::FR] = {}, vf[C::FR] = {};
-#pragma unroll
-    for (int j = 0; j < C::FR; ++j)
-        if (key < kend) {
-            kf[j] = *reinterpret_cast<const V*>(kb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
-            vf[j] = *reinterpret_cast<const V*>(vb_ + (int64_t)key * a.ld + (2 * j + h2) * (16 / C::ES));
-        }
-    const TrAt<C, false> tr(lane);
-    const RowAt<C, false> rows(lane);
-    f32x16_t dk[C::DB], dv[C::DB];
-#pragma unroll
-    for (int db = 0; db < C::DB; ++db) dk[db] = dv[db] = splat16(0.f);
-    const int t0 = (k0 + a.left + 1) / 32, nt = max(0, (len - 1) / 32 - t0 + 1);         // empty where the window reaches the end
-    const int total = nt * rep, per = (total + 4 * nblk - 1) / (4 * nblk), i0 = part * per, i1 = min(total, i0 + per);
-    unsigned char *ql = smem + wave * STAGE, *gl = ql + C::TILE;
-    float* cst = reinterpret_cast<float*>(gl + C::TILE) + h2 * 64 + r;
-    const unsigned la = lds_u32(ql);
-    const int lim = min(kend - 1, k0 + 31) + a.left;        // queries past this see every key of the group
-    V qr[NL], gr[NL];
-    float cr = 0.f;
-    auto fetch = [&](int it) {
-        const int h = hk * rep + it / nt, q0 = (t0 + it % nt) * 32;
-        const T *qs = base + h * HD, *gs = (const T*)a.dout + start * a.H * HD + h * HD;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int id = lane + i * 64, row = q0 + id / C::CH, col = (id % C::CH) * (16 / C::ES);
-            qr[i] = gr[i] = V{};
-            if (row < len) {
-                qr[i] = *reinterpret_cast<const V*>(qs + (int64_t)row * a.ld + col);
-                gr[i] = *reinterpret_cast<const V*>(gs + (int64_t)row * a.H * HD + col);
-            }
-        }
-        cr = q0 + r < len ? (h2 ? a.ndelta : a.lse)[(int64_t)h * a.R + start + q0 + r] : 0.f;
-    };
-    if (i0 < i1) fetch(i0);
-    for (int it = i0; it < i1; ++it) {
-        const int q0 = (t0 + it % nt) * 32;
-        wave_sync();                                        // the previous tile's reads are done
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int id = lane + i * 64, at = C::at(id / C::CH, id % C::CH);
-            *reinterpret_cast<V*>(ql + at) = qr[i];
-            *reinterpret_cast<V*>(gl + at) = gr[i];
-        }
-        *cst = cr;
-        wave_sync();
-        if (it + 1 < i1) fetch(it + 1);
-        dkv_block<C, 0>(la, la + C::TILE, la + 2 * C::TILE, rows, kf, vf, c, q0 > lim && q0 + 31 < len && kend >= k0 + 32,
-                        key + a.left + 1 - q0, key < kend ? len - 1 - q0 : -1, tr, dk, dv, h2);
-    }
-    // the block's four parts become one, added in their order: every wave adds four of an accumulator's sixteen registers
-    float* w = a.far_ws + (((int64_t)(b * a.KV + hk) * a.far_groups + grp) * nblk + blockIdx.x % nblk) * (2 * C::DB * 1024);
-    float* sum = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int i = 0; i < 2 * C::DB; ++i) {
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sum[(wave * 16 + e) * 64 + lane] = i < C::DB ? dk[i % C::DB][e] : dv[i % C::DB][e];
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int at = (wave * 4 + e) * 64 + lane;
-            w[i * 1024 + at] = (sum[at] + sum[1024 + at]) + (sum[2048 + at] + sum[3072 + at]);
-        }
     }
 }
 
@@ -914,10 +850,12 @@ template <typename T, int HD, bool SPLIT> static int launch_dq(const WArgs& a, h
     constexpr int LDS = SPLIT ? 4 * Ring::BYTES : Ring::BYTES;
     return launch<window_dq_kernel<T, HD, SPLIT>>("star_attn_window_bwd", grid_of(a, SPLIT ? 32 : WROWS, a.H), SPLIT && LDS < 16384 ? 16384 : LDS, a, s);
 }
-template <typename T, int HD, bool SPLIT> static int launch_dkv(const WArgs& a, hipStream_t s) {
-    using D = DkvCfg<T, HD, SPLIT>;
-    constexpr int LDS = SPLIT ? 4 * D::BYTES : D::BYTES;
-    return launch<window_dkv_kernel<T, HD, SPLIT>>("star_attn_window_bwd", grid_of(a, SPLIT ? 32 : WROWS, a.KV), SPLIT && LDS < 16384 ? 16384 : LDS, a, s);
+template <typename T, int HD, int FORM> static int launch_dkv(const WArgs& a, hipStream_t s) {
+    constexpr bool OWN = FORM != ROW_FORM;
+    using D = DkvCfg<T, HD, OWN>;
+    constexpr int LDS = OWN ? 4 * D::BYTES : D::BYTES;
+    const int64_t blocks = FORM == FAR_FORM ? (int64_t)a.NB * a.KV * a.far_groups * a.far_parts : grid_of(a, OWN ? 32 : WROWS, a.KV);
+    return launch<window_dkv_kernel<T, HD, FORM>>("star_attn_window_bwd", blocks, OWN && LDS < 16384 ? 16384 : LDS, a, s);
 }
 template <typename T, int HD> static int run_fwd(const WArgs& a, hipStream_t s) {
     using S = SplitUpTo<T, HD>;
@@ -934,31 +872,32 @@ template <typename T, int HD> static int run_dq(const WArgs& a, hipStream_t s) {
 template <typename T, int HD> static int run_dkv(const WArgs& a, hipStream_t s) {
     using S = SplitUpTo<T, HD>;
     if constexpr (S::EVER)
-        if (few_blocks(a, a.KV, S::KEYS)) return launch_dkv<T, HD, true>(a, s);
-    return launch_dkv<T, HD, false>(a, s);
+        if (few_blocks(a, a.KV, S::KEYS)) return launch_dkv<T, HD, SPLIT_FORM>(a, s);
+    return launch_dkv<T, HD, ROW_FORM>(a, s);
 }
 template <typename T, int HD> static int run_bwd(const WArgs& a, hipStream_t s) {
     const char* who = "star_attn_window_bwd";
     int rc = run_dq<T, HD>(a, s);
     if (rc) return rc;
-    if (a.far_parts) {
-        constexpr int FAR_LDS = 4 * (2 * WCfg<T, HD, 32>::TILE + 512);
-        const int lists = a.NB * a.KV * a.far_groups, size = 2 * WCfg<T, HD>::DB * 1024;
-        if ((rc = launch<window_far_kernel<T, HD>>(who, (int64_t)lists * a.far_parts, FAR_LDS < 16384 ? 16384 : FAR_LDS, a, s))) return rc;
-        if (a.far_parts > 1) {
-            hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, lists), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
-            STAR_LAUNCH_CHECK(who);
+    if constexpr (SplitUpTo<T, HD>::EVER)
+        if (a.far_parts) {
+            if ((rc = launch_dkv<T, HD, FAR_FORM>(a, s))) return rc;
+            if (a.far_parts > 1) {
+                const int size = 2 * WCfg<T, HD>::DB * 1024;
+                hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, a.NB * a.KV * a.far_groups), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
+                STAR_LAUNCH_CHECK(who);
+            }
         }
-    }
     return run_dkv<T, HD>(a, s);
 }
 
 // How the far queries of the sinks are cut: about two blocks of four waves per compute unit in all, no more than 16 parts to add up, and at least
 // two 32-query tiles for a wave.  With over 256 sinks, or very many heads, there are enough key blocks with a long sweep to fill the chip: no parts.
-static void far_plan(int NB, int L, int H, int KV, int left, int sinks, int& groups, int& parts) {
+// (None for float32 rows of 128 either: four rings do not fit into LDS, and the matrix rate of float32 leaves the sinks' block less far behind.)
+static void far_plan(int NB, int L, int H, int KV, int row_bytes, int left, int sinks, int& groups, int& parts) {
     groups = parts = 0;
     sinks = sinks < L ? sinks : L;
-    if (sinks <= 0 || sinks > 256 || left >= L - 1) return;
+    if (sinks <= 0 || sinks > 256 || left >= L - 1 || row_bytes > 256) return;
     const int64_t lists = (int64_t)NB * KV * cdiv(sinks, 32), tiles = (int64_t)(H / KV) * cdiv(L - left - 1, 32);
     if (lists > 65535) return;
     groups = cdiv(sinks, 32);
@@ -999,10 +938,10 @@ extern "C" int star_attn_window_fwd(const StarAttnWindow* g, void* stream) {
     return g->dt == STAR_BF16 ? BY_HD(run_fwd, bf16_t) : BY_HD(run_fwd, float);
 }
 
-extern "C" int64_t star_attn_window_bwd_ws(int64_t R, int NB, int L, int H, int KV, int hd, int left, int sinks) {
+extern "C" int64_t star_attn_window_bwd_ws(int64_t R, int NB, int L, int H, int KV, int hd, int left, int sinks, int dt) {
     if (R < 0 || NB <= 0 || L <= 0 || H <= 0 || KV <= 0 || H % KV || hd <= 0 || left < 0 || sinks < 0) return 0;
     int groups, parts;
-    far_plan(NB, L, H, KV, left, sinks, groups, parts);
+    far_plan(NB, L, H, KV, hd * (dt == STAR_BF16 ? 2 : 4), left, sinks, groups, parts);
     return (H * R + 63) / 64 * 64 + (int64_t)NB * KV * groups * parts * 2 * 32 * (hd < 32 ? 32 : hd);
 }
 
@@ -1014,7 +953,7 @@ extern "C" int star_attn_window_bwd(const StarAttnWindow* g, void* stream) {
     a.dout = g->dout;
     a.dqkv = g->dqkv;
     a.ndelta = g->ws;
-    far_plan(g->NB, g->L, g->H, g->KV, g->left, g->sinks, a.far_groups, a.far_parts);
+    far_plan(g->NB, g->L, g->H, g->KV, g->hd * (g->dt == STAR_BF16 ? 2 : 4), g->left, g->sinks, a.far_groups, a.far_parts);
     a.far_ws = g->ws + (g->H * g->R + 63) / 64 * 64;
     hipStream_t s = (hipStream_t)stream;
     return g->dt == STAR_BF16 ? BY_HD(run_bwd, bf16_t) : BY_HD(run_bwd, float);

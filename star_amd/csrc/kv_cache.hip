@@ -334,7 +334,7 @@ static int step_group(int NB, int H, int KV) {
     if ((int64_t)NB * KV < star_num_cus()) return rep > 1 ? 2 : 1;
     return rep > 4 ? 8 : rep > 2 ? 4 : rep;
 }
-// Threads of a block and splits.  Where there is a block per compute unit, or two rounds of a wide block take all rows, a wide block takes the
+// Threads of a block and splits.  Where there is a block per compute unit, or three rounds of a wide block take all rows, a wide block takes the
 // whole sequence: one launch (5 sequences, 12 heads of 64, 300 visible tokens 6.9 us against 8.2 with narrow blocks, splits and their join; 32 x 8 heads of 128, 500
 // tokens 21 against 25).  Else few (sequence, key head) pairs would leave the chip idle: narrow blocks, the tokens split until there are about
 // four of them per compute unit (8 heads of 128, 4096 tokens 25 us against 70).
@@ -346,7 +346,7 @@ static StepPlan step_plan(int NB, int H, int KV, int hd, int es, int cap, int le
     const int64_t blocks = (int64_t)NB * KV * cdiv(rep, G);
     const int64_t vis = (int64_t)left + 1 + sinks < cap ? (int64_t)left + 1 + sinks : cap;
     const int per = 4 * 64 / (hd * es / 16);              // rows of a wave's round
-    if (blocks >= star_num_cus() || vis <= 2 * per * (wide / 64)) return {wide, 1};
+    if (blocks >= star_num_cus() || vis <= 3 * per * (wide / 64)) return {wide, 1};
     const int64_t rounds = (vis + per * 4 - 1) / (per * 4);
     int64_t s = (4 * (int64_t)star_num_cus() + blocks - 1) / blocks;
     if (s > rounds) s = rounds;

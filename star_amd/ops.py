@@ -535,7 +535,7 @@ def _window_bwd(home, qkv, out, dout, lse, nb, l, h, hd, kv_heads, left, right, 
         assert dqkv.shape == qkv.shape and dqkv.dtype == qkv.dtype and dqkv.is_contiguous()
     if r:
         lib = L.lib()
-        ws = qkv.new_empty(lib.star_attn_window_bwd_ws(r, nb, l, h, g.KV, hd, g.left, sinks), dtype=torch.float32)
+        ws = qkv.new_empty(lib.star_attn_window_bwd_ws(r, nb, l, h, g.KV, hd, g.left, sinks, g.dt), dtype=torch.float32)
         g.out, g.lse, g.dout, g.dqkv, g.ws = out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dqkv.data_ptr(), ws.data_ptr()
         _call("attn_window_bwd", 2 * r * (qkv.shape[1] + h * hd) * qkv.element_size(), lib.star_attn_window_bwd, g, _raw_stream(home))
     return dqkv
