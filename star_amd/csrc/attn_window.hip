@@ -345,6 +345,98 @@ template <class C> struct KvRing {
     }
 };
 
+// A masked weight is 0, and 0 * inf in a product is NaN: an infinity or a NaN in a row that a query does not see would reach it where both meet in
+// one tile.  Results that came out not finite are therefore formed again, one visible row at a time, with no arithmetic on hidden ones: nothing is
+// paid where all results are finite.  Where the row's own statistics are NaN (or, for a key, its own row), so is the result by the formula, and
+// it stays: data that has gone NaN altogether takes no longer than other data.  A lane works on its half of a row, the partner on the other (the
+// layout of an accumulator).
+template <class C> __device__ __forceinline__ bool any_bad(const f32x16_t (&acc)[C::DB]) {
+    float t = 0.f;
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (db * 32 + acc_row(e, 0) < C::HDIM) t = __builtin_fmaf(acc[db][e], 0.f, t);
+    return !(t == 0.f);
+}
+template <class C> __device__ __forceinline__ void read_half(const typename C::Type* row, int h2, f32x16_t (&v)[C::DB]) {
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (db * 32 + 8 * t < C::HDIM) ld4(row + db * 32 + 8 * t + 4 * h2, x);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[db][4 * t + u] = x[u];
+        }
+}
+template <class C> __device__ __forceinline__ float dot_half(const f32x16_t (&v)[C::DB], const typename C::Type* row, int h2) {
+    float d = 0.f;
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (db * 32 + 8 * t < C::HDIM) {
+                float x[4];
+                ld4(row + db * 32 + 8 * t + 4 * h2, x);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) d = __builtin_fmaf(v[db][4 * t + u], x[u], d);
+            }
+    return pair_sum(d);
+}
+// acc = acc * alpha + p * row where seen
+template <class C> __device__ __forceinline__ void add_half(f32x16_t (&acc)[C::DB], float alpha, bool seen, float p, const typename C::Type* row, int h2) {
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (db * 32 + 8 * t < C::HDIM) {
+                float x[4];
+                ld4(row + db * 32 + 8 * t + 4 * h2, x);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) acc[db][4 * t + u] = acc[db][4 * t + u] * alpha + (seen ? p * x[u] : 0.f);
+            }
+}
+__device__ __forceinline__ bool sees(const WArgs& a, int i, int j) { return j <= i + a.right && (j >= i - a.left || j < a.sinks); }
+// the next row after j of those that some query of q0 .. qlast sees
+__device__ __forceinline__ int next_key(const WArgs& a, int j, int q0) { return j + 1 >= a.sinks && j + 1 < q0 - a.left ? q0 - a.left : j + 1; }
+
+// the lane's output row (or, with dO, -delta and lse, its dQ row) from visible keys alone
+template <class C, bool GRAD> __device__ __forceinline__ void redo_query(const WArgs& a, const typename C::Type* base, const typename C::Type* grow, int h, int q, int q0, int len, float ls,
+                                                                         float ndl, int h2, f32x16_t (&acc)[C::DB]) {
+    using T = typename C::Type;
+    constexpr int HD = C::HDIM;
+    const float c = a.scale * LOG2E;
+    const T* kp = base + (a.H + h / (a.H / a.KV)) * HD;
+    const int qlast = min(q0 + 31, len - 1);
+    f32x16_t qv[C::DB], gv[C::DB];
+    read_half<C>(base + (int64_t)q * a.ld + h * HD, h2, qv);
+    if constexpr (GRAD) read_half<C>(grow, h2, gv);
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db) acc[db] = splat16(0.f);
+    float m = -INFINITY, l = 0.f;
+    for (int j = next_key(a, -1, q0); j <= min(len - 1, qlast + a.right); j = next_key(a, j, q0)) {
+        const T *kr = kp + (int64_t)j * a.ld, *vr = kr + a.KV * HD;
+        const bool seen = sees(a, q, j);
+        const float s = dot_half<C>(qv, kr, h2) * c;
+        if constexpr (GRAD) {
+            const float dp = dot_half<C>(gv, vr, h2) + ndl;
+            add_half<C>(acc, 1.0f, seen, __builtin_amdgcn_exp2f(s - ls) * dp, kr, h2);
+        } else {
+            const float mn = seen ? __builtin_elementwise_maximum(m, s) : m;
+            const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn), p = __builtin_amdgcn_exp2f(s - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l = l * alpha + (seen ? p : 0.f);
+            add_half<C>(acc, alpha, seen, p, vr, h2);
+        }
+    }
+    const float mul = GRAD ? a.scale : 1.0f / l;
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[db][e] *= mul;
+}
+
 // Split form: the four waves of a block work on the same 32 rows (dK/dV: keys), each on every fourth tile with a ring of its own, and are added up
 // through LDS, in their order, when all are done.  For launches whose row form (a wave per 32 rows, four sharing the tiles) leaves most of the
 // chip idle (SplitUpTo).
@@ -359,6 +451,14 @@ __device__ __forceinline__ void join_block(const f32x16_t& acc, float mul, float
         const int at = (wave * 4 + e) * 64 + lane;
         v[e] = (sum[at] + sum[1024 + at]) + (sum[2048 + at] + sum[3072 + at]);
     }
+}
+// whether a wave has found its part of the lane pair's row not finite; st: 256 floats of LDS
+__device__ __forceinline__ bool any_wave_bad(bool bad, float* st, int wave, int lane) {
+    const float mine = pair_sum(bad ? 1.0f : 0.f);
+    __syncthreads();
+    st[wave * 64 + lane] = mine;
+    __syncthreads();
+    return st[lane] + st[64 + lane] + st[128 + lane] + st[192 + lane] != 0.f;
 }
 // mul * sum of the waves' accumulators -> the lane's row
 template <class C> __device__ __forceinline__ void join_rows(const f32x16_t (&acc)[C::DB], float mul, float* sum, bool valid, typename C::Type* row, int wave, int lane) {
@@ -489,12 +589,22 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_FWD(sizeof(T) * 
             l += mw == -INFINITY ? 0.f : st[w * 128 + 64 + lane] * __builtin_amdgcn_exp2f((mw - m) * c);
         }
         const float f = own_m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((own_m - m) * c) / l;
-        join_rows<C>(o, f, st + 512, q < len, (T*)a.out + (start + q) * a.H * HD + h * HD, wave, lane);
+        const bool bad = any_wave_bad(any_bad<C>(o), st, wave, lane) && l == l;
+        join_rows<C>(o, f, st + 512, q < len && !bad, (T*)a.out + (start + q) * a.H * HD + h * HD, wave, lane);
+        if (bad && q < len && wave == 0) {
+            redo_query<C, false>(a, base, nullptr, h, q, q0, len, 0.f, 0.f, h2, o);
+            store_rows<T, HD>(o, 1.0f, (T*)a.out + (start + q) * a.H * HD + h * HD, h2);
+        }
         if (q < len && a.lse && h2 == 0 && wave == 0) a.lse[(int64_t)h * a.R + start + q] = m * c + log2f(l);
         return;
     }
     if (q < len) {
-        store_rows<T, HD>(o, 1.0f / l, (T*)a.out + (start + q) * a.H * HD + h * HD, h2);
+        float mul = 1.0f / l;
+        if (pair_sum(any_bad<C>(o) ? 1.0f : 0.f) != 0.f && l == l) {
+            redo_query<C, false>(a, base, nullptr, h, q, q0, len, 0.f, 0.f, h2, o);
+            mul = 1.0f;
+        }
+        store_rows<T, HD>(o, mul, (T*)a.out + (start + q) * a.H * HD + h * HD, h2);
         if (a.lse && h2 == 0) a.lse[(int64_t)h * a.R + start + q] = m * c + log2f(l);
     }
 }
@@ -598,11 +708,27 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DQ(sizeof(T) * H
         half(std::integral_constant<int, 0>{});
         if constexpr (C::KB == 2) half(std::integral_constant<int, 1>{});
     }
+    T* qrow = (T*)a.dqkv + (start + q) * (a.H + 2 * a.KV) * HD + h * HD;
+    const T* grow = (const T*)a.dout + (start + q) * a.H * HD + h * HD;
     if constexpr (SPLIT) {
-        join_rows<C>(dq, a.scale, reinterpret_cast<float*>(smem), q < len, (T*)a.dqkv + (start + q) * (a.H + 2 * a.KV) * HD + h * HD, wave, lane);
+        float* st = reinterpret_cast<float*>(smem);
+        __syncthreads();
+        const bool bad = any_wave_bad(any_bad<C>(dq), st, wave, lane) && ls + dl == ls + dl;
+        join_rows<C>(dq, a.scale, st + 512, q < len && !bad, qrow, wave, lane);
+        if (bad && q < len && wave == 0) {
+            redo_query<C, true>(a, base, grow, h, q, q0, len, ls, -dl, h2, dq);
+            store_rows<T, HD>(dq, 1.0f, qrow, h2);
+        }
         return;
     }
-    if (q < len) store_rows<T, HD>(dq, a.scale, (T*)a.dqkv + (start + q) * (a.H + 2 * a.KV) * HD + h * HD, h2);
+    if (q < len) {
+        float mul = a.scale;
+        if (pair_sum(any_bad<C>(dq) ? 1.0f : 0.f) != 0.f && ls + dl == ls + dl) {
+            redo_query<C, true>(a, base, grow, h, q, q0, len, ls, -dl, h2, dq);
+            mul = 1.0f;
+        }
+        store_rows<T, HD>(dq, mul, qrow, h2);
+    }
 }
 
 // P and dS of 32 queries (rows BLK .. of the images at ql and gl, their log-sum-exps and negated row dots at cst and cst + 256) x 32 keys (kf,
@@ -646,6 +772,42 @@ __device__ __forceinline__ void dkv_block(unsigned ql, unsigned gl, unsigned cst
     }
     mma_tr<C, BLK>(gl, tr, Block<T>(s), dv);
     mma_tr<C, BLK>(ql, tr, Block<T>(dp), dk);
+}
+
+// the lane's dV row, then its dK row, from the queries that see the key alone (see redo_query)
+template <class C> __device__ __forceinline__ void redo_key(const WArgs& a, const typename C::Type* base, int64_t start, int hk, int key, int k0, int len, int h2, typename C::Type* row) {
+    using T = typename C::Type;
+    constexpr int HD = C::HDIM;
+    const float c = a.scale * LOG2E;
+    const int rep = a.H / a.KV, last = k0 < a.sinks ? len - 1 : min(len - 1, min(k0 + 31, len - 1) + a.left);
+    f32x16_t kv[C::DB], vv[C::DB], acc[C::DB];
+    read_half<C>(base + (int64_t)key * a.ld + (a.H + hk) * HD, h2, kv);
+    read_half<C>(base + (int64_t)key * a.ld + (a.H + a.KV + hk) * HD, h2, vv);
+    float nans = 0.f;
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nans += kv[db][e] == kv[db][e] ? 0.f : 1.0f;
+    if (pair_sum(nans) != 0.f) {
+#pragma unroll
+        for (int db = 0; db < C::DB; ++db) acc[db] = splat16(NAN);
+        store_rows<T, HD>(acc, 1.0f, row, h2);
+        store_rows<T, HD>(acc, 1.0f, row + a.KV * HD, h2);
+        return;
+    }
+    for (int grad = 0; grad < 2; ++grad) {          // 0: dV, 1: dK
+#pragma unroll
+        for (int db = 0; db < C::DB; ++db) acc[db] = splat16(0.f);
+        for (int h = hk * rep; h < (hk + 1) * rep; ++h)
+            for (int i = max(0, k0 - a.right); i <= last; ++i) {
+                const T *qr = base + (int64_t)i * a.ld + h * HD, *gr = (const T*)a.dout + (start + i) * a.H * HD + h * HD;
+                const int64_t at = (int64_t)h * a.R + start + i;
+                float w = __builtin_amdgcn_exp2f(dot_half<C>(kv, qr, h2) * c - a.lse[at]);
+                if (grad) w *= dot_half<C>(vv, gr, h2) + a.ndelta[at];
+                add_half<C>(acc, 1.0f, sees(a, i, key), w, grad ? qr : gr, h2);
+            }
+        store_rows<T, HD>(acc, grad ? a.scale : 1.0f, grad ? row : row + a.KV * HD, h2);
+    }
 }
 
 // dK and dV, the key on the lane: sweeps the queries that see the block's keys, for every query head of the group.
@@ -783,13 +945,21 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DKV(sizeof(T) * 
     }
     T* row = (T*)a.dqkv + (start + key) * (a.H + 2 * a.KV) * HD + (a.H + hk) * HD;
     if constexpr (OWN) {
-        join_rows<C>(dk, a.scale, reinterpret_cast<float*>(smem), key < len, row, wave, lane);
-        join_rows<C>(dv, 1.0f, reinterpret_cast<float*>(smem), key < len, row + a.KV * HD, wave, lane);
+        float* st = reinterpret_cast<float*>(smem);
+        __syncthreads();
+        const bool bad = any_wave_bad(any_bad<C>(dk) || any_bad<C>(dv), st, wave, lane);
+        join_rows<C>(dk, a.scale, st + 512, key < len && !bad, row, wave, lane);
+        join_rows<C>(dv, 1.0f, st + 512, key < len && !bad, row + a.KV * HD, wave, lane);
+        if (bad && key < len && wave == 0) redo_key<C>(a, base, start, hk, key, k0, len, h2, row);
         return;
     }
     if (key < len) {
-        store_rows<T, HD>(dk, a.scale, row, h2);
-        store_rows<T, HD>(dv, 1.0f, row + a.KV * HD, h2);
+        if (pair_sum(any_bad<C>(dk) || any_bad<C>(dv) ? 1.0f : 0.f) != 0.f) {
+            redo_key<C>(a, base, start, hk, key, k0, len, h2, row);
+        } else {
+            store_rows<T, HD>(dk, a.scale, row, h2);
+            store_rows<T, HD>(dv, 1.0f, row + a.KV * HD, h2);
+        }
     }
 }
 
@@ -848,14 +1018,14 @@ template <typename T, int HD, bool SPLIT> static int launch_fwd(const WArgs& a, 
 template <typename T, int HD, bool SPLIT> static int launch_dq(const WArgs& a, hipStream_t s) {
     using Ring = KvRing<RowCfg<T, HD, SPLIT>>;
     constexpr int LDS = SPLIT ? 4 * Ring::BYTES : Ring::BYTES;
-    return launch<window_dq_kernel<T, HD, SPLIT>>("star_attn_window_bwd", grid_of(a, SPLIT ? 32 : WROWS, a.H), SPLIT && LDS < 16384 ? 16384 : LDS, a, s);
+    return launch<window_dq_kernel<T, HD, SPLIT>>("star_attn_window_bwd", grid_of(a, SPLIT ? 32 : WROWS, a.H), SPLIT && LDS < 18432 ? 18432 : LDS, a, s);
 }
 template <typename T, int HD, int FORM> static int launch_dkv(const WArgs& a, hipStream_t s) {
     constexpr bool OWN = FORM != ROW_FORM;
     using D = DkvCfg<T, HD, OWN>;
     constexpr int LDS = OWN ? 4 * D::BYTES : D::BYTES;
     const int64_t blocks = FORM == FAR_FORM ? (int64_t)a.NB * a.KV * a.far_groups * a.far_parts : grid_of(a, OWN ? 32 : WROWS, a.KV);
-    return launch<window_dkv_kernel<T, HD, FORM>>("star_attn_window_bwd", blocks, OWN && LDS < 16384 ? 16384 : LDS, a, s);
+    return launch<window_dkv_kernel<T, HD, FORM>>("star_attn_window_bwd", blocks, OWN && LDS < 18432 ? 18432 : LDS, a, s);
 }
 template <typename T, int HD> static int run_fwd(const WArgs& a, hipStream_t s) {
     using S = SplitUpTo<T, HD>;

@@ -3,7 +3,7 @@ where they can go wrong.  Bounds are derived in window_util."""
 import pytest
 import torch
 
-from window_util import assert_within, half, heads, reference, rotate, slot_of, unpack
+from window_util import assert_within, half, heads, reference, rotate, seen, slot_of, unpack
 
 pytestmark = pytest.mark.gpu
 
@@ -134,6 +134,41 @@ def test_ragged_batch_leaves_rows_outside_every_sequence(dtype):
     assert torch.equal(short[1:65], want) and not short[65:].any()
     wild, _ = ops.attn_window_fwd(qkv, 3, 64, h, hd, kv_heads=kv, offsets=torch.tensor([-5, -1, rows + 4, rows + 900], device=DEV))
     assert wild.shape == (rows, h * hd)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("nb", [1, 40])
+@pytest.mark.parametrize("window", [(None, 0, 0), (20, 0, 0), (33, 7, 0), (40, 0, 3)])
+def test_what_a_row_does_not_see_does_not_reach_it(dtype, hd, nb, window):
+    """rows that hold infinities and NaN, in few and in many sequences: every row that sees none of them keeps its result and its gradient"""
+    left, right, sinks = window
+    g = _gen(hd + nb)
+    n, h, kv = 150, 12, 6
+    see = seen(n, left, right, sinks)
+    clean, dout = _rand(g, nb * n, (h + 2 * kv) * hd, dtype=dtype), _rand(g, nb * n, h * hd, dtype=dtype)
+    wild = torch.zeros(n, dtype=torch.bool)
+    wild[[70, 71, 140] + list(range(147, 150))] = True
+    for value, cols in ((float("nan"), slice(None)), (float("inf"), slice((h + kv) * hd, None))):
+        qkv, grad = clean.clone().view(nb, n, -1), dout.clone().view(nb, n, -1)
+        qkv[:, wild.to(DEV), cols] = value
+        if cols == slice(None):
+            grad[:, wild.to(DEV)] = value
+        qkv, grad = qkv.view(nb * n, -1), grad.view(nb * n, -1)
+        kw = dict(kv_heads=kv, left=left, right=right, sinks=sinks)
+        out, lse = ops.attn_window_fwd(qkv, nb, n, h, hd, **kw)
+        dqkv = ops.attn_window_bwd(qkv, out, grad, lse, nb, n, h, hd, **kw)
+        hit = (see & wild).any(1) | (wild if cols == slice(None) else False)       # queries that see such a row
+        hit_key = (see & hit[:, None]).any(0) | wild                              # keys that such a query sees
+        for b in {0, nb // 2, nb - 1}:
+            rows = slice(b * n, (b + 1) * n)
+            q, k, v = unpack(clean[rows], h, kv, hd)
+            want = reference(q, k, v, left, right, sinks, None, heads(dout[rows], hd), dtype)
+            o, d = heads(out[rows], hd), heads(dqkv[rows], hd)
+            assert not torch.isfinite(o[:, hit]).all(-1).any()
+            assert_within(o[:, ~hit], want["out"][:, ~hit], want["tol_out"][:, ~hit], "out")
+            assert_within(d[:h, ~hit], want["dqkv"][:h, ~hit], want["tol_dqkv"][:h, ~hit], "dq")
+            assert_within(d[h:, ~hit_key], want["dqkv"][h:, ~hit_key], want["tol_dqkv"][h:, ~hit_key], "dk, dv")
 
 
 @pytest.mark.parametrize("dtype", TYPES)
