@@ -80,9 +80,9 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned char* 
 __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, unsigned char* lds, unsigned off) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 4, off, 0, 0, 0);
 }
-template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-// every wave's DMA of the tile has landed, and every wave is done with the stage that is filled next
-// (a wave with a ring of its own needs no barrier: its reads of a stage have returned when it fills it again)
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+// every wave's DMA of the tile has landed, and every wave's reads of the stage that is filled next have returned
+// (a wave with a ring of its own needs no barrier)
 template <int N, bool OWN> __device__ __forceinline__ void tile_ready(bool last) {
     if (last) wait_vm<0>();
     else wait_vm<N>();
@@ -586,7 +586,7 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_FWD(sizeof(T) * 
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float mw = st[w * 128 + lane];
-            l += mw == -INFINITY ? 0.f : st[w * 128 + 64 + lane] * __builtin_amdgcn_exp2f((mw - m) * c);
+            l += st[w * 128 + 64 + lane] * (mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * c));       // -inf: 0, or NaN of a NaN score
         }
         const float f = own_m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((own_m - m) * c) / l;
         const bool bad = any_wave_bad(any_bad<C>(o), st, wave, lane) && l == l;

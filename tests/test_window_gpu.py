@@ -166,6 +166,7 @@ def test_what_a_row_does_not_see_does_not_reach_it(dtype, hd, nb, window):
             want = reference(q, k, v, left, right, sinks, None, heads(dout[rows], hd), dtype)
             o, d = heads(out[rows], hd), heads(dqkv[rows], hd)
             assert not torch.isfinite(o[:, hit]).all(-1).any()
+            assert cols != slice(None) or lse[:, rows].cpu()[:, hit].isnan().all()
             assert_within(o[:, ~hit], want["out"][:, ~hit], want["tol_out"][:, ~hit], "out")
             assert_within(d[:h, ~hit], want["dqkv"][:h, ~hit], want["tol_dqkv"][:h, ~hit], "dq")
             assert_within(d[h:, ~hit_key], want["dqkv"][h:, ~hit_key], want["tol_dqkv"][h:, ~hit_key], "dk, dv")
@@ -474,6 +475,92 @@ def test_captured_and_replayed(dtype):
         eager = (*train(), step(), cache, lengths)
         for a, b in zip(kept, eager):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_that_lie_past_two_to_the_31_elements(dtype):
+    """the last rows of a matrix of over 2^31 elements (and, float32, 2^33 bytes): rotation, both passes, append"""
+    g = _gen(51)
+    h, kv, hd, sections = 4, 2, 64, (8, 12, 12)
+    w, ld = (h + 2 * kv) * hd, 1 << 16
+    lens = [70, 0, 129]
+    rows = (1 << 15) + 900
+    first = rows - sum(lens)
+    wide = torch.empty(rows, ld, dtype=dtype, device=DEV)
+    qkv = wide[:, ld - w:]
+    assert first * ld > 1 << 31
+    qkv[first:] = _rand(g, sum(lens), w, dtype=dtype)
+    pos = torch.randint(0, 5000, (3, rows), generator=g).to(torch.int32).to(DEV)
+    want = ops.rope_fwd(qkv[first:].contiguous(), pos[:, first:].contiguous(), h + kv, hd, sections)
+    assert torch.equal(ops.rope_fwd(qkv, pos, h + kv, hd, sections, out=qkv)[first:], want)
+    offsets = torch.tensor([first, first + 70, first + 70, rows], device=DEV)
+    dout = torch.zeros(rows, h * hd, dtype=dtype, device=DEV)
+    dout[first:] = _rand(g, sum(lens), h * hd, dtype=dtype)
+    at = first
+    kw = dict(kv_heads=kv, left=40, sinks=2, offsets=offsets)
+    out, lse = ops.attn_window_fwd(qkv, 3, 129, h, hd, **kw)
+    dqkv = ops.attn_window_bwd(qkv, out, dout, lse, 3, 129, h, hd, **kw)
+    for n in lens:
+        if n:
+            q, k, v = unpack(qkv[at:at + n].contiguous(), h, kv, hd)
+            ref = reference(q, k, v, 40, 0, 2, dout=heads(dout[at:at + n], hd), dtype=dtype)
+            assert_within(heads(out[at:at + n], hd), ref["out"], ref["tol_out"], "out of %d" % n)
+            assert_within(heads(dqkv[at:at + n], hd), ref["dqkv"], ref["tol_dqkv"], "dqkv of %d" % n)
+        at += n
+    cache = torch.zeros(2, 3, kv, 140, hd, dtype=dtype, device=DEV)
+    lengths = torch.tensor([70, 0, 129], dtype=torch.int32, device=DEV)
+    ops.kv_append(qkv, cache, lengths, 129, h, sinks=2, offsets=offsets)
+    x = qkv[first:].reshape(-1, h + 2 * kv, hd)
+    assert torch.equal(cache[0, 2, :, :129], x[70:, h:h + kv].transpose(0, 1)) and torch.equal(cache[1, 0, :, :70], x[:70, h + kv:].transpose(0, 1))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_cache_past_two_to_the_31_elements(dtype):
+    """two sequences of millions of slots: what the steps read and write lies behind 2^31 elements; the ring's end is passed on the way"""
+    g = _gen(52)
+    h, kv, hd, cap, sinks, left = 4, 1, 64, 1 << 24, 3, 500
+    cache = torch.empty(2, 2, kv, cap, hd, dtype=dtype, device=DEV)
+    lengths = [cap + 200, cap - 5]
+    for b, n in enumerate(lengths):
+        for p in list(range(sinks)) + list(range(n - 2 - left, n)):
+            cache[:, b, :, slot_of(p, sinks, cap)] = _rand(g, 2, kv, hd, dtype=dtype)
+    n32 = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    small = torch.zeros(2, 2, kv, 700, hd, dtype=dtype, device=DEV)      # the same tokens in a cache of the ordinary size, counted from there
+    shift = [n - 650 for n in lengths]
+    for b, n in enumerate(lengths):
+        for p in list(range(sinks)) + list(range(n - 2 - left, n)):
+            small[:, b, :, p if p < sinks else slot_of(p - shift[b], sinks, 700)] = cache[:, b, :, slot_of(p, sinks, cap)]
+    s32 = torch.full((2,), 650, dtype=torch.int32, device=DEV)
+    for _ in range(3):
+        row = _rand(g, 2, (h + 2 * kv) * hd, dtype=dtype)
+        out = ops.attn_window_step(row, cache, n32, h, left=left, sinks=sinks)
+        assert torch.equal(out, ops.attn_window_step(row, small, s32, h, left=left, sinks=sinks))
+        for b in range(2):
+            slot = slot_of(int(n32[b]) - 1, sinks, cap)
+            assert torch.equal(cache[0, b, 0, slot], row[b, h * hd:(h + 1) * hd]) and torch.equal(cache[1, b, 0, slot], row[b, (h + 1) * hd:])
+        n32 += 1
+        s32 += 1
+
+
+def test_many_short_sequences():
+    """more sequences than a grid has rows in its second dimension, one and two tokens each"""
+    g = _gen(53)
+    nb, h, kv, hd = 70000, 2, 1, 16
+    qkv = _rand(g, nb, (h + 2 * kv) * hd, dtype=torch.bfloat16)
+    dout = _rand(g, nb, h * hd, dtype=torch.bfloat16)
+    out, lse = ops.attn_window_fwd(qkv, nb, 1, h, hd, kv_heads=kv)
+    dqkv = ops.attn_window_bwd(qkv, out, dout, lse, nb, 1, h, hd, kv_heads=kv)
+    v = qkv[:, 3 * hd:]
+    assert torch.equal(out, v.repeat(1, 2))              # one visible key: its value, and a softmax without a gradient
+    got = dqkv[:, 3 * hd:].double()
+    want = dout.double().view(nb, 2, hd).sum(1)
+    assert ((got - want).abs() <= half(torch.bfloat16) * want.abs() + 2.0 ** -20).all()
+    # P dP - P delta: both are the same float32 sum but for its order and out's rounding (none here) -> a few 2^-24 of sums of 16 products
+    assert (dqkv[:, :3 * hd].double().abs() < 2.0 ** -14).all()
+    cache = torch.zeros(2, nb, kv, 4, hd, dtype=torch.bfloat16, device=DEV)
+    n = torch.ones(nb, dtype=torch.int32, device=DEV)
+    assert torch.equal(ops.attn_window_step(qkv, cache, n, h), out)
+    assert torch.equal(cache[1, :, 0, 0], v) and not cache[:, :, :, 1:].any()
 
 
 def test_empty_batches():
