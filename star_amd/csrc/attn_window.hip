@@ -609,7 +609,11 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_FWD(sizeof(T) * 
     }
 }
 
-// dQ, the query on the lane; also -delta = -rowsum(dO * O), which the dK/dV kernels launched behind this one read
+// dQ, the query on the lane; also -delta = -rowsum(dO * O), which the dK/dV kernels launched behind this one read.
+// In bf16 the rows of O are rounded, and with few visible keys that is felt: dP - delta cancels, and dQ and dK are up to 1.9 times as far off as one
+// rounding of the results leaves them (7 keys a row 1.72, 33 on average 1.55, 184 1.48, 258 and more 1.45).  The sum of the row's dS, which is
+// zero by the formula, is just what delta is short of: blocks whose rows see at most FEW_KEYS take it in a sweep of its own first.
+#define FEW_KEYS 256
 template <typename T, int HD, bool SPLIT>
 __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DQ(sizeof(T) * HD), sizeof(T) * HD, SPLIT && sizeof(T) == 2)) void window_dq_kernel(WArgs a) {
     using C = RowCfg<T, HD, SPLIT>;
@@ -648,10 +652,7 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DQ(sizeof(T) * H
             }
         }
     dl = pair_sum(dl);
-    if (q < len) {
-        ls = a.lse[(int64_t)h * a.R + start + q];
-        if (h2 == 0 && (!SPLIT || wave == 0)) a.ndelta[(int64_t)h * a.R + start + q] = -dl;
-    }
+    if (q < len) ls = a.lse[(int64_t)h * a.R + start + q];
 #pragma unroll
     for (int j = 0; j < C::FR; ++j) {
         pin(qf[j]);
@@ -675,39 +676,66 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DQ(sizeof(T) * H
         const int it = first + i * STEP;
         return it < ns ? it : w0 + it - ns;
     };
-    int fill = 0, use = 0;
-    for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), own + fill * Ring::STAGE);
-    fill = Ring::STAGES - 1;
-    for (int it = 0; it < nt; ++it) {
-        tile_ready<(Ring::STAGES - 2) * C::NI, SPLIT>(it + Ring::STAGES - 1 > nt);
-        if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), own + fill * Ring::STAGE);
-        fill = fill + 1 == Ring::STAGES ? 0 : fill + 1;
-        const unsigned kl = lds + use * Ring::STAGE, vl = kl + C::TILE;
-        use = use + 1 == Ring::STAGES ? 0 : use + 1;
-        const int k0 = tile(it) * C::KT, k1 = k0 + C::KT - 1;
-        if (q0 >= len || k0 > qlast + a.right || (k1 < q0 - a.left && k0 >= a.sinks)) continue;
-        const bool whole = k1 < len && k1 <= q0 + a.right && (k0 >= qlast - a.left || k1 < a.sinks);
-        auto half = [&](auto kb_) {
-            constexpr int kb = decltype(kb_)::value;
-            f32x16_t s = splat16(0.f), dp = splat16(-dl);
+    float short_of = 0.f;
+    auto sweep = [&](auto sum_) {
+        constexpr bool SUM = decltype(sum_)::value;
+        int fill = 0, use = 0;
+        for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), own + fill * Ring::STAGE);
+        fill = Ring::STAGES - 1;
+        for (int it = 0; it < nt; ++it) {
+            tile_ready<(Ring::STAGES - 2) * C::NI, SPLIT>(it + Ring::STAGES - 1 > nt);
+            if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), own + fill * Ring::STAGE);
+            fill = fill + 1 == Ring::STAGES ? 0 : fill + 1;
+            const unsigned kl = lds + use * Ring::STAGE, vl = kl + C::TILE;
+            use = use + 1 == Ring::STAGES ? 0 : use + 1;
+            const int k0 = tile(it) * C::KT, k1 = k0 + C::KT - 1;
+            if (q0 >= len || k0 > qlast + a.right || (k1 < q0 - a.left && k0 >= a.sinks)) continue;
+            const bool whole = k1 < len && k1 <= q0 + a.right && (k0 >= qlast - a.left || k1 < a.sinks);
+            auto half = [&](auto kb_) {
+                constexpr int kb = decltype(kb_)::value;
+                f32x16_t s = splat16(0.f), dp = splat16(-dl);
 #pragma unroll
-            for (int j = 0; j < C::FR; ++j) {
-                s = mma_frag<T>(row.template read<kb * 32>(kl, j), qf[j], s);
-                dp = mma_frag<T>(row.template read<kb * 32>(vl, j), gf[j], dp);
+                for (int j = 0; j < C::FR; ++j) {
+                    s = mma_frag<T>(row.template read<kb * 32>(kl, j), qf[j], s);
+                    dp = mma_frag<T>(row.template read<kb * 32>(vl, j), gf[j], dp);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -ls)) * dp[e];
+                if (!whole) {
+                    const int kk = k0 + kb * 32;
+                    const unsigned in = block_mask(q - a.left - kk, min(q + a.right, len - 1) - kk, a.sinks - kk, h2);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[e] = keep_or(row_in(in, e), s[e], 0u);
+                }
+                if constexpr (SUM) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) short_of += s[e];
+                } else {
+                    mma_tr<C, kb * 32>(kl, tr, Block<T>(s), dq);
+                }
+            };
+            half(std::integral_constant<int, 0>{});
+            if constexpr (C::KB == 2) half(std::integral_constant<int, 1>{});
+        }
+    };
+    if constexpr (C::ES == 2) {
+        const int last = min(len - 1, min(rblk * ROWS + ROWS, len) - 1 + a.right);
+        if (min(last + 1, a.left + a.right + 1 + a.sinks) <= FEW_KEYS) {
+            sweep(std::true_type{});
+            short_of = pair_sum(short_of);
+            __syncthreads();
+            if constexpr (SPLIT) {
+                float* st = reinterpret_cast<float*>(smem);
+                st[wave * 64 + lane] = short_of;
+                __syncthreads();
+                short_of = (st[lane] + st[64 + lane]) + (st[128 + lane] + st[192 + lane]);
+                __syncthreads();
             }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -ls)) * dp[e];
-            if (!whole) {
-                const int kk = k0 + kb * 32;
-                const unsigned in = block_mask(q - a.left - kk, min(q + a.right, len - 1) - kk, a.sinks - kk, h2);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = keep_or(row_in(in, e), s[e], 0u);
-            }
-            mma_tr<C, kb * 32>(kl, tr, Block<T>(s), dq);
-        };
-        half(std::integral_constant<int, 0>{});
-        if constexpr (C::KB == 2) half(std::integral_constant<int, 1>{});
+            dl += short_of;
+        }
     }
+    if (q < len && h2 == 0 && (!SPLIT || wave == 0)) a.ndelta[(int64_t)h * a.R + start + q] = -dl;
+    sweep(std::false_type{});
     T* qrow = (T*)a.dqkv + (start + q) * (a.H + 2 * a.KV) * HD + h * HD;
     const T* grow = (const T*)a.dout + (start + q) * a.H * HD + h * HD;
     if constexpr (SPLIT) {

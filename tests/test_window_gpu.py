@@ -172,6 +172,26 @@ def test_what_a_row_does_not_see_does_not_reach_it(dtype, hd, nb, window):
             assert_within(d[h:, ~hit_key], want["dqkv"][h:, ~hit_key], want["tol_dqkv"][h:, ~hit_key], "dk, dv")
 
 
+@pytest.mark.parametrize("n,hd", [(3, 64), (7, 128), (40, 32), (130, 16)])
+@pytest.mark.parametrize("nb", [9, 300])
+def test_gradients_of_few_visible_keys_carry_two_roundings(n, hd, nb):
+    """dP - delta cancels where a key dominates, so a delta from rounded rows would be felt.  Left are the rounding of P or dS and that of the
+    result, each off by at most half a step and evenly spread, so 1/sqrt(3) of that in the mean square: half(bf16) sqrt(2 / 3) together"""
+    g = _gen(n)
+    h = 6
+    qkv, dout = _rand(g, nb * n, 3 * h * hd, dtype=torch.bfloat16, mul=1.2), _rand(g, nb * n, h * hd, dtype=torch.bfloat16)
+    out, lse = ops.attn_window_fwd(qkv, nb, n, h, hd)
+    dqkv = ops.attn_window_bwd(qkv, out, dout, lse, nb, n, h, hd)
+    want = []
+    for b in range(nb):
+        rows = slice(b * n, (b + 1) * n)
+        want.append(reference(*unpack(qkv[rows], h, h, hd), None, 0, 0, dout=heads(dout[rows], hd), dtype=torch.bfloat16)["dqkv"].transpose(0, 1).reshape(n, -1))
+    want, got = torch.cat(want), dqkv.cpu().double()
+    for i in range(3):
+        cols = slice(i * h * hd, (i + 1) * h * hd)
+        assert (got[:, cols] - want[:, cols]).norm() <= half(torch.bfloat16) * (2 / 3) ** 0.5 * want[:, cols].norm(), "dqdkdv"[2 * i:2 * i + 2]
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_strided_rows_and_scale(dtype):
     g = _gen(9)
