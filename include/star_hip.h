@@ -226,7 +226,7 @@ int star_attn_bwd(const void* qkv, const void* out, const void* dout, const floa
  * star_rope: y = x with the first rot_heads heads of every row turned: pair i of a head by theta = 2 pi pos[axis[i]] rev[i] --
  *   y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin -- or by -theta (inverse != 0: the backward pass).  The pair is elements (i, i + pairs),
  *   or (2 i, 2 i + 1) when interleaved; elements from 2 * pairs on do not turn.  pos int32 [axes] rows of R, pos_ld elements apart.
- *   y == x: in place, only the turning elements are touched; else every one of the W columns is written.  W % 8 == 0, hd % 16 == 0,
+ *   y == x: in place, only the turning elements are touched; else every one of the W columns is written, and x and y share no element.  W % 8 == 0, hd % 16 == 0,
  *   pairs % 8 == 0.  Angles are formed in float64. */
 typedef struct StarRope {
     double rev[64];       /* revolutions per unit of position */
@@ -237,7 +237,8 @@ int star_rope(const void* x, int64_t x_ld, void* y, int64_t y_ld, const int32_t*
               int rot_heads, int hd, int inverse, int dt, void* stream);
 /* star_attn_window_fwd: key j is visible to query i iff j <= i + right and (j >= i - left or j < sinks), both inside the sequence.
  * Sequence b is rows [b L, (b + 1) L) or, with offsets int64 [NB + 1] on the device, rows [offsets[b], offsets[b+1]), of which the first
- * L are used (L = the longest sequence); rows of no sequence are neither read nor written.  hd in {16, 32, 64, 128}.
+ * L are used (L = the longest sequence); rows of no sequence are neither read nor written.  What a row does not see does not reach its
+ * result, infinities and NaN included.  hd in {16, 32, 64, 128}.
  *   out dt [R, H*hd]; lse float32 [H, R]: log2-domain log-sum-exp of every row (optional in the forward pass).
  * star_attn_window_bwd: reads out, lse, dout dt [R, H*hd]; writes dqkv dt [R, (H + 2 KV) hd] (dense rows; gradients of a shared key/value head
  *   are summed over its query heads).  ws float32 [star_attn_window_bwd_ws(...)], any content.  No atomics: bitwise reproducible. */

@@ -12,6 +12,15 @@
 // statistics are in-lane reductions plus one exchange with lane ^ 32, and P^T feeds the next product as it lies in the registers.
 // bf16 runs on v_mfma_f32_32x32x16_bf16, float32 on v_mfma_f32_32x32x2_f32 (full float32 products): an operand fragment is 16 bytes
 // per lane in both, so the tile layout and the address arithmetic are shared.
+//
+// Measured (kernels alone): forward 5 x 4096 rows, 12 heads of 64, window 1024: 94 us = 0.61 PFLOP/s; 8192 rows, 32 heads of 128 on 8, window 4096:
+// 412 .. 490 us = 1.0 .. 0.85 PFLOP/s (a large library product reaches 1.29).  2 x 8192 rows, 16 heads of 128, window 2048: forward 302 us, dQ 433,
+// dK/dV 622 = 0.8 PFLOP/s each.  What bounds them: the softmax's vector instructions and the matrix pipe add up (64-wide heads: 207 instructions a
+// 64 x 32 tile, 65 % and 35 % of the busy time; wave priorities around either change nothing); for 128-wide heads, backward, the LDS reads
+// of the fragments beside the products (dK/dV without its transposed products 470 us, without its score products 431, without both 300).
+// Short sequences are bound by the latency of few tiles per wave.
+// P and dS are rounded to bf16 for the second products (the matrix instruction's operand): with the rounding of the result the backward pass
+// is sqrt 2 as far off as that rounding alone.  Sums, statistics and row dots are float32.
 #include "common.h"
 #include <atomic>
 #include <type_traits>
@@ -449,7 +458,7 @@ __device__ __forceinline__ void join_block(const f32x16_t& acc, float mul, float
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int at = (wave * 4 + e) * 64 + lane;
-        v[e] = (sum[at] + sum[1024 + at]) + (sum[2048 + at] + sum[3072 + at]);
+        v[e] = (sum[at] + sum[at + 1024]) + (sum[at + 2 * 1024] + sum[at + 3 * 1024]);
     }
 }
 // whether a wave has found its part of the lane pair's row not finite; st: 256 floats of LDS

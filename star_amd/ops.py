@@ -452,6 +452,7 @@ def _rope(home, x, pos, rot_heads, hd, sections, base, per_axis, interleaved, ou
     shape = x.shape
     ld = _rows2d(x, shape, "x")
     r, w = shape
+    assert r < 1 << 31, "%d rows" % r
     plan = rope_plan(tuple(sections), base, per_axis, interleaved)
     pos, pos_ld = _positions(pos, plan.axes, r)
     if out is None:
@@ -469,7 +470,7 @@ def rope_fwd(x, pos, rot_heads, hd, sections, base=10000.0, per_axis=False, inte
     """Rotary positions with several axes.  x [R, W] (bf16 / float32, dense rows that may lie apart): the first rot_heads heads of hd elements
     of every row turn (packed qkv rows: the query and key heads, H + KV of them), the other columns are copied.  pos int32 [axes, R]: the
     tokens' coordinates, one row per entry of `sections` (see rope_plan).  interleaved: pairs are neighbours (2 i, 2 i + 1) instead of
-    (i, i + n).  out=x turns in place.  -> [R, W]"""
+    (i, i + n).  out=x turns in place; else out and x share no element.  -> [R, W]"""
     return _rope(x, pos, rot_heads, hd, sections, base, per_axis, interleaved, out, 0)
 
 
@@ -516,7 +517,8 @@ def attn_window_fwd(qkv, nb, l, h, hd, kv_heads=None, left=None, right=0, sinks=
     """Sliding-window attention with sinks.  qkv [R, (h + 2 kv_heads) hd]: packed rows (bf16 / float32, dense rows that may lie apart), query head i
     reads key/value head i // (h // kv_heads).  Key j is visible to query i iff j <= i + right and (j >= i - left or j < sinks); None: no
     bound (right=0: causal; left=right=None: everything).  nb sequences of l rows, or ragged: offsets int64 [nb + 1] on the device, l >= the
-    longest sequence (of a longer one only the first l rows take part).  Rows outside every sequence are neither read nor written.
+    longest sequence (of a longer one only the first l rows take part).  Rows outside every sequence are neither read nor written, and what a
+    row does not see does not reach its result, infinities and NaN included (rows that meet such in a tile cost more time).
     -> (out [R, h*hd], lse float32 [h, R] or None)"""
     return _window_fwd(qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale, want_lse, out)
 
@@ -585,6 +587,7 @@ def _window_step(home, qkv, cache, lengths, h, left, sinks, pos, sections, base,
     ld = _rows2d(qkv, shape, "qkv")
     nb, kv, cap, hd = _cache_dims(cache, qkv, shape[1], h, lengths)
     assert shape[0] == nb, "%d rows for %d cache entries" % (shape[0], nb)
+    assert (pos is None) == (sections is None), "a rotation needs pos and sections"
     if out is None:
         out = qkv.new_empty((nb, h * hd))
     else:

@@ -82,7 +82,9 @@ def test_append_refuses(change, words):
 @pytest.mark.parametrize("change,words", [
     (dict(x=None), "null"), (dict(pos=None), "null"), (dict(dt=2), "dtype"), (dict(hd=24), "bad shape"), (dict(W=300), "bad shape"), (dict(rot=0), "bad shape"),
     (dict(rot=9), "bad shape"), (dict(R=-1), "bad shape"), (dict(hd=16), "pairs"), (dict(x_ld=8 * 64 - 8), "rows"), (dict(y_ld=8 * 64 + 2), "rows"),
-    (dict(y=(1 << 20) + 8), "aligned"), (dict(pos_ld=3), "position"), (dict(y=1 << 20, y_ld=8 * 64 + 8), "strides")])
+    (dict(y=(1 << 20) + 8), "aligned"), (dict(pos_ld=3), "position"), (dict(y=1 << 20, y_ld=8 * 64 + 8), "strides"),
+    (dict(y=(1 << 20) + 1024), "overlap"), (dict(y=(1 << 20) - 1024 * 9), "overlap"), (dict(x_ld=1200, y_ld=1200, y=(1 << 20) + 1008), "overlap"),
+    (dict(x_ld=1200, y_ld=1200, y=(1 << 20) + 2 * 704), "overlap"), (dict(x_ld=1200, y_ld=1208, y=(1 << 20) + 2 * 600), "overlap")])
 def test_rope_refuses(change, words):
     plan = ops.rope_plan((8, 12, 12))
     a = dict(x=1 << 20, x_ld=8 * 64, y=1 << 22, y_ld=8 * 64, pos=1 << 20, pos_ld=10, R=10, W=8 * 64, rot=6, hd=64, dt=L.BF16)
@@ -114,6 +116,16 @@ def test_wrappers_refuse_host_tensors():
                  lambda: ops.attn_window_step(x, cache, n, 4), lambda: ops.rope_fwd(x, n, 8, 16, (8,)), lambda: ops.rope_bwd(x, n, 8, 16, (8,))):
         with pytest.raises(RuntimeError, match="device tensors"):
             call()
+
+
+def test_step_takes_positions_and_sections_together():
+    x, cache, n = torch.zeros(4, 192, device="meta"), torch.zeros(2, 4, 4, 8, 16, device="meta"), torch.zeros(4, dtype=torch.int32, device="meta")
+    fn = ops._window_step.__wrapped__
+    for pos, sections in ((None, (8,)), (torch.zeros(1, 4, dtype=torch.int32, device="meta"), None)):
+        with pytest.MonkeyPatch.context() as m:
+            m.setattr(ops, "_home", lambda *t: 0)
+            with pytest.raises(AssertionError, match="pos and sections"):
+                fn(0, x, cache, n, 4, None, 0, pos, sections, 10000.0, False, False, None, None)
 
 
 def test_structs_match_the_header(tmp_path):

@@ -294,6 +294,9 @@ def test_rope_against_float64(dtype, hd, sections, interleaved):
         assert ops.rope_fwd(view, pos, rot, hd, sections, out=view, **kw) is view
         assert torch.equal(view, y) and (wide[:, :16] == 3).all() and (wide[:, 16 + w:] == 3).all()
         assert torch.equal(ops.rope_fwd(view.copy_(x), pos, rot, hd, sections, **kw), y)
+        both = torch.zeros(r, 2 * w, dtype=dtype, device=DEV)      # from one half of a matrix into the other
+        both[:, :w] = x
+        assert torch.equal(ops.rope_fwd(both[:, :w], pos, rot, hd, sections, out=both[:, w:], **kw), y) and torch.equal(both[:, :w], x)
 
 
 def test_rope_gradient_is_the_adjoint_and_matches_differences():
