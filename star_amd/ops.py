@@ -375,6 +375,7 @@ def attn_bwd(qkv, out, dout, lse, nb, l, h, hd):
 # These calls are short (a decoding step is a few microseconds of GPU time), so their host side is kept lean: no context managers and no
 # keyword calls on the usual path.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _home(first, *rest):
@@ -394,21 +395,16 @@ def _at_home(fn):
     @functools.wraps(fn)
     def call(first, *args, **kw):
         home = _home(first)
-        if home == torch.cuda.current_device():
+        if home == _current_device():
             return fn(home, first, *args, **kw)
         with torch.cuda.device(home):
             return fn(home, first, *args, **kw)
     return call
 
 
-def _call(tag, nbytes, fn, *args):
-    if PROFILER is None:
-        rc = fn(*args)
-    else:
-        with _timed(tag, 0.0, float(nbytes)):
-            rc = fn(*args)
-    if rc:
-        L.check(rc)
+def _profiled(tag, nbytes, fn, *args):
+    with _timed(tag, 0.0, float(nbytes)):
+        return fn(*args)
 
 
 def _rows2d(t, shape, name):
@@ -456,13 +452,15 @@ def _rope(home, x, pos, rot_heads, hd, sections, base, per_axis, interleaved, ou
     plan = rope_plan(tuple(sections), base, per_axis, interleaved)
     pos, pos_ld = _positions(pos, plan.axes, r)
     if out is None:
-        out, out_ld = x.new_empty(shape), w
+        out, out_ld = x.new_empty(r, w), w
     else:
         assert out.shape == shape and out.dtype == x.dtype
         out_ld = _rows2d(out, shape, "out")
     if r:
-        _call("rope", 2 * r * w * x.element_size(), L.lib().star_rope, x.data_ptr(), ld, out.data_ptr(), out_ld, pos.data_ptr(), pos_ld, plan, r, w,
-              rot_heads, hd, inverse, L.dt_of(x), _raw_stream(home))
+        args = (x.data_ptr(), ld, out.data_ptr(), out_ld, pos.data_ptr(), pos_ld, plan, r, w, rot_heads, hd, inverse, L.dt_of(x), _raw_stream(home))
+        rc = L.lib().star_rope(*args) if PROFILER is None else _profiled("rope", 2 * r * w * x.element_size(), L.lib().star_rope, *args)
+        if rc:
+            L.check(rc)
     return out
 
 
@@ -501,7 +499,7 @@ def _window_fwd(home, qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, 
     g = _window(qkv, nb, l, h, hd, h if kv_heads is None else kv_heads, left, right, sinks, offsets, scale)
     r = g.R
     if out is None:
-        out = (qkv.new_empty if offsets is None else qkv.new_zeros)((r, h * hd))     # rows of no sequence stay as they are: zeros here
+        out = qkv.new_empty(r, h * hd) if offsets is None else qkv.new_zeros((r, h * hd))     # rows of no sequence stay as they are: zeros here
     else:
         assert out.shape == (r, h * hd) and out.dtype == qkv.dtype and out.is_contiguous()
     lse = qkv.new_empty((h, r), dtype=torch.float32) if want_lse else None
@@ -509,7 +507,10 @@ def _window_fwd(home, qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, 
         g.out = out.data_ptr()
         if want_lse:
             g.lse = lse.data_ptr()
-        _call("attn_window_fwd", r * (qkv.shape[1] + h * hd) * qkv.element_size(), L.lib().star_attn_window_fwd, g, _raw_stream(home))
+        fn, stream = L.lib().star_attn_window_fwd, _raw_stream(home)
+        rc = fn(g, stream) if PROFILER is None else _profiled("attn_window_fwd", r * (qkv.shape[1] + h * hd) * qkv.element_size(), fn, g, stream)
+        if rc:
+            L.check(rc)
     return out, lse
 
 
@@ -539,7 +540,10 @@ def _window_bwd(home, qkv, out, dout, lse, nb, l, h, hd, kv_heads, left, right, 
         lib = L.lib()
         ws = qkv.new_empty(lib.star_attn_window_bwd_ws(r, nb, l, h, g.KV, hd, g.left, sinks, g.dt), dtype=torch.float32)
         g.out, g.lse, g.dout, g.dqkv, g.ws = out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dqkv.data_ptr(), ws.data_ptr()
-        _call("attn_window_bwd", 2 * r * (qkv.shape[1] + h * hd) * qkv.element_size(), lib.star_attn_window_bwd, g, _raw_stream(home))
+        fn, stream = lib.star_attn_window_bwd, _raw_stream(home)
+        rc = fn(g, stream) if PROFILER is None else _profiled("attn_window_bwd", 2 * r * (qkv.shape[1] + h * hd) * qkv.element_size(), fn, g, stream)
+        if rc:
+            L.check(rc)
     return dqkv
 
 
@@ -567,8 +571,11 @@ def _kv_append(home, qkv, cache, lengths, l, h, sinks, offsets):
     nb, kv, cap, hd = _cache_dims(cache, qkv, shape[1], h, lengths)
     assert offsets is not None or r == nb * l, "%d rows for %d sequences of %d" % (r, nb, l)
     if r and nb:
-        _call("kv_append", 4 * r * kv * hd * qkv.element_size(), L.lib().star_kv_append, qkv.data_ptr(), ld, None if offsets is None else _offsets(offsets, nb),
-              cache.data_ptr(), lengths.data_ptr(), r, nb, l, h, kv, hd, cap, sinks, L.dt_of(qkv), _raw_stream(home))
+        args = (qkv.data_ptr(), ld, None if offsets is None else _offsets(offsets, nb), cache.data_ptr(), lengths.data_ptr(), r, nb, l, h, kv, hd, cap, sinks,
+                L.dt_of(qkv), _raw_stream(home))
+        rc = L.lib().star_kv_append(*args) if PROFILER is None else _profiled("kv_append", 4 * r * kv * hd * qkv.element_size(), L.lib().star_kv_append, *args)
+        if rc:
+            L.check(rc)
     return cache
 
 
@@ -589,7 +596,7 @@ def _window_step(home, qkv, cache, lengths, h, left, sinks, pos, sections, base,
     assert shape[0] == nb, "%d rows for %d cache entries" % (shape[0], nb)
     assert (pos is None) == (sections is None), "a rotation needs pos and sections"
     if out is None:
-        out = qkv.new_empty((nb, h * hd))
+        out = qkv.new_empty(nb, h * hd)
     else:
         assert out.shape == (nb, h * hd) and out.dtype == qkv.dtype and out.is_contiguous()
     if nb:
@@ -605,7 +612,10 @@ def _window_step(home, qkv, cache, lengths, h, left, sinks, pos, sections, base,
             plan = rope_plan(tuple(sections), base, per_axis, interleaved)
             pos, g.pos_ld = _positions(pos, plan.axes, nb)
             g.pos, g.h_rope = pos.data_ptr(), C.pointer(plan)
-        _call("attn_window_step", nb * min(cap, left + 1 + sinks) * 2 * kv * hd * qkv.element_size(), lib.star_attn_window_step, g, _raw_stream(home))
+        fn, stream = lib.star_attn_window_step, _raw_stream(home)
+        rc = fn(g, stream) if PROFILER is None else _profiled("attn_window_step", nb * min(cap, left + 1 + sinks) * 2 * kv * hd * qkv.element_size(), fn, g, stream)
+        if rc:
+            L.check(rc)
     return out
 
 

@@ -586,6 +586,32 @@ def test_many_short_sequences():
     assert torch.equal(cache[1, :, 0, 0], v) and not cache[:, :, :, 1:].any()
 
 
+def test_calls_are_timed_by_the_profiler():
+    g = _gen(61)
+    h, kv, hd, nb, l = 4, 2, 32, 2, 40
+    qkv, dout = _rand(g, nb * l, (h + 2 * kv) * hd), _rand(g, nb * l, h * hd)
+    pos = torch.zeros(1, nb * l, dtype=torch.int32, device=DEV)
+    cache, n = torch.zeros(2, nb, kv, 64, hd, device=DEV), torch.full((nb,), l, dtype=torch.int32, device=DEV)
+
+    def run():
+        x = ops.rope_fwd(qkv, pos, h + kv, hd, (8,))
+        out, lse = ops.attn_window_fwd(x, nb, l, h, hd, kv_heads=kv)
+        grad = ops.attn_window_bwd(x, out, dout, lse, nb, l, h, hd, kv_heads=kv)
+        ops.kv_append(x, cache, n, l, h)
+        return out, grad, ops.attn_window_step(qkv[:nb], cache, n, h)
+
+    want = run()
+    ops.PROFILER = ops.Profiler()
+    try:
+        got = run()
+        torch.cuda.synchronize()
+        tags = [r[0] for r in ops.PROFILER.records]
+    finally:
+        ops.PROFILER = None
+    assert tags == ["rope", "attn_window_fwd", "attn_window_bwd", "kv_append", "attn_window_step"]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_empty_batches():
     none = torch.zeros(0, 192, device=DEV)
     out, lse = ops.attn_window_fwd(none, 2, 0, 4, 16, offsets=torch.zeros(3, dtype=torch.int64, device=DEV))
