@@ -279,28 +279,46 @@ __global__ __launch_bounds__(NT) void step_kernel(StepArgs a) {
     }
 }
 
-// The splits (at most 64) of one (sequence, query head), in their order: a wave per row, a split's weight on a lane.
-template <typename T>
-__global__ __launch_bounds__(KT_) void step_join_kernel(const float* __restrict__ ws, T* __restrict__ out, int rows, int hd, int splits) {
-    const int lane = threadIdx.x & 63, row = blockIdx.x * (KT_ / 64) + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const float* w = ws + (int64_t)row * splits * (hd + 2);
-    const float m = lane < splits ? w[lane * (hd + 2) + hd] : -INFINITY, l = lane < splits ? w[lane * (hd + 2) + hd + 1] : 0.f;
-    const float mn = wave_max(m);
-    const float f = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn), sum = wave_sum(l * f);
-    const float inv = mn == -INFINITY ? 0.f : 1.0f / sum;         // an idle entry saw nothing: zeros
-    // eight splits' rows on their way at a time; lanes past the last split have weight 0 and read its row
-    for (int d = lane; d < hd; d += 64) {
-        float t = 0.f;
-        for (int s0 = 0; s0 < splits; s0 += 8) {
-            float v[8];
+// The splits (at most 64) of one (sequence, query head): a block per row.  Groups of HD / 2 threads take every GR-th split, all on their way before
+// the weights are known; the groups are added in their order.  (32 rows of 128 from 64 splits: XJOINX us; a wave per row that walks the splits eight at
+// a time 14 us.)
+template <typename T, int HD>
+__global__ __launch_bounds__(KT_) void step_join_kernel(const float* __restrict__ ws, T* __restrict__ out, int splits) {
+    constexpr int TR = HD / 2, GR = KT_ / TR, K = 64 / GR > 0 ? 64 / GR : 1;
+    __shared__ float sf[64];
+    __shared__ float so[GR][HD];
+    const int tid = threadIdx.x, lane = tid & 63, g = tid / TR, d = tid % TR * 2;
+    const float* w = ws + (int64_t)blockIdx.x * splits * (HD + 2);
+    float2 v[K];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = w[min(s0 + k, splits - 1) * (hd + 2) + d];
+    for (int k = 0; k < K; ++k) {
+        const int sp = k * GR + g;
+        v[k] = sp < splits ? *reinterpret_cast<const float2*>(w + sp * (HD + 2) + d) : make_float2(0.f, 0.f);
+    }
+    if (tid < 64) {
+        const float m = lane < splits ? w[lane * (HD + 2) + HD] : -INFINITY, l = lane < splits ? w[lane * (HD + 2) + HD + 1] : 0.f;
+        const float mn = wave_max(m);
+        const float f = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn), sum = wave_sum(l * f);
+        sf[lane] = mn == -INFINITY ? 0.f : f / sum;         // an idle entry saw nothing: zeros
+    }
+    __syncthreads();
+    float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (s0 + k < splits) t = __builtin_fmaf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + k)), v[k], t);
+    for (int k = 0; k < K; ++k) {
+        const int sp = k * GR + g;
+        if (sp < splits) {
+            t.x = __builtin_fmaf(sf[sp], v[k].x, t.x);
+            t.y = __builtin_fmaf(sf[sp], v[k].y, t.y);
         }
-        Act<T>::st(out + (int64_t)row * hd + d, t * inv);
+    }
+    so[g][d] = t.x;
+    so[g][d + 1] = t.y;
+    __syncthreads();
+    if (tid < HD) {
+        float r = 0.f;
+#pragma unroll
+        for (int i = 0; i < GR; ++i) r += so[i][tid];
+        Act<T>::st(out + (int64_t)blockIdx.x * HD + tid, r);
     }
 }
 
@@ -371,14 +389,13 @@ template <typename T, int HD> static void step_heads(const StepArgs& a, int G, i
     else if (G == 2) step_launch<T, HD, 2>(a, threads, grid, s);
     else if (G == 4) step_launch<T, HD, 4>(a, threads, grid, s);
     else step_launch<T, HD, 8>(a, threads, grid, s);
+    if (a.splits > 1) hipLaunchKernelGGL((step_join_kernel<T, HD>), dim3((unsigned)(a.NB * a.H)), dim3(KT_), 0, s, a.ws, (T*)a.out, a.splits);
 }
 template <typename T> static void step_run(const StepArgs& a, int hd, int G, int threads, dim3 grid, hipStream_t s) {
     if (hd == 16) step_heads<T, 16>(a, G, threads, grid, s);
     else if (hd == 32) step_heads<T, 32>(a, G, threads, grid, s);
     else if (hd == 64) step_heads<T, 64>(a, G, threads, grid, s);
     else step_heads<T, 128>(a, G, threads, grid, s);
-    if (a.splits > 1)
-        hipLaunchKernelGGL(step_join_kernel<T>, dim3(cdiv((int64_t)a.NB * a.H, KT_ / 64)), dim3(KT_), 0, s, a.ws, (T*)a.out, a.NB * a.H, hd, a.splits);
 }
 
 extern "C" int star_attn_window_step(const StarAttnStep* g, void* stream) {
