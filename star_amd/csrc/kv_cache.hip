@@ -118,8 +118,10 @@ __global__ __launch_bounds__(NT) void step_kernel(StepArgs a) {
     __shared__ float so[NW][G][HD];
     __shared__ float sm[NW][G], sl[NW][G];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int split = blockIdx.x % a.splits, gc = (blockIdx.x / a.splits) % a.chunks;
-    const int hk = (blockIdx.x / (a.splits * a.chunks)) % a.KV, b = blockIdx.x / (a.splits * a.chunks * a.KV);
+    // blocks go to the 8 XCDs in turn: those that read the same rows for other query heads are 8 apart, in one L2
+    const int gc = (blockIdx.x >> 3) % a.chunks, unit = (blockIdx.x >> 3) / a.chunks * 8 + (blockIdx.x & 7);
+    const int split = unit % a.splits, hk = unit / a.splits % a.KV, b = unit / (a.splits * a.KV);
+    if (b >= a.NB) return;
     const int rep = a.H / a.KV, h0 = hk * rep + gc * G, ng = min(G, rep - gc * G);
     const int len = max(0, a.lengths[b]);
     const Seen seen(len, a.left, a.sinks, a.cap);
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(NT) void step_kernel(StepArgs a) {
 }
 
 // The splits (at most 64) of one (sequence, query head): a block per row.  Groups of HD / 2 threads take every GR-th split, all on their way before
-// the weights are known; the groups are added in their order.  (32 rows of 128 from 64 splits: XJOINX us; a wave per row that walks the splits eight at
+// the weights are known; the groups are added in their order.  (32 rows of 128 from 64 splits: 3.8 us; a wave per row that walks the splits eight at
 // a time 14 us.)
 template <typename T, int HD>
 __global__ __launch_bounds__(KT_) void step_join_kernel(const float* __restrict__ ws, T* __restrict__ out, int splits) {
@@ -347,17 +349,19 @@ extern "C" int star_kv_append(const void* qkv, int64_t ld, const int64_t* offset
 }
 
 // Query heads of a key head that one block serves: they share every row it reads, but its one or two rounds of rows cost the more arithmetic.  More
-// than two only where the key heads alone fill the chip (1 sequence, 32 heads of 128 on 8, 1000 tokens: 14.4 us with four, 11.8 with two; 16 x 8 heads of
-// 64 on 1, 2000 tokens: 19.8 with eight, 14.3 with four, 13.4 with two; 8 x 32 on 8, 4096 tokens: 37.1 with four, 33.6 with two, 83.6 with one).
+// than two only where the key heads alone fill the chip (1 sequence, 32 heads of 128 on 8, 1000 tokens: 11.8 us with four, 9.1 with two, 8.5 with one; 16 x
+// 8 heads of 64 on 1, 2000 tokens: 12.8, 11.7, 11.0; 8 x 32 on 8, 4096 tokens: 33.6, 31.5, 82.3).
 static int step_group(int NB, int H, int KV) {
     const int rep = H / KV;
     if ((int64_t)NB * KV < star_num_cus()) return rep > 1 ? 2 : 1;
     return rep > 4 ? 8 : rep > 2 ? 4 : rep;
 }
-// Threads of a block and splits.  Where there is a block per compute unit, or three rounds of a wide block take all rows, a wide block takes the
-// whole sequence: one launch (5 sequences, 12 heads of 64, 300 visible tokens 6.9 us against 8.2 with narrow blocks, splits and their join; 32 x 8 heads of 128, 500
-// tokens 21 against 25).  Else few (sequence, key head) pairs would leave the chip idle: narrow blocks, the tokens split until there are about
-// four of them per compute unit (8 heads of 128, 4096 tokens 25 us against 70).
+// Threads of a block and splits.  A wide block takes a whole sequence, in one launch, where three rounds of its rows hold it (5 sequences, 12 heads of
+// 64, 1000 tokens: 8.6 us against 8.1 with narrow blocks, splits and their join, but a second launch takes the host 4 us longer: 10.4 against 14.6
+// called one by one), and where the blocks fill every round of the compute units to nine tenths (64 sequences, 12 heads of 64, 1000 tokens: equal).
+// Else narrow blocks, the tokens split until there are about four per compute unit for few (sequence, key head) pairs, eight for many (8 sequences,
+// 32 heads on 8 of 128, 1000 tokens 14.9 us against 18.2 with eight; 33 x 8 heads of 128, 6000 tokens 152 us, 195 with whole sequences, which
+// leave the second round of compute units nearly empty); no more splits than hold rows.
 struct StepPlan {
     int threads, splits;
 };
@@ -366,11 +370,13 @@ static StepPlan step_plan(int NB, int H, int KV, int hd, int es, int cap, int le
     const int64_t blocks = (int64_t)NB * KV * cdiv(rep, G);
     const int64_t vis = (int64_t)left + 1 + sinks < cap ? (int64_t)left + 1 + sinks : cap;
     const int per = 4 * 64 / (hd * es / 16);              // rows of a wave's round
-    if (blocks >= star_num_cus() || vis <= 3 * per * (wide / 64)) return {wide, 1};
+    const int64_t cus = star_num_cus();
+    if (vis <= 3 * per * (wide / 64) || (blocks >= cus && blocks * 10 >= cdiv(blocks, cus) * cus * 9)) return {wide, 1};
     const int64_t rounds = (vis + per * 4 - 1) / (per * 4);
-    int64_t s = (4 * (int64_t)star_num_cus() + blocks - 1) / blocks;
-    if (s > rounds) s = rounds;
-    return {KT_, (int)(s < 1 ? 1 : s > 64 ? 64 : s)};
+    int64_t s = ((blocks < cus ? 4 : 8) * cus + blocks - 1) / blocks;
+    s = s < 1 ? 1 : s > 64 ? 64 : s > rounds ? rounds : s;
+    const int64_t each = (rounds + s - 1) / s;
+    return {KT_, (int)((rounds + each - 1) / each)};
 }
 
 extern "C" int64_t star_attn_window_step_ws(int NB, int H, int KV, int hd, int cap, int left, int sinks, int dt) {
@@ -424,7 +430,7 @@ extern "C" int star_attn_window_step(const StarAttnStep* g, void* stream) {
     const StepPlan plan = step_plan(g->NB, g->H, g->KV, g->hd, es, g->cap, g->left, g->sinks);
     a.splits = plan.splits;
     STAR_CHECK(a.splits == 1 || g->ws, "star_attn_window_step: null workspace (star_attn_window_step_ws)");
-    const int64_t blocks = (int64_t)g->NB * g->KV * a.chunks * a.splits;
+    const int64_t blocks = ((int64_t)g->NB * g->KV * a.splits + 7) / 8 * 8 * a.chunks;
     STAR_CHECK(blocks < (1ll << 31), "star_attn_window_step: NB, KV too large for the grid");
     hipStream_t s = (hipStream_t)stream;
     if (g->dt == STAR_BF16) step_run<bf16_t>(a, g->hd, G, plan.threads, dim3((unsigned)blocks), s);

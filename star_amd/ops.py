@@ -433,6 +433,12 @@ def rope_plan(sections, base=10000.0, per_axis=False, interleaved=False):
     return f
 
 
+@functools.lru_cache(maxsize=256)
+def _rope_ref(sections, base, per_axis, interleaved):
+    plan = rope_plan(sections, base, per_axis, interleaved)
+    return C.pointer(plan), plan.axes
+
+
 def _positions(pos, axes, r):
     if pos.dim() == 1:
         pos = pos.unsqueeze(0)
@@ -587,6 +593,11 @@ def kv_append(qkv, cache, lengths, l, h, sinks=0, offsets=None):
     return _kv_append(qkv, cache, lengths, l, h, sinks, offsets)
 
 
+@functools.lru_cache(maxsize=1024)
+def _step_ws(home, *args):
+    return L.lib().star_attn_window_step_ws(*args)
+
+
 @_at_home
 def _window_step(home, qkv, cache, lengths, h, left, sinks, pos, sections, base, per_axis, interleaved, scale, out):
     _home(qkv, cache, lengths, pos, out)
@@ -604,14 +615,14 @@ def _window_step(home, qkv, cache, lengths, h, left, sinks, pos, sections, base,
         if left is None:
             left = cap - sinks - 1
         dt = L.dt_of(qkv)
-        need = lib.star_attn_window_step_ws(nb, h, kv, hd, cap, left, sinks, dt)
+        need = _step_ws(home, nb, h, kv, hd, cap, left, sinks, dt)
         ws = qkv.new_empty(need, dtype=torch.float32) if need else None
         g = L.StarAttnStep(qkv.data_ptr(), cache.data_ptr(), lengths.data_ptr(), None, None, out.data_ptr(), None if ws is None else ws.data_ptr(), ld, 0, nb, h, kv,
                            hd, cap, left, sinks, hd ** -0.5 if scale is None else scale, dt)
         if sections is not None:
-            plan = rope_plan(tuple(sections), base, per_axis, interleaved)
-            pos, g.pos_ld = _positions(pos, plan.axes, nb)
-            g.pos, g.h_rope = pos.data_ptr(), C.pointer(plan)
+            g.h_rope, axes = _rope_ref(tuple(sections), base, per_axis, interleaved)
+            pos, g.pos_ld = _positions(pos, axes, nb)
+            g.pos = pos.data_ptr()
         fn, stream = lib.star_attn_window_step, _raw_stream(home)
         rc = fn(g, stream) if PROFILER is None else _profiled("attn_window_step", nb * min(cap, left + 1 + sinks) * 2 * kv * hd * qkv.element_size(), fn, g, stream)
         if rc:
