@@ -66,13 +66,33 @@ struct StepArgs {
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
     return v + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xf, 0xf, true));
 }
+__device__ __forceinline__ float swap16_add(float v) {          // + lane ^ 16
+    typedef __attribute__((ext_vector_type(2))) unsigned u2;
+    const u2 x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
 template <int LPR> __device__ __forceinline__ float lane_sum(float v) {
     if constexpr (LPR >= 2) v = dpp_add<0xB1>(v);        // quad_perm 1,0,3,2
     if constexpr (LPR >= 4) v = dpp_add<0x4E>(v);        // quad_perm 2,3,0,1
     if constexpr (LPR >= 8) v = dpp_add<0x141>(v);       // row_half_mirror: the other quad of eight
     if constexpr (LPR >= 16) v = dpp_add<0x140>(v);      // row_mirror: the other eight of sixteen
-    if constexpr (LPR >= 32) v += __shfl_xor(v, 16, 64);
+    if constexpr (LPR >= 32) v = swap16_add(v);
     return v;
+}
+// op over the 64 / LPR lanes that hold the same chunk of other rows (lane % LPR), in every one of them: rotations within 16 lanes, then swaps
+// (a shuffle through LDS costs several times as much, and a block has 16 waves and up to 8 heads to join)
+template <int CTRL> __device__ __forceinline__ float dpp_get(float v) { return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xf, 0xf, true)); }
+template <int LPR, class OP> __device__ __forceinline__ float over_rows(float v, OP op) {
+    typedef __attribute__((ext_vector_type(2))) unsigned u2;
+    if constexpr (LPR <= 8) v = op(v, dpp_get<0x128>(v));          // row_ror 8, 4, 2
+    if constexpr (LPR <= 4) v = op(v, dpp_get<0x124>(v));
+    if constexpr (LPR <= 2) v = op(v, dpp_get<0x122>(v));
+    if constexpr (LPR <= 16) {
+        const u2 x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = op(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    }
+    const u2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(x[0]), __uint_as_float(x[1]));
 }
 template <typename T> __device__ __forceinline__ void unpack(uint4 w, float (&v)[16 / sizeof(T)]) {
     const unsigned x[4] = {w.x, w.y, w.z, w.w};
@@ -233,20 +253,16 @@ __global__ __launch_bounds__(NT) void step_kernel(StepArgs a) {
         }
     }
     // join the row groups of the wave, then the waves
+    auto add = [](float x, float y) { return x + y; };
+    auto larger = [](float x, float y) { return fmaxf(x, y); };
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-        float mn = m[g];
-#pragma unroll
-        for (int x = LPR; x < 64; x <<= 1) mn = fmaxf(mn, __shfl_xor(mn, x, 64));
+        const float mn = over_rows<LPR>(m[g], larger);
         const float ref = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(m[g] - ref);
-        float ls = l[g] * f;
-#pragma unroll
-        for (int x = LPR; x < 64; x <<= 1) ls += __shfl_xor(ls, x, 64);
+        const float ls = over_rows<LPR>(l[g] * f, add);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            float t = o[g][e] * f;
-#pragma unroll
-            for (int x = LPR; x < 64; x <<= 1) t += __shfl_xor(t, x, 64);
+            const float t = over_rows<LPR>(o[g][e] * f, add);
             if (lane < LPR) so[wave][g][ch * E + e] = t;
         }
         if (lane == 0) {
