@@ -254,6 +254,8 @@ typedef struct StarAttnWindow {
     int32_t NB, L, H, KV, hd, left, right, sinks;
     float scale;
     int32_t dt;
+    int32_t zero_rest;        /* with offsets: != 0 sets the rows of out (forward) and dqkv (backward) that no sequence holds to zero */
+    int32_t reserved;
 } StarAttnWindow;
 int star_attn_window_fwd(const StarAttnWindow* g, void* stream);
 int64_t star_attn_window_bwd_ws(int64_t R, int NB, int L, int H, int KV, int hd, int left, int sinks, int dt);

@@ -45,7 +45,8 @@ class StarRope(C.Structure):
 class StarAttnWindow(C.Structure):
     _fields_ = [("qkv", C.c_void_p), ("offsets", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("dout", C.c_void_p), ("dqkv", C.c_void_p),
                 ("ws", C.c_void_p), ("ld", C.c_int64), ("R", C.c_int64), ("NB", C.c_int32), ("L", C.c_int32), ("H", C.c_int32), ("KV", C.c_int32),
-                ("hd", C.c_int32), ("left", C.c_int32), ("right", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float), ("dt", C.c_int32)]
+                ("hd", C.c_int32), ("left", C.c_int32), ("right", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float), ("dt", C.c_int32),
+                ("zero_rest", C.c_int32), ("reserved", C.c_int32)]
 
 
 class StarAttnStep(C.Structure):

@@ -285,6 +285,7 @@ struct WArgs {
     int NB, L, H, KV, left, right, sinks;
     float scale;
     int far_groups, far_parts;
+    int rest_blocks;         // blocks at the grid's end that zero the rows of no sequence
 };
 
 // rows of sequence b.  The device-side offsets cannot be checked by the host: whatever they hold, rows stay inside [0, R) and a
@@ -301,6 +302,31 @@ __device__ __forceinline__ int seq_rows(const WArgs& a, int b, int64_t& start) {
     return (int)(e - s > a.L ? a.L : e - s);
 }
 
+// Zeros in the rows [R, width] of y that no sequence holds: in front of the first, behind the last, and those of a sequence past its first L.
+template <typename T> __device__ __forceinline__ void zero_rest(const WArgs& a, T* y, int64_t width) {
+    const int part = blockIdx.x - (gridDim.x - a.rest_blocks), tid = threadIdx.x, lane = tid & 63;
+    const int64_t chunks = width * sizeof(T) / 16, R = a.R;
+    uint4* out = reinterpret_cast<uint4*>(y);
+    auto fill = [&](int64_t lo, int64_t hi, int64_t first, int64_t step) {
+        for (int64_t i = lo * chunks + first; i < hi * chunks; i += step) out[i] = make_uint4(0, 0, 0, 0);
+    };
+    const int64_t s0 = a.offsets[0], e0 = a.offsets[a.NB];
+    fill(0, s0 < 0 ? 0 : s0 > R ? R : s0, part * WT + tid, (int64_t)a.rest_blocks * WT);
+    fill(e0 < 0 ? 0 : e0 > R ? R : e0, R, part * WT + tid, (int64_t)a.rest_blocks * WT);
+    for (int64_t b0 = (int64_t)(part * (WT / 64) + (tid >> 6)) * 64; b0 < a.NB; b0 += (int64_t)a.rest_blocks * WT) {
+        int64_t lo = 0, hi = 0;
+        if (b0 + lane < a.NB) {
+            const int64_t s = a.offsets[b0 + lane], e = a.offsets[b0 + lane + 1];
+            lo = (s < 0 ? 0 : s > R ? R : s) + a.L;
+            hi = e > R ? R : e;
+        }
+        for (unsigned long long left = __builtin_amdgcn_ballot_w64(hi > lo); left; left &= left - 1) {
+            const int i = __builtin_ctzll(left);
+            fill(__shfl(lo, i, 64), __shfl(hi, i, 64), lane, 64);
+        }
+    }
+}
+
 // Block -> (stream = one head of one sequence, row block).  The row blocks of a stream stay on one XCD and share its L2.  Sequences of one
 // length: every XCD walks a contiguous range of streams, which balances at any count; `side` streams go row block by row block together (the
 // query heads of a group, which read the same keys: prefill of 8192 rows, 32 heads on 8, 532 -> 493 us; unrelated heads gain nothing).  Ragged with enough streams: they are dealt to the
@@ -315,7 +341,7 @@ __device__ __forceinline__ bool place(const WArgs& a, int rows, int streams, int
         rblk = i % nrb;
         return stream < streams;
     }
-    const int work = xcd_remap(blockIdx.x, gridDim.x), set = work / (nrb * side), rest = work - set * nrb * side;
+    const int work = xcd_remap(blockIdx.x, gridDim.x - a.rest_blocks), set = work / (nrb * side), rest = work - set * nrb * side;
     stream = set * side + rest % side;
     rblk = rest / side;
     return true;
@@ -486,6 +512,7 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_FWD(sizeof(T) * 
     constexpr int ROWS = SPLIT ? 32 : WROWS, STEP = SPLIT ? 4 : 1;
     using Ring = KvRing<C>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    if (a.rest_blocks && blockIdx.x >= gridDim.x - a.rest_blocks) return zero_rest(a, (T*)a.out, (int64_t)a.H * HD);
     int stream, rblk;
     if (!place(a, ROWS, a.NB * a.H, a.H / a.KV, stream, rblk)) return;
     const int h = stream % a.H, b = stream / a.H;
@@ -629,6 +656,7 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DQ(sizeof(T) * H
     constexpr int ROWS = SPLIT ? 32 : WROWS, STEP = SPLIT ? 4 : 1;
     using Ring = KvRing<C>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    if (a.rest_blocks && blockIdx.x >= gridDim.x - a.rest_blocks) return zero_rest(a, (T*)a.dqkv, (int64_t)(a.H + 2 * a.KV) * HD);
     int stream, rblk;
     if (!place(a, ROWS, a.NB * a.H, a.H / a.KV, stream, rblk)) return;
     const int h = stream % a.H, b = stream / a.H;
@@ -1050,12 +1078,12 @@ static bool few_blocks(const WArgs& a, int heads, int eighths) {
 template <typename T, int HD, bool SPLIT> static int launch_fwd(const WArgs& a, hipStream_t s) {
     using Ring = KvRing<RowCfg<T, HD, SPLIT>>;
     constexpr int LDS = SPLIT ? 4 * Ring::BYTES : Ring::BYTES;
-    return launch<window_fwd_kernel<T, HD, SPLIT>>("star_attn_window_fwd", grid_of(a, SPLIT ? 32 : WROWS, a.H), SPLIT && LDS < 18432 ? 18432 : LDS, a, s);
+    return launch<window_fwd_kernel<T, HD, SPLIT>>("star_attn_window_fwd", grid_of(a, SPLIT ? 32 : WROWS, a.H) + a.rest_blocks, SPLIT && LDS < 18432 ? 18432 : LDS, a, s);
 }
 template <typename T, int HD, bool SPLIT> static int launch_dq(const WArgs& a, hipStream_t s) {
     using Ring = KvRing<RowCfg<T, HD, SPLIT>>;
     constexpr int LDS = SPLIT ? 4 * Ring::BYTES : Ring::BYTES;
-    return launch<window_dq_kernel<T, HD, SPLIT>>("star_attn_window_bwd", grid_of(a, SPLIT ? 32 : WROWS, a.H), SPLIT && LDS < 18432 ? 18432 : LDS, a, s);
+    return launch<window_dq_kernel<T, HD, SPLIT>>("star_attn_window_bwd", grid_of(a, SPLIT ? 32 : WROWS, a.H) + a.rest_blocks, SPLIT && LDS < 18432 ? 18432 : LDS, a, s);
 }
 template <typename T, int HD, int FORM> static int launch_dkv(const WArgs& a, hipStream_t s) {
     constexpr bool OWN = FORM != ROW_FORM;
@@ -1082,10 +1110,12 @@ template <typename T, int HD> static int run_dkv(const WArgs& a, hipStream_t s) 
         if (few_blocks(a, a.KV, S::KEYS)) return launch_dkv<T, HD, SPLIT_FORM>(a, s);
     return launch_dkv<T, HD, ROW_FORM>(a, s);
 }
-template <typename T, int HD> static int run_bwd(const WArgs& a, hipStream_t s) {
+template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t s) {
     const char* who = "star_attn_window_bwd";
-    int rc = run_dq<T, HD>(a, s);
+    int rc = run_dq<T, HD>(first, s);
     if (rc) return rc;
+    WArgs a = first;
+    a.rest_blocks = 0;
     if constexpr (SplitUpTo<T, HD>::EVER)
         if (a.far_parts) {
             if ((rc = launch_dkv<T, HD, FAR_FORM>(a, s))) return rc;
@@ -1128,11 +1158,18 @@ static int window_args(const char* who, const StarAttnWindow* g, WArgs& a) {
                "%s: qkv rows of %lld elements must hold all heads and be 16-byte aligned", who, (long long)g->ld);
     STAR_CHECK(g->ld * es < (1 << 24), "%s: qkv rows %lld elements apart", who, (long long)g->ld);       // a tile's offsets are 32 bits
     STAR_CHECK((uintptr_t)g->out % 16 == 0, "%s: out must be 16-byte aligned", who);
-    STAR_CHECK((int64_t)cdiv(g->L, 32) * ((int64_t)g->H * g->NB + 7) < (1ll << 31), "%s: NB, H, L too large for the grid", who);
+    STAR_CHECK((int64_t)cdiv(g->L, 32) * ((int64_t)g->H * g->NB + 7) < (1ll << 31) - 1024, "%s: NB, H, L too large for the grid", who);
     // a bound over L says the same as L: what is left cannot overflow in i + right and i - left
     a = WArgs{g->qkv, g->offsets, g->out, g->lse, nullptr, nullptr, nullptr, nullptr, g->ld, g->R, g->NB, g->L, g->H, g->KV,
-              g->left < g->L ? g->left : g->L, g->right < g->L ? g->right : g->L, g->sinks < g->L ? g->sinks : g->L, g->scale, 0, 0};
+              g->left < g->L ? g->left : g->L, g->right < g->L ? g->right : g->L, g->sinks < g->L ? g->sinks : g->L, g->scale, 0, 0, 0};
     return 0;
+}
+// a block per 256 KiB of a matrix of R rows that is to be zeroed outside the sequences (most of it is inside as a rule): a fill of the whole
+// costs a launch and all its bytes
+static int rest_blocks(const StarAttnWindow* g, int64_t width) {
+    if (!g->offsets || !g->zero_rest) return 0;
+    const int64_t n = g->R * width * (g->dt == STAR_BF16 ? 2 : 4) >> 18;
+    return n < 1 ? 1 : n > 512 ? 512 : (int)n;
 }
 
 #define BY_HD(F, T)                                                                         \
@@ -1141,6 +1178,7 @@ static int window_args(const char* who, const StarAttnWindow* g, WArgs& a) {
 extern "C" int star_attn_window_fwd(const StarAttnWindow* g, void* stream) {
     WArgs a;
     if (int rc = window_args("star_attn_window_fwd", g, a)) return rc;
+    a.rest_blocks = rest_blocks(g, (int64_t)g->H * g->hd);
     hipStream_t s = (hipStream_t)stream;
     return g->dt == STAR_BF16 ? BY_HD(run_fwd, bf16_t) : BY_HD(run_fwd, float);
 }
@@ -1160,6 +1198,7 @@ extern "C" int star_attn_window_bwd(const StarAttnWindow* g, void* stream) {
     a.dout = g->dout;
     a.dqkv = g->dqkv;
     a.ndelta = g->ws;
+    a.rest_blocks = rest_blocks(g, (int64_t)(g->H + 2 * g->KV) * g->hd);
     far_plan(g->NB, g->L, g->H, g->KV, g->hd * (g->dt == STAR_BF16 ? 2 : 4), g->left, g->sinks, a.far_groups, a.far_parts);
     a.far_ws = g->ws + (g->H * g->R + 63) / 64 * 64;
     hipStream_t s = (hipStream_t)stream;

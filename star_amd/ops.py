@@ -505,7 +505,8 @@ def _window_fwd(home, qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, 
     g = _window(qkv, nb, l, h, hd, h if kv_heads is None else kv_heads, left, right, sinks, offsets, scale)
     r = g.R
     if out is None:
-        out = qkv.new_empty(r, h * hd) if offsets is None else qkv.new_zeros((r, h * hd))     # rows of no sequence stay as they are: zeros here
+        out = qkv.new_empty(r, h * hd)
+        g.zero_rest = offsets is not None          # rows of no sequence stay as they are in a given out; here they become zeros
     else:
         assert out.shape == (r, h * hd) and out.dtype == qkv.dtype and out.is_contiguous()
     lse = qkv.new_empty((h, r), dtype=torch.float32) if want_lse else None
@@ -524,8 +525,8 @@ def attn_window_fwd(qkv, nb, l, h, hd, kv_heads=None, left=None, right=0, sinks=
     """Sliding-window attention with sinks.  qkv [R, (h + 2 kv_heads) hd]: packed rows (bf16 / float32, dense rows that may lie apart), query head i
     reads key/value head i // (h // kv_heads).  Key j is visible to query i iff j <= i + right and (j >= i - left or j < sinks); None: no
     bound (right=0: causal; left=right=None: everything).  nb sequences of l rows, or ragged: offsets int64 [nb + 1] on the device, l >= the
-    longest sequence (of a longer one only the first l rows take part).  Rows outside every sequence are neither read nor written, and what a
-    row does not see does not reach its result, infinities and NaN included (rows that meet such in a tile cost more time).
+    longest sequence (of a longer one only the first l rows take part).  Rows outside every sequence are neither read nor written (zeros in an
+    out that is made here), and what a row does not see does not reach its result, infinities and NaN included (rows that meet such in a tile cost more time).
     -> (out [R, h*hd], lse float32 [h, R] or None)"""
     return _window_fwd(qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale, want_lse, out)
 
@@ -539,7 +540,8 @@ def _window_bwd(home, qkv, out, dout, lse, nb, l, h, hd, kv_heads, left, right, 
         assert t.shape == (r, h * hd) and t.dtype == qkv.dtype and t.is_contiguous()
     assert lse.shape == (h, r) and lse.dtype == torch.float32 and lse.is_contiguous()
     if dqkv is None:
-        dqkv = (qkv.new_empty if offsets is None else qkv.new_zeros)(qkv.shape)
+        dqkv = qkv.new_empty(qkv.shape)
+        g.zero_rest = offsets is not None
     else:
         assert dqkv.shape == qkv.shape and dqkv.dtype == qkv.dtype and dqkv.is_contiguous()
     if r:

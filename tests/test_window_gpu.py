@@ -137,6 +137,35 @@ def test_ragged_batch_leaves_rows_outside_every_sequence(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,l,front,back", [([5, 0, 90], 90, 700, 0), ([40, 7, 33], 20, 0, 1500), ([3, 70, 1, 0, 64, 65] * 120, 33, 5, 9), ([0, 0], 4, 0, 0), ([10], 10, 0, 0)])
+def test_rows_of_no_sequence_become_zeros(dtype, lens, l, front, back):
+    """in matrices that the calls make, whose memory held something else before: rows in front, behind, and of sequences over l rows"""
+    g = _gen(len(lens) + l)
+    h, kv, hd, rows = 4, 2, 32, front + sum(lens) + back
+    if rows == 0:
+        front, rows = 3, 3
+    w = (h + 2 * kv) * hd
+    qkv, dout = _rand(g, rows, w, dtype=dtype), _rand(g, rows, h * hd, dtype=dtype)
+    at = [front]
+    inside = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    for n in lens:
+        inside[at[-1]:at[-1] + min(n, l)] = True
+        at.append(at[-1] + n)
+    offsets = torch.tensor(at, device=DEV)
+    kw = dict(kv_heads=kv, left=20, sinks=2, offsets=offsets)
+    kept, grad = torch.zeros(rows, h * hd, dtype=dtype, device=DEV), torch.zeros(rows, w, dtype=dtype, device=DEV)
+    _, lse = ops.attn_window_fwd(qkv, len(lens), l, h, hd, out=kept, **kw)
+    ops.attn_window_bwd(qkv, kept, dout, lse, len(lens), l, h, hd, dqkv=grad, **kw)
+    for _ in range(3):
+        poison = [torch.full((rows, c), float("nan"), dtype=dtype, device=DEV) for c in (h * hd, w) for _ in range(2)]
+        del poison
+        out, lse = ops.attn_window_fwd(qkv, len(lens), l, h, hd, **kw)
+        dqkv = ops.attn_window_bwd(qkv, out, dout, lse, len(lens), l, h, hd, **kw)
+        assert not out[~inside].any() and not dqkv[~inside].any()
+        assert torch.equal(out, kept) and torch.equal(dqkv, grad)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hd", [16, 64, 128])
 @pytest.mark.parametrize("nb", [1, 40])
 @pytest.mark.parametrize("window", [(None, 0, 0), (20, 0, 0), (33, 7, 0), (40, 0, 3)])
