@@ -928,15 +928,17 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DKV(sizeof(T) * 
     f32x16_t dk[C::DB], dv[C::DB];
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) dk[db] = dv[db] = splat16(0.f);
-    if (!FAR && a.far_parts && k0 < min(a.sinks, len) && (!OWN || wave == 0)) {
+    constexpr bool ADD = OWN && C::RB < 256;          // a split block's waves each add up a share of the far parts; else they come folded, to one wave
+    if (!FAR && a.far_parts && k0 < min(a.sinks, len) && (ADD || !OWN || wave == 0)) {
         const float* w = a.far_ws + ((int64_t)(b * a.KV + hk) * a.far_groups + k0 / 32) * a.far_parts * (2 * C::DB * 1024) + lane;
+        for (int p = ADD ? wave : 0; p < (ADD ? a.far_parts : 1); p += 4)
 #pragma unroll
-        for (int db = 0; db < C::DB; ++db)
+            for (int db = 0; db < C::DB; ++db)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                dk[db][e] = w[(db * 16 + e) * 64];
-                dv[db][e] = w[((C::DB + db) * 16 + e) * 64];
-            }
+                for (int e = 0; e < 16; ++e) {
+                    dk[db][e] += w[(int64_t)p * (2 * C::DB * 1024) + (db * 16 + e) * 64];
+                    dv[db][e] += w[(int64_t)p * (2 * C::DB * 1024) + ((C::DB + db) * 16 + e) * 64];
+                }
     }
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) asm volatile("" : "+v"(dk[db]), "+v"(dv[db]));
@@ -1119,7 +1121,9 @@ template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t
     if constexpr (SplitUpTo<T, HD>::EVER)
         if (a.far_parts) {
             if ((rc = launch_dkv<T, HD, FAR_FORM>(a, s))) return rc;
-            if (a.far_parts > 1) {
+            // the split form adds the parts up itself where a row is under 256 bytes (7 sequences of 0 .. 2043 rows, 16 heads on 4 of 64: 122 us against
+            // 128; 128-wide heads have too few registers to keep the loads in flight: 102 against 48)
+            if (a.far_parts > 1 && !(HD * sizeof(T) < 256 && few_blocks(a, a.KV, SplitUpTo<T, HD>::KEYS))) {
                 const int size = 2 * WCfg<T, HD>::DB * 1024;
                 hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, a.NB * a.KV * a.far_groups), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
                 STAR_LAUNCH_CHECK(who);
