@@ -1149,6 +1149,7 @@ static void far_plan(int NB, int L, int H, int KV, int row_bytes, int left, int 
     parts = p < 1 ? 1 : p > 16 ? 16 : (int)p;
 }
 
+static int longest(int L, int64_t R) { return L < R ? L : R < 1 ? 1 : (int)R; }
 static int window_args(const char* who, const StarAttnWindow* g, WArgs& a) {
     STAR_CHECK(g && g->qkv && g->out, "%s: null pointer", who);
     STAR_CHECK(g->dt == STAR_BF16 || g->dt == STAR_F32, "%s: dtype %d is neither STAR_BF16 nor STAR_F32", who, g->dt);
@@ -1164,10 +1165,11 @@ static int window_args(const char* who, const StarAttnWindow* g, WArgs& a) {
                "%s: qkv rows of %lld elements must hold all heads and be 16-byte aligned", who, (long long)g->ld);
     STAR_CHECK(g->ld * es < (1 << 24), "%s: qkv rows %lld elements apart", who, (long long)g->ld);       // a tile's offsets are 32 bits
     STAR_CHECK((uintptr_t)g->out % 16 == 0, "%s: out must be 16-byte aligned", who);
-    STAR_CHECK((int64_t)cdiv(g->L, 32) * ((int64_t)g->H * g->NB + 7) < (1ll << 31) - 1024, "%s: NB, H, L too large for the grid", who);
-    // a bound over L says the same as L: what is left cannot overflow in i + right and i - left
-    a = WArgs{g->qkv, g->offsets, g->out, g->lse, nullptr, nullptr, nullptr, nullptr, g->ld, g->R, g->NB, g->L, g->H, g->KV,
-              g->left < g->L ? g->left : g->L, g->right < g->L ? g->right : g->L, g->sinks < g->L ? g->sinks : g->L, g->scale, 0, 0, 0};
+    STAR_CHECK((int64_t)cdiv(longest(g->L, g->R), 32) * ((int64_t)g->H * g->NB + 7) < (1ll << 31) - 1024, "%s: NB, H, L too large for the grid", who);
+    // a bound over L says the same as L (what is left cannot overflow in i + right and i - left), and L over all rows the same as R: no blocks for those
+    const int L = longest(g->L, g->R);
+    a = WArgs{g->qkv, g->offsets, g->out, g->lse, nullptr, nullptr, nullptr, nullptr, g->ld, g->R, g->NB, L, g->H, g->KV,
+              g->left < L ? g->left : L, g->right < L ? g->right : L, g->sinks < L ? g->sinks : L, g->scale, 0, 0, 0};
     return 0;
 }
 // a block per 256 KiB of a matrix of R rows that is to be zeroed outside the sequences (most of it is inside as a rule): a fill of the whole
@@ -1192,7 +1194,7 @@ extern "C" int star_attn_window_fwd(const StarAttnWindow* g, void* stream) {
 extern "C" int64_t star_attn_window_bwd_ws(int64_t R, int NB, int L, int H, int KV, int hd, int left, int sinks, int dt) {
     if (R < 0 || NB <= 0 || L <= 0 || H <= 0 || KV <= 0 || H % KV || hd <= 0 || left < 0 || sinks < 0) return 0;
     int groups, parts;
-    far_plan(NB, L, H, KV, hd * (dt == STAR_BF16 ? 2 : 4), left, sinks, groups, parts);
+    far_plan(NB, longest(L, R), H, KV, hd * (dt == STAR_BF16 ? 2 : 4), left, sinks, groups, parts);
     return (H * R + 63) / 64 * 64 + (int64_t)NB * KV * groups * parts * 2 * 32 * (hd < 32 ? 32 : hd);
 }
 
@@ -1205,7 +1207,7 @@ extern "C" int star_attn_window_bwd(const StarAttnWindow* g, void* stream) {
     a.dqkv = g->dqkv;
     a.ndelta = g->ws;
     a.rest_blocks = rest_blocks(g, (int64_t)(g->H + 2 * g->KV) * g->hd);
-    far_plan(g->NB, g->L, g->H, g->KV, g->hd * (g->dt == STAR_BF16 ? 2 : 4), g->left, g->sinks, a.far_groups, a.far_parts);
+    far_plan(g->NB, a.L, g->H, g->KV, g->hd * (g->dt == STAR_BF16 ? 2 : 4), g->left, g->sinks, a.far_groups, a.far_parts);
     a.far_ws = g->ws + (g->H * g->R + 63) / 64 * 64;
     hipStream_t s = (hipStream_t)stream;
     return g->dt == STAR_BF16 ? BY_HD(run_bwd, bf16_t) : BY_HD(run_bwd, float);

@@ -353,6 +353,7 @@ extern "C" int star_kv_append(const void* qkv, int64_t ld, const int64_t* offset
     STAR_CHECK(R >= 0 && (offsets || R == (int64_t)NB * L), "star_kv_append: %lld rows for %d sequences of %d", (long long)R, NB, L);
     STAR_CHECK(ld * es % 16 == 0 && (uintptr_t)qkv % 16 == 0 && (uintptr_t)cache % 16 == 0, "star_kv_append: rows and cache must be 16-byte aligned");
     if (L == 0 || R == 0) return 0;
+    if (L > R) L = (int)R;          // ragged: no sequence has more
     const AppendArgs a = {qkv, offsets, cache, lengths, ld, R, NB, L, H, KV, hd, cap, sinks};
     const int64_t chunks = (int64_t)L * 2 * KV * (hd * es / 16);
     const int64_t want = (chunks + KT_ - 1) / KT_;

@@ -165,6 +165,23 @@ def test_rows_of_no_sequence_become_zeros(dtype, lens, l, front, back):
         assert torch.equal(out, kept) and torch.equal(dqkv, grad)
 
 
+def test_an_upper_bound_far_over_the_lengths():
+    """l only bounds the sequences: a bound of millions costs and changes nothing"""
+    g = _gen(71)
+    h, kv, hd, lens = 4, 2, 64, [90, 0, 41]
+    rows = sum(lens)
+    qkv, dout = _rand(g, rows, (h + 2 * kv) * hd), _rand(g, rows, h * hd)
+    offsets = torch.tensor([0, 90, 90, rows], device=DEV)
+    got = []
+    for l in (90, 1 << 28):
+        kw = dict(kv_heads=kv, left=30, sinks=2, offsets=offsets)
+        out, lse = ops.attn_window_fwd(qkv, 3, l, h, hd, **kw)
+        cache = torch.zeros(2, 3, kv, 100, hd, device=DEV)
+        ops.kv_append(qkv, cache, torch.tensor(lens, dtype=torch.int32, device=DEV), l, h, sinks=2, offsets=offsets)
+        got.append((out, lse, ops.attn_window_bwd(qkv, out, dout, lse, 3, l, h, hd, **kw), cache))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hd", [16, 64, 128])
 @pytest.mark.parametrize("nb", [1, 40])
