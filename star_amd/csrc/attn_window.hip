@@ -1064,15 +1064,35 @@ static int64_t grid_of(const WArgs& a, int rows, int heads) {
 }
 // Split form or row form, by the 128-row blocks that the row form would have, in eighths of the compute units.  Below the limits the split form
 // was faster, above them the row form (1024 rows, 8 .. 80 heads, windows 64 and 512, forward in us, split / row: hd 32 10.5 / 12.0 at 256 blocks
-// and 15.4 / 15.7 at 448; hd 64 9.2 / 13.8 at 128, 13.8 / 14.2 at 192, 26.1 / 19.2 at 448; hd 128 10.1 / 17.1 at 64, 18.2 / 18.0 at 128; float32 hd 32
-// 29.5 / 35.5 at 256, hd 64 34.8 / 57.2 at 128, 61.3 / 58.4 at 256).  dK/dV has a longer sweep per block, over every head of a group: its limits lie
-// higher (dK/dV + dQ, 4 heads a group, window 256: hd 128 44.6 / 95.7 at 64 blocks, 120 / 131 at 160; hd 64 55 / 69 at 160).
+// and 15.4 / 15.7 at 448; hd 64 9.2 / 13.8 at 128, 13.8 / 14.2 at 192, 26.1 / 19.2 at 448; hd 128 10.1 / 17.1 at 64, 18.2 / 18.0 at 128; float32 hd 16
+// 40.5 / 46.9 at 896, hd 32 29.5 / 35.5 at 256, hd 64 34.8 / 57.2 at 128, 61.3 / 58.4 at 256).  dK/dV has a longer sweep per block, over every head of
+// a group: its limits lie higher (dK/dV + dQ, 4 heads a group, window 256: hd 128 44.6 / 95.7 at 64 blocks, 120 / 131 at 160; hd 64 55 / 69 at 160).
+// A window open to one side leaves blocks with long and with short sweeps, and the launch waits for the longest, which the split form cuts in four:
+// higher limits from 1024 and from 2048 keys on (causal, 4096 rows: hd 32 47 / 68 at 512 blocks, 71 / 89 at 768; hd 64 36 / 65 at 256, 97 / 106 at
+// 768; hd 128 69 / 79 at 256, 136 / 113 at 512; float32 hd 32 165 / 309 at 512, 247 / 442 at 768; with a window of 1024 as for the others.  The
+// whole backward pass, dK/dV split / row: hd 32 114 / 144 at 512, hd 64 174 / 203, hd 128 214 / 290 at 256, 4 heads a group 599 / 959; float32 hd
+// 64 1124 / 1476 at 512).
 template <typename T, int HD> struct SplitUpTo {
     static constexpr int RB = HD * sizeof(T);
-    static constexpr bool EVER = RB <= 256;                  // wider rows: four rings do not fit into LDS
-    static constexpr int ROWS = sizeof(T) == 2 ? (RB <= 64 ? 10 : RB <= 128 ? 4 : 3) : (RB <= 128 ? 10 : 5);
-    static constexpr int KEYS = sizeof(T) == 2 ? (RB <= 64 ? 12 : RB <= 128 ? 8 : 5) : (RB <= 128 ? 20 : 12);
+    static constexpr bool EVER = RB <= 256, BF = sizeof(T) == 2;                  // wider rows: four rings do not fit into LDS
+    static int rows(int sweep) {
+        constexpr int R[3] = {BF ? (RB <= 64 ? 10 : RB <= 128 ? 4 : 3) : (RB <= 64 ? 28 : RB <= 128 ? 10 : 5),
+                              BF ? (RB <= 64 ? 16 : RB <= 128 ? 8 : 4) : (RB <= 64 ? 28 : 24), BF ? (RB <= 128 ? 24 : 8) : (RB <= 64 ? 28 : 24)};
+        return R[sweep];
+    }
+    static int keys(int sweep) {
+        constexpr int K[3] = {BF ? (RB <= 64 ? 12 : RB <= 128 ? 8 : 5) : (RB <= 128 ? 20 : 12), BF ? (RB <= 64 ? 24 : RB <= 128 ? 12 : 10) : (RB <= 128 ? 40 : 24),
+                              BF ? (RB <= 64 ? 24 : RB <= 128 ? 16 : 20) : (RB <= 128 ? 40 : 24)};
+        return K[sweep];
+    }
 };
+// 0: sweeps of about one length, or short ones; 1, 2: a window open to one side with sweeps of up to 1024, 2048 keys and more
+static int sweep_class(const WArgs& a) {
+    const int wide = a.left > a.right ? a.left : a.right, other = a.left > a.right ? a.right : a.left;
+    if (2 * wide < a.L || 4 * other >= a.L) return 0;
+    const int keys = wide + other + WROWS < a.L ? wide + other + WROWS : a.L;
+    return keys >= 2048 ? 2 : keys >= 1024 ? 1 : 0;
+}
 static bool few_blocks(const WArgs& a, int heads, int eighths) {
     const int64_t blocks = (a.offsets ? cdiv(a.R, WROWS) : (int64_t)a.NB * cdiv(a.L, WROWS)) * (int64_t)heads;
     return blocks * 8 <= (int64_t)eighths * star_num_cus();
@@ -1097,19 +1117,19 @@ template <typename T, int HD, int FORM> static int launch_dkv(const WArgs& a, hi
 template <typename T, int HD> static int run_fwd(const WArgs& a, hipStream_t s) {
     using S = SplitUpTo<T, HD>;
     if constexpr (S::EVER)
-        if (few_blocks(a, a.H, S::ROWS)) return launch_fwd<T, HD, true>(a, s);
+        if (few_blocks(a, a.H, S::rows(sweep_class(a)))) return launch_fwd<T, HD, true>(a, s);
     return launch_fwd<T, HD, false>(a, s);
 }
 template <typename T, int HD> static int run_dq(const WArgs& a, hipStream_t s) {
     using S = SplitUpTo<T, HD>;
     if constexpr (S::EVER)
-        if (few_blocks(a, a.H, S::ROWS)) return launch_dq<T, HD, true>(a, s);
+        if (few_blocks(a, a.H, S::rows(sweep_class(a)))) return launch_dq<T, HD, true>(a, s);
     return launch_dq<T, HD, false>(a, s);
 }
 template <typename T, int HD> static int run_dkv(const WArgs& a, hipStream_t s) {
     using S = SplitUpTo<T, HD>;
     if constexpr (S::EVER)
-        if (few_blocks(a, a.KV, S::KEYS)) return launch_dkv<T, HD, SPLIT_FORM>(a, s);
+        if (few_blocks(a, a.KV, S::keys(sweep_class(a)))) return launch_dkv<T, HD, SPLIT_FORM>(a, s);
     return launch_dkv<T, HD, ROW_FORM>(a, s);
 }
 template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t s) {
@@ -1123,7 +1143,7 @@ template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t
             if ((rc = launch_dkv<T, HD, FAR_FORM>(a, s))) return rc;
             // the split form adds the parts up itself where a row is under 256 bytes (7 sequences of 0 .. 2043 rows, 16 heads on 4 of 64: 122 us against
             // 128; 128-wide heads have too few registers to keep the loads in flight: 102 against 48)
-            if (a.far_parts > 1 && !(HD * sizeof(T) < 256 && few_blocks(a, a.KV, SplitUpTo<T, HD>::KEYS))) {
+            if (a.far_parts > 1 && !(HD * sizeof(T) < 256 && few_blocks(a, a.KV, SplitUpTo<T, HD>::keys(sweep_class(a))))) {
                 const int size = 2 * WCfg<T, HD>::DB * 1024;
                 hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, a.NB * a.KV * a.far_groups), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
                 STAR_LAUNCH_CHECK(who);
