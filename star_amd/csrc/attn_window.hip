@@ -473,8 +473,8 @@ template <class C, bool GRAD> __device__ __forceinline__ void redo_query(const W
 }
 
 // Split form: the four waves of a block work on the same 32 rows (dK/dV: keys), each on every fourth tile with a ring of its own, and are added up
-// through LDS, in their order, when all are done.  For launches whose row form (a wave per 32 rows, four sharing the tiles) leaves most of the
-// chip idle (SplitUpTo).
+// through LDS, in their order, when all are done.  For launches whose row form (a wave per 32 rows, four sharing the tiles) leaves much of the
+// chip idle, or waiting for the blocks with the longest sweeps (SplitUpTo).
 // Sum of the waves' accumulator block, in their order: a wave gets four of the sixteen registers, 4 wave .. 4 wave + 3.
 __device__ __forceinline__ void join_block(const f32x16_t& acc, float mul, float* sum, float (&v)[4], int wave, int lane) {
     __syncthreads();
