@@ -1154,15 +1154,16 @@ template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t
 
 // How the far queries of the sinks are cut: about two blocks of four waves per compute unit in all, no more than 16 parts to add up, and at least
 // two 32-query tiles for a wave.  With over 256 sinks, or very many heads, there are enough key blocks with a long sweep to fill the chip: no parts.
-// Nor with under 32 tiles per key head, which the sinks' own block takes in the time of the two launches (float32, 130 rows, 8 heads of 64: 33 us without
-// parts, 54 with; 4 x 700 rows, 16 heads: 212 against 226; 1000 rows, 4 heads a group: 62 without, 49 with).
+// Nor with under 24 tiles per key head, which the sinks' own block takes in the time of the other launches (without parts / with: float32, 500 rows,
+// 8 heads of 64, 13 tiles: 49 / 75 us; 4 x 700 rows, 16 heads, 18 tiles: 212 / 226; 2 x 1000 rows, 12 heads of 32, 24 tiles: 91.7 / 88.5; 4 x 1000 rows,
+// 16 heads of 64, 29 tiles: 390 / 263; bf16, 20 x 900 rows, 12 heads of 64, 27 tiles: 192 / 169).
 // (None for float32 rows of 128 either: four rings do not fit into LDS, and the matrix rate of float32 leaves the sinks' block less far behind.)
 static void far_plan(int NB, int L, int H, int KV, int row_bytes, int left, int sinks, int& groups, int& parts) {
     groups = parts = 0;
     sinks = sinks < L ? sinks : L;
     if (sinks <= 0 || sinks > 256 || left >= L - 1 || row_bytes > 256) return;
     const int64_t lists = (int64_t)NB * KV * cdiv(sinks, 32), tiles = (int64_t)(H / KV) * cdiv(L - left - 1, 32);
-    if (lists > 65535 || tiles < 32) return;
+    if (lists > 65535 || tiles < 24) return;
     groups = cdiv(sinks, 32);
     int64_t p = cdiv(2 * (int64_t)star_num_cus(), lists);
     if (p > tiles / 8) p = tiles / 8;
