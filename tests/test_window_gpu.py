@@ -106,6 +106,16 @@ def test_every_tile_border(dtype, n):
         _check(qkv, _rand(g, n, h * hd, dtype=dtype), [n], h, kv, hd, left, right, sinks)
 
 
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.float32, 32), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("window", [(None, 0, 0), (0, None, 0), (300, 0, 70)])
+def test_long_sweeps(dtype, hd, window):
+    """over 2048 rows: unequal sweeps of a window open to one side; sinks with a thousand queries beyond their window"""
+    g = _gen(hd)
+    n, h, kv = 2110, 2, 1
+    left, right, sinks = window
+    _check(_rand(g, n, (h + 2 * kv) * hd, dtype=dtype, mul=1.2), _rand(g, n, h * hd, dtype=dtype), [n], h, kv, hd, left, right, sinks)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_ragged_batch_leaves_rows_outside_every_sequence(dtype):
     g = _gen(5)
@@ -453,6 +463,23 @@ def test_step(dtype, hd, kv, h):
                 assert (off <= 2 * 2 * half(dtype) * after.double().abs()[~same] + 2.0 ** -20).all()
             else:
                 assert same.all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,kv,rep,nb,cap,left", [(128, 8, 4, 36, 300, 290), (128, 8, 4, 36, 900, 880), (64, 8, 8, 34, 700, 600), (64, 8, 8, 34, 2500, 2400), (16, 16, 3, 20, 9000, 8990),
+                                                   (32, 8, 5, 32, 3500, 3400), (32, 8, 8, 40, 100, 90)])
+def test_step_with_key_heads_enough_to_fill_the_chip(dtype, hd, kv, rep, nb, cap, left):
+    """four and eight query heads a block, whole sequences and splits"""
+    g = _gen(hd + cap)
+    h, sinks = kv * rep, 4
+    lengths = [1 + (cap + 50) * b // (nb - 1) for b in range(nb)]
+    lengths[nb // 2] = 0
+    qkv = _rand(g, nb, (h + 2 * kv) * hd, dtype=dtype)
+    cache = torch.randn(2, nb, kv, cap, hd, generator=torch.Generator(DEV).manual_seed(3), device=DEV).to(dtype)
+    want, tol, after = _step_reference(qkv, cache, lengths, h, left, sinks, None, None, hd ** -0.5)
+    out = ops.attn_window_step(qkv, cache, torch.tensor(lengths, dtype=torch.int32, device=DEV), h, left=left, sinks=sinks)
+    assert_within(out.cpu().double(), want, tol, "step")
+    assert torch.equal(cache, after)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
