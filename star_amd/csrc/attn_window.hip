@@ -90,6 +90,7 @@ __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, unsigned char* l
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 4, off, 0, 0, 0);
 }
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 // every wave's DMA of the tile has landed, and every wave's reads of the stage that is filled next have returned
 // (a wave with a ring of its own needs no barrier)
 template <int N, bool OWN> __device__ __forceinline__ void tile_ready(bool last) {
@@ -358,9 +359,10 @@ template <int KT> __device__ __forceinline__ int key_tiles(int q0, int q1, int l
 // the tiles of a launch form (see the split form below): shared by four waves, or a wave's own
 template <typename T, int HD, bool SPLIT> using RowCfg = std::conditional_t<SPLIT, WCfg<T, HD, 32, 1>, WCfg<T, HD>>;
 
-// A ring of STAGES (K image | V image) stages: while one tile is worked on the next STAGES - 1 are on their way, without registers.
+// A ring of STAGES (K image | V image) stages: while one tile is worked on the next STAGES - 1 are on their way, without registers.  (Four rings of
+// float32 rows of 128 leave room for one stage each: a tile's products take several times the time that it is waited for.)
 template <class C> struct KvRing {
-    static constexpr int STAGE = 2 * C::TILE, STAGES = C::NW == 1 || STAGE > 8192 ? 2 : 3, BYTES = STAGES * STAGE;
+    static constexpr int STAGE = 2 * C::TILE, STAGES = C::NW == 1 && C::RB > 256 ? 1 : C::NW == 1 || STAGE > 8192 ? 2 : 3, BYTES = STAGES * STAGE;
     const typename C::Type* k;              // key 0 of the head; its value lies v columns further on
     int64_t ld;
     int v, len, wave;
@@ -554,8 +556,14 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_FWD(sizeof(T) * 
     for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), own + fill * Ring::STAGE);
     fill = Ring::STAGES - 1;
     for (int it = 0; it < nt; ++it) {
-        tile_ready<(Ring::STAGES - 2) * C::NI, SPLIT>(it + Ring::STAGES - 1 > nt);
-        if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), own + fill * Ring::STAGE);
+        if constexpr (Ring::STAGES == 1) {
+            wait_lds();
+            ring.issue(tile(it), own);
+            wait_vm<0>();
+        } else {
+            tile_ready<(Ring::STAGES - 2) * C::NI, SPLIT>(it + Ring::STAGES - 1 > nt);
+            if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), own + fill * Ring::STAGE);
+        }
         fill = fill + 1 == Ring::STAGES ? 0 : fill + 1;
         const unsigned kl = lds + use * Ring::STAGE, vl = kl + C::TILE;
         use = use + 1 == Ring::STAGES ? 0 : use + 1;
@@ -720,8 +728,14 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DQ(sizeof(T) * H
         for (; fill < Ring::STAGES - 1 && fill < nt; ++fill) ring.issue(tile(fill), own + fill * Ring::STAGE);
         fill = Ring::STAGES - 1;
         for (int it = 0; it < nt; ++it) {
-            tile_ready<(Ring::STAGES - 2) * C::NI, SPLIT>(it + Ring::STAGES - 1 > nt);
-            if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), own + fill * Ring::STAGE);
+            if constexpr (Ring::STAGES == 1) {
+                wait_lds();
+                ring.issue(tile(it), own);
+                wait_vm<0>();
+            } else {
+                tile_ready<(Ring::STAGES - 2) * C::NI, SPLIT>(it + Ring::STAGES - 1 > nt);
+                if (it + Ring::STAGES - 1 < nt) ring.issue(tile(it + Ring::STAGES - 1), own + fill * Ring::STAGE);
+            }
             fill = fill + 1 == Ring::STAGES ? 0 : fill + 1;
             const unsigned kl = lds + use * Ring::STAGE, vl = kl + C::TILE;
             use = use + 1 == Ring::STAGES ? 0 : use + 1;
@@ -883,7 +897,7 @@ template <class C> __device__ __forceinline__ void redo_key(const WArgs& a, cons
 enum { ROW_FORM, SPLIT_FORM, FAR_FORM };
 template <typename T, int HD, bool OWN> struct DkvCfg {
     using C = std::conditional_t<OWN, WCfg<T, HD, 32, 1>, WCfg<T, HD, (sizeof(T) == 2 && HD < 128) ? 64 : 32>>;
-    static constexpr int STAGE = 2 * C::TILE + 512, STAGES = OWN || STAGE > 20480 ? 2 : 3, BYTES = STAGES * STAGE;      // Q image | dO image | 64 log-sum-exps | 64 row dots
+    static constexpr int STAGE = 2 * C::TILE + 512, STAGES = OWN && C::RB > 256 ? 1 : OWN || STAGE > 20480 ? 2 : 3, BYTES = STAGES * STAGE;      // Q image | dO image | 64 log-sum-exps | 64 row dots
 };
 template <typename T, int HD, int FORM>
 __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DKV(sizeof(T) * HD), sizeof(T) * HD, FORM == FAR_FORM || (FORM == SPLIT_FORM && sizeof(T) == 2))) void window_dkv_kernel(WArgs a) {
@@ -985,8 +999,14 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DKV(sizeof(T) * 
     for (; fill < STAGES - 1 && fill < total; ++fill) issue(own + fill * STAGE);
     fill = STAGES - 1;
     for (int it = 0; it < total; ++it) {
-        tile_ready<(STAGES - 2) * (C::NI + NC), OWN>(it + STAGES - 1 > total);
-        if (it + STAGES - 1 < total) issue(own + fill * STAGE);
+        if constexpr (STAGES == 1) {
+            wait_lds();
+            issue(own);
+            wait_vm<0>();
+        } else {
+            tile_ready<(STAGES - 2) * (C::NI + NC), OWN>(it + STAGES - 1 > total);
+            if (it + STAGES - 1 < total) issue(own + fill * STAGE);
+        }
         fill = fill + 1 == STAGES ? 0 : fill + 1;
         const unsigned ql = lds + use * STAGE, gl = ql + C::TILE;
         use = use + 1 == STAGES ? 0 : use + 1;
@@ -1065,7 +1085,7 @@ static int64_t grid_of(const WArgs& a, int rows, int heads) {
 // Split form or row form, by the 128-row blocks that the row form would have, in eighths of the compute units.  Below the limits the split form
 // was faster, above them the row form (1024 rows, 8 .. 80 heads, windows 64 and 512, forward in us, split / row: hd 32 10.5 / 12.0 at 256 blocks
 // and 15.4 / 15.7 at 448; hd 64 9.2 / 13.8 at 128, 13.8 / 14.2 at 192, 26.1 / 19.2 at 448; hd 128 10.1 / 17.1 at 64, 18.2 / 18.0 at 128; float32 hd 16
-// 40.5 / 46.9 at 896, hd 32 29.5 / 35.5 at 256, hd 64 34.8 / 57.2 at 128, 61.3 / 58.4 at 256).  dK/dV has a longer sweep per block, over every head of
+// 40.5 / 46.9 at 896, hd 32 29.5 / 35.5 at 256, hd 64 34.8 / 57.2 at 128, 61.3 / 58.4 at 256, hd 128 17 / 55 at 48, 168 / 149 at 256).  dK/dV has a longer sweep per block, over every head of
 // a group: its limits lie higher (dK/dV + dQ, 4 heads a group, window 256: hd 128 44.6 / 95.7 at 64 blocks, 120 / 131 at 160; hd 64 55 / 69 at 160).
 // A window open to one side leaves blocks with long and with short sweeps, and the launch waits for the longest, which the split form cuts in four:
 // higher limits from 1024 and from 2048 keys on (causal, 4096 rows: hd 32 47 / 68 at 512 blocks, 71 / 89 at 768; hd 64 36 / 65 at 256, 97 / 106 at
@@ -1074,15 +1094,15 @@ static int64_t grid_of(const WArgs& a, int rows, int heads) {
 // 64 1124 / 1476 at 512).
 template <typename T, int HD> struct SplitUpTo {
     static constexpr int RB = HD * sizeof(T);
-    static constexpr bool EVER = RB <= 256, BF = sizeof(T) == 2;                  // wider rows: four rings do not fit into LDS
+    static constexpr bool BF = sizeof(T) == 2;
     static int rows(int sweep) {
-        constexpr int R[3] = {BF ? (RB <= 64 ? 10 : RB <= 128 ? 4 : 3) : (RB <= 64 ? 28 : RB <= 128 ? 10 : 5),
-                              BF ? (RB <= 64 ? 16 : RB <= 128 ? 8 : 4) : (RB <= 64 ? 28 : 24), BF ? (RB <= 128 ? 24 : 8) : (RB <= 64 ? 28 : 24)};
+        constexpr int R[3] = {BF ? (RB <= 64 ? 10 : RB <= 128 ? 4 : 3) : (RB <= 64 ? 28 : RB <= 128 ? 10 : RB <= 256 ? 5 : 4),
+                              BF ? (RB <= 64 ? 16 : RB <= 128 ? 8 : 4) : (RB <= 64 ? 28 : RB <= 256 ? 24 : 16), BF ? (RB <= 128 ? 24 : 8) : (RB <= 64 ? 28 : RB <= 256 ? 24 : 16)};
         return R[sweep];
     }
     static int keys(int sweep) {
-        constexpr int K[3] = {BF ? (RB <= 64 ? 12 : RB <= 128 ? 8 : 5) : (RB <= 128 ? 20 : 12), BF ? (RB <= 64 ? 24 : RB <= 128 ? 12 : 10) : (RB <= 128 ? 40 : 24),
-                              BF ? (RB <= 64 ? 24 : RB <= 128 ? 16 : 20) : (RB <= 128 ? 40 : 24)};
+        constexpr int K[3] = {BF ? (RB <= 64 ? 12 : RB <= 128 ? 8 : 5) : (RB <= 128 ? 20 : RB <= 256 ? 12 : 7), BF ? (RB <= 64 ? 24 : RB <= 128 ? 12 : 10) : (RB <= 128 ? 40 : RB <= 256 ? 24 : 16),
+                              BF ? (RB <= 64 ? 24 : RB <= 128 ? 16 : 20) : (RB <= 128 ? 40 : RB <= 256 ? 24 : 16)};
         return K[sweep];
     }
 };
@@ -1093,7 +1113,9 @@ static int sweep_class(const WArgs& a) {
     const int keys = wide + other + WROWS < a.L ? wide + other + WROWS : a.L;
     return keys >= 2048 ? 2 : keys >= 1024 ? 1 : 0;
 }
+// (a sweep of one tile has nothing to split: 1 x 32 rows, 8 heads, forward 4.4 us by rows and 4.6 split at hd 32, 8.7 and 11.0 in float32 at hd 128)
 static bool few_blocks(const WArgs& a, int heads, int eighths) {
+    if ((int64_t)(a.H / heads) * cdiv(a.L, 32) == 1) return false;
     const int64_t blocks = (a.offsets ? cdiv(a.R, WROWS) : (int64_t)a.NB * cdiv(a.L, WROWS)) * (int64_t)heads;
     return blocks * 8 <= (int64_t)eighths * star_num_cus();
 }
@@ -1116,20 +1138,17 @@ template <typename T, int HD, int FORM> static int launch_dkv(const WArgs& a, hi
 }
 template <typename T, int HD> static int run_fwd(const WArgs& a, hipStream_t s) {
     using S = SplitUpTo<T, HD>;
-    if constexpr (S::EVER)
-        if (few_blocks(a, a.H, S::rows(sweep_class(a)))) return launch_fwd<T, HD, true>(a, s);
+    if (few_blocks(a, a.H, S::rows(sweep_class(a)))) return launch_fwd<T, HD, true>(a, s);
     return launch_fwd<T, HD, false>(a, s);
 }
 template <typename T, int HD> static int run_dq(const WArgs& a, hipStream_t s) {
     using S = SplitUpTo<T, HD>;
-    if constexpr (S::EVER)
-        if (few_blocks(a, a.H, S::rows(sweep_class(a)))) return launch_dq<T, HD, true>(a, s);
+    if (few_blocks(a, a.H, S::rows(sweep_class(a)))) return launch_dq<T, HD, true>(a, s);
     return launch_dq<T, HD, false>(a, s);
 }
 template <typename T, int HD> static int run_dkv(const WArgs& a, hipStream_t s) {
     using S = SplitUpTo<T, HD>;
-    if constexpr (S::EVER)
-        if (few_blocks(a, a.KV, S::keys(sweep_class(a)))) return launch_dkv<T, HD, SPLIT_FORM>(a, s);
+    if (few_blocks(a, a.KV, S::keys(sweep_class(a)))) return launch_dkv<T, HD, SPLIT_FORM>(a, s);
     return launch_dkv<T, HD, ROW_FORM>(a, s);
 }
 template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t s) {
@@ -1138,17 +1157,16 @@ template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t
     if (rc) return rc;
     WArgs a = first;
     a.rest_blocks = 0;
-    if constexpr (SplitUpTo<T, HD>::EVER)
-        if (a.far_parts) {
-            if ((rc = launch_dkv<T, HD, FAR_FORM>(a, s))) return rc;
-            // the split form adds the parts up itself where a row is under 256 bytes (7 sequences of 0 .. 2043 rows, 16 heads on 4 of 64: 122 us against
-            // 128; 128-wide heads have too few registers to keep the loads in flight: 102 against 48)
-            if (a.far_parts > 1 && !(HD * sizeof(T) < 256 && few_blocks(a, a.KV, SplitUpTo<T, HD>::keys(sweep_class(a))))) {
-                const int size = 2 * WCfg<T, HD>::DB * 1024;
-                hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, a.NB * a.KV * a.far_groups), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
-                STAR_LAUNCH_CHECK(who);
-            }
+    if (a.far_parts) {
+        if ((rc = launch_dkv<T, HD, FAR_FORM>(a, s))) return rc;
+        // the split form adds the parts up itself where a row is under 256 bytes (7 sequences of 0 .. 2043 rows, 16 heads on 4 of 64: 122 us against
+        // 128; 128-wide heads have too few registers to keep the loads in flight: 102 against 48)
+        if (a.far_parts > 1 && !(HD * sizeof(T) < 256 && few_blocks(a, a.KV, SplitUpTo<T, HD>::keys(sweep_class(a))))) {
+            const int size = 2 * WCfg<T, HD>::DB * 1024;
+            hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, a.NB * a.KV * a.far_groups), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
+            STAR_LAUNCH_CHECK(who);
         }
+    }
     return run_dkv<T, HD>(a, s);
 }
 
@@ -1157,11 +1175,10 @@ template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t
 // Nor with under 24 tiles per key head, which the sinks' own block takes in the time of the other launches (without parts / with: float32, 500 rows,
 // 8 heads of 64, 13 tiles: 49 / 75 us; 4 x 700 rows, 16 heads, 18 tiles: 212 / 226; 2 x 1000 rows, 12 heads of 32, 24 tiles: 91.7 / 88.5; 4 x 1000 rows,
 // 16 heads of 64, 29 tiles: 390 / 263; bf16, 20 x 900 rows, 12 heads of 64, 27 tiles: 192 / 169).
-// (None for float32 rows of 128 either: four rings do not fit into LDS, and the matrix rate of float32 leaves the sinks' block less far behind.)
-static void far_plan(int NB, int L, int H, int KV, int row_bytes, int left, int sinks, int& groups, int& parts) {
+static void far_plan(int NB, int L, int H, int KV, int left, int sinks, int& groups, int& parts) {
     groups = parts = 0;
     sinks = sinks < L ? sinks : L;
-    if (sinks <= 0 || sinks > 256 || left >= L - 1 || row_bytes > 256) return;
+    if (sinks <= 0 || sinks > 256 || left >= L - 1) return;
     const int64_t lists = (int64_t)NB * KV * cdiv(sinks, 32), tiles = (int64_t)(H / KV) * cdiv(L - left - 1, 32);
     if (lists > 65535 || tiles < 24) return;
     groups = cdiv(sinks, 32);
@@ -1215,7 +1232,7 @@ extern "C" int star_attn_window_fwd(const StarAttnWindow* g, void* stream) {
 extern "C" int64_t star_attn_window_bwd_ws(int64_t R, int NB, int L, int H, int KV, int hd, int left, int sinks, int dt) {
     if (R < 0 || NB <= 0 || L <= 0 || H <= 0 || KV <= 0 || H % KV || hd <= 0 || left < 0 || sinks < 0) return 0;
     int groups, parts;
-    far_plan(NB, longest(L, R), H, KV, hd * (dt == STAR_BF16 ? 2 : 4), left, sinks, groups, parts);
+    far_plan(NB, longest(L, R), H, KV, left, sinks, groups, parts);
     return (H * R + 63) / 64 * 64 + (int64_t)NB * KV * groups * parts * 2 * 32 * (hd < 32 ? 32 : hd);
 }
 
@@ -1228,7 +1245,7 @@ extern "C" int star_attn_window_bwd(const StarAttnWindow* g, void* stream) {
     a.dqkv = g->dqkv;
     a.ndelta = g->ws;
     a.rest_blocks = rest_blocks(g, (int64_t)(g->H + 2 * g->KV) * g->hd);
-    far_plan(g->NB, a.L, g->H, g->KV, g->hd * (g->dt == STAR_BF16 ? 2 : 4), g->left, g->sinks, a.far_groups, a.far_parts);
+    far_plan(g->NB, a.L, g->H, g->KV, g->left, g->sinks, a.far_groups, a.far_parts);
     a.far_ws = g->ws + (g->H * g->R + 63) / 64 * 64;
     hipStream_t s = (hipStream_t)stream;
     return g->dt == STAR_BF16 ? BY_HD(run_bwd, bf16_t) : BY_HD(run_bwd, float);
