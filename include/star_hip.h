@@ -239,7 +239,8 @@ int star_rope(const void* x, int64_t x_ld, void* y, int64_t y_ld, const int32_t*
  * Sequence b is rows [b L, (b + 1) L) or, with offsets int64 [NB + 1] on the device, rows [offsets[b], offsets[b+1]), of which the first
  * L are used (L = the longest sequence); rows of no sequence are neither read nor written.  What a row does not see does not reach its
  * result, infinities and NaN included.  hd in {16, 32, 64, 128}.
- *   out dt [R, H*hd]; lse float32 [H, R]: log2-domain log-sum-exp of every row (optional in the forward pass).
+ *   out dt [R, H*hd]; lse float32 [H, R]: log2-domain log-sum-exp of every row (optional in the forward pass).  What a call writes shares no
+ *   memory with its other operands, in all calls of this section (star_rope apart; a single row's out may lie on its qkv): overlaps are refused.
  * star_attn_window_bwd: reads out, lse, dout dt [R, H*hd]; writes dqkv dt [R, (H + 2 KV) hd] (dense rows; gradients of a shared key/value head
  *   are summed over its query heads).  ws float32 [star_attn_window_bwd_ws(...)], any content.  No atomics: bitwise reproducible. */
 typedef struct StarAttnWindow {

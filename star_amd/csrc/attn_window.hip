@@ -1224,6 +1224,11 @@ static int rest_blocks(const StarAttnWindow* g, int64_t width) {
 extern "C" int star_attn_window_fwd(const StarAttnWindow* g, void* stream) {
     WArgs a;
     if (int rc = window_args("star_attn_window_fwd", g, a)) return rc;
+    // blocks read rows that others may have written results over already.  (A single row in place: a head's block alone reads its query.)
+    const int64_t es = g->dt == STAR_BF16 ? 2 : 4, orow = (int64_t)g->H * g->hd * es, lse = (int64_t)g->H * g->R * 4;
+    const int64_t row = ((int64_t)g->H + 2 * (int64_t)g->KV) * g->hd * es;
+    STAR_CHECK((g->R == 1 && g->out == g->qkv) || !star_meets(g->out, g->R * orow, g->qkv, g->R, g->ld * es, row), "star_attn_window_fwd: out overlaps qkv");
+    STAR_CHECK(!star_meets(g->lse, lse, g->qkv, g->R, g->ld * es, row) && !star_meets(g->lse, lse, g->out, g->R * orow), "star_attn_window_fwd: lse overlaps qkv or out");
     a.rest_blocks = rest_blocks(g, (int64_t)g->H * g->hd);
     hipStream_t s = (hipStream_t)stream;
     return g->dt == STAR_BF16 ? BY_HD(run_fwd, bf16_t) : BY_HD(run_fwd, float);
@@ -1241,6 +1246,15 @@ extern "C" int star_attn_window_bwd(const StarAttnWindow* g, void* stream) {
     if (int rc = window_args("star_attn_window_bwd", g, a)) return rc;
     STAR_CHECK(g->lse && g->dout && g->dqkv && g->ws, "star_attn_window_bwd: null pointer");
     STAR_CHECK((uintptr_t)g->dout % 16 == 0 && (uintptr_t)g->dqkv % 16 == 0, "star_attn_window_bwd: dout and dqkv must be 16-byte aligned");
+    // the dK/dV launches read what the dQ launch has read before them
+    const int64_t es = g->dt == STAR_BF16 ? 2 : 4, orow = (int64_t)g->H * g->hd * es, lse = (int64_t)g->H * g->R * 4;
+    const int64_t row = ((int64_t)g->H + 2 * (int64_t)g->KV) * g->hd * es;
+    const int64_t ws = star_attn_window_bwd_ws(g->R, g->NB, g->L, g->H, g->KV, g->hd, g->left, g->sinks, g->dt) * 4;
+    auto meets = [&](const void* p, int64_t n) {
+        return star_meets(p, n, g->qkv, g->R, g->ld * es, row) || star_meets(p, n, g->out, g->R * orow) || star_meets(p, n, g->dout, g->R * orow) || star_meets(p, n, g->lse, lse);
+    };
+    STAR_CHECK(!meets(g->dqkv, g->R * row), "star_attn_window_bwd: dqkv overlaps qkv, out, dout or lse");
+    STAR_CHECK(!meets(g->ws, ws) && !star_meets(g->ws, ws, g->dqkv, g->R * row), "star_attn_window_bwd: ws overlaps another operand");
     a.dout = g->dout;
     a.dqkv = g->dqkv;
     a.ndelta = g->ws;

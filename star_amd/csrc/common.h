@@ -128,6 +128,14 @@ __device__ __forceinline__ int xcd_remap(int bid, int nblk) {
 
 static inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+// whether the n bytes at p meet one of R rows of w bytes that lie ld bytes apart from q on (ld >= w; what lies between the rows is not theirs)
+static inline bool star_meets(const void* p, int64_t n, const void* q, int64_t R, int64_t ld, int64_t w) {
+    if (!p || !q || n <= 0 || R <= 0 || w <= 0) return false;
+    const int64_t d = (int64_t)((intptr_t)p - (intptr_t)q), first = d < w ? 0 : (d - w) / ld + 1;       // the first row that ends behind p
+    return first < R && first * ld < d + n;
+}
+static inline bool star_meets(const void* p, int64_t n, const void* q, int64_t w) { return star_meets(p, n, q, 1, w, w); }
+
 // hipFuncSetAttribute(MaxDynamicSharedMemorySize) belongs to the CURRENT device: a "done" flag has to be kept per device ordinal.
 // Returns true the first time it sees the current device with this mask (a race between two threads sets the attribute twice: harmless).
 static inline bool star_once_per_device(unsigned long long& mask) {

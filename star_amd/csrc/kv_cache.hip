@@ -352,6 +352,7 @@ extern "C" int star_kv_append(const void* qkv, int64_t ld, const int64_t* offset
     STAR_CHECK(sinks >= 0 && cap > sinks, "star_kv_append: a cache of %d slots does not hold %d sinks and a ring", cap, sinks);
     STAR_CHECK(R >= 0 && (offsets || R == (int64_t)NB * L), "star_kv_append: %lld rows for %d sequences of %d", (long long)R, NB, L);
     STAR_CHECK(ld * es % 16 == 0 && (uintptr_t)qkv % 16 == 0 && (uintptr_t)cache % 16 == 0, "star_kv_append: rows and cache must be 16-byte aligned");
+    STAR_CHECK(!star_meets(cache, 2 * (int64_t)NB * KV * cap * hd * es, qkv, R, ld * es, ((int64_t)H + 2 * (int64_t)KV) * hd * es), "star_kv_append: cache overlaps qkv");
     if (L == 0 || R == 0) return 0;
     if (L > R) L = (int)R;          // ragged: no sequence has more
     const AppendArgs a = {qkv, offsets, cache, lengths, ld, R, NB, L, H, KV, hd, cap, sinks};
@@ -449,6 +450,14 @@ extern "C" int star_attn_window_step(const StarAttnStep* g, void* stream) {
     STAR_CHECK(a.splits == 1 || g->ws, "star_attn_window_step: null workspace (star_attn_window_step_ws)");
     const int64_t blocks = ((int64_t)g->NB * g->KV * a.splits + 7) / 8 * 8 * a.chunks;
     STAR_CHECK(blocks < (1ll << 31), "star_attn_window_step: NB, KV too large for the grid");
+    // (a single row in place: the blocks of a head alone read its query)
+    const int64_t out_bytes = (int64_t)g->NB * g->H * g->hd * es, cache_bytes = 2 * (int64_t)g->NB * g->KV * g->cap * g->hd * es, row = (int64_t)(g->H + 2 * g->KV) * g->hd * es;
+    const int64_t ws_bytes = a.splits == 1 ? 0 : (int64_t)g->NB * g->H * a.splits * (g->hd + 2) * 4;
+    auto meets = [&](const void* p, int64_t n) { return star_meets(p, n, g->qkv, g->NB, g->ld * es, row); };
+    STAR_CHECK((g->NB == 1 && g->out == g->qkv) || !meets(g->out, out_bytes), "star_attn_window_step: out overlaps qkv");
+    STAR_CHECK(!meets(g->cache, cache_bytes) && !star_meets(g->cache, cache_bytes, g->out, out_bytes), "star_attn_window_step: cache overlaps qkv or out");
+    STAR_CHECK(!meets(g->ws, ws_bytes) && !star_meets(g->ws, ws_bytes, g->out, out_bytes) && !star_meets(g->ws, ws_bytes, g->cache, cache_bytes),
+               "star_attn_window_step: ws overlaps another operand");
     hipStream_t s = (hipStream_t)stream;
     if (g->dt == STAR_BF16) step_run<bf16_t>(a, g->hd, G, plan.threads, dim3((unsigned)blocks), s);
     else step_run<float>(a, g->hd, G, plan.threads, dim3((unsigned)blocks), s);

@@ -1,0 +1,54 @@
+"""What the window attention, rotary and cache entry points refuse or decide on the host beyond the shapes: operands that share memory, bounds past 32
+bits, grids past the hardware's, plans, launch forms.  No GPU: every refused call ends before a launch."""
+import ctypes as C
+
+import pytest
+
+from star_amd import _lib as L
+
+A = 1 << 20          # operands A apart, none of them longer
+
+
+def _refused(rc, *words):
+    said = L.lib().star_last_error().decode()
+    assert rc != 0 and all(w in said for w in words), (rc, said)
+
+
+def _attn(**kw):
+    a = dict(qkv=A, out=2 * A, lse=3 * A, dout=4 * A, dqkv=5 * A, ws=6 * A, ld=8 * 64, R=40, NB=2, L=20, H=4, KV=2, hd=64, left=5, right=0, sinks=1,
+             scale=0.125, dt=L.BF16)
+    a.update(kw)
+    return L.StarAttnWindow(**a)
+
+
+# rows of qkv: 40 of 1024 bytes; of out and dout: 40 of 512; lse: 4 x 40 floats
+@pytest.mark.parametrize("change,words", [
+    (dict(out=A), "out overlaps qkv"), (dict(out=A + 1024 * 40 - 16), "out overlaps qkv"), (dict(out=A - 512 * 40 + 16), "out overlaps qkv"),
+    (dict(out=A, ld=2048), "out overlaps qkv"), (dict(out=A + 1024, ld=2048), "out overlaps qkv"), (dict(lse=A + 1024), "lse overlaps"),
+    (dict(lse=2 * A + 512 * 40 - 4), "lse overlaps")])
+def test_window_forward_refuses_shared_memory(change, words):
+    _refused(L.lib().star_attn_window_fwd(C.byref(_attn(**change)), None), "star_attn_window_fwd", words)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(dqkv=A), "dqkv overlaps"), (dict(dqkv=A + 1024 * 40 - 16), "dqkv overlaps"), (dict(dqkv=A - 1024 * 40 + 16), "dqkv overlaps"),
+    (dict(dqkv=2 * A), "dqkv overlaps"), (dict(dqkv=4 * A + 512 * 39), "dqkv overlaps"), (dict(dqkv=3 * A + 4 * 40 * 4 - 16), "dqkv overlaps"),
+    (dict(ws=A), "ws overlaps"), (dict(ws=2 * A), "ws overlaps"), (dict(ws=3 * A), "ws overlaps"), (dict(ws=4 * A), "ws overlaps"), (dict(ws=5 * A), "ws overlaps")])
+def test_window_backward_refuses_shared_memory(change, words):
+    _refused(L.lib().star_attn_window_bwd(C.byref(_attn(**change)), None), "star_attn_window_bwd", words)
+
+
+# rows of qkv: 2 of 1024 bytes; cache: 2 x 2 x 2 x 64 rows of 128 bytes
+@pytest.mark.parametrize("change,words", [
+    (dict(out=A), "out overlaps qkv"), (dict(out=A + 512), "out overlaps qkv"), (dict(NB=1, out=A + 16), "out overlaps qkv"), (dict(cache=A + 2032), "cache overlaps"),
+    (dict(out=2 * A + 64), "cache overlaps"), (dict(NB=1, cap=1 << 16, left=1 << 15, cache=1 << 34, ws=A), "ws overlaps"),
+    (dict(NB=1, cap=1 << 16, left=1 << 15, cache=1 << 34, ws=4 * A), "ws overlaps"), (dict(NB=1, cap=1 << 16, left=1 << 15, cache=1 << 34, ws=1 << 34), "ws overlaps")])
+def test_step_refuses_shared_memory(change, words):
+    a = dict(qkv=A, cache=2 * A, lengths=3 * A, out=4 * A, ws=5 * A, ld=8 * 64, NB=2, H=4, KV=2, hd=64, cap=64, left=31, sinks=4, scale=0.125, dt=L.BF16)
+    a.update(change)
+    _refused(L.lib().star_attn_window_step(C.byref(L.StarAttnStep(**a)), None), "star_attn_window_step", words)
+
+
+@pytest.mark.parametrize("cache", [A, A + 40 * 1024 - 16, A - 2 * 2 * 2 * 64 * 64 * 2 + 16])
+def test_append_refuses_shared_memory(cache):
+    _refused(L.lib().star_kv_append(A, 8 * 64, None, cache, 8 * A, 40, 2, 20, 4, 2, 64, 64, 4, L.BF16, None), "star_kv_append", "cache overlaps")

@@ -1,0 +1,56 @@
+"""Calls of the window attention, rotary and cache operators at the edges of what they take: results on operands, bounds past 32 bits, rows
+without a finite score, data that has gone NaN, the far queries of many sinks, very many rows."""
+import pytest
+import torch
+
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from star_amd import ops
+
+DEV = "cuda"
+TYPES = [torch.bfloat16, torch.float32]
+
+
+def _rand(g, *shape, dtype=torch.float32, mul=1.0):
+    return (torch.randn(*shape, generator=g) * mul).to(DEV).to(dtype)
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- results that would lie on operands ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+def test_results_on_operands_are_refused(dtype):
+    g = _gen(1)
+    n, h, kv, hd = 70, 4, 2, 32
+    w = (h + 2 * kv) * hd
+    qkv, dout = _rand(g, n, w, dtype=dtype), _rand(g, n, h * hd, dtype=dtype)
+    out, lse = ops.attn_window_fwd(qkv, 1, n, h, hd, kv_heads=kv)
+    want = ops.attn_window_bwd(qkv, out, dout, lse, 1, n, h, hd, kv_heads=kv)
+    kept = qkv.clone()
+    with pytest.raises(RuntimeError, match="dqkv overlaps"):
+        ops.attn_window_bwd(qkv, out, dout, lse, 1, n, h, hd, kv_heads=kv, dqkv=qkv)
+    with pytest.raises(RuntimeError, match="out overlaps"):
+        ops.attn_window_fwd(qkv, 1, n, h, hd, kv_heads=kv, out=qkv.view(-1)[:n * h * hd].view(n, h * hd))
+    cache, lengths = torch.zeros(2, 2, kv, 8, hd, dtype=dtype, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match="out overlaps"):
+        ops.attn_window_step(qkv[:2], cache, lengths, h, out=qkv.view(-1)[:2 * h * hd].view(2, h * hd))
+    assert torch.equal(qkv, kept) and not cache.any()
+    # between the rows of a wider matrix there is room for results
+    wide = torch.zeros(3, w + 4 * h * hd, dtype=dtype, device=DEV)
+    wide[:2, :w] = qkv[:2]
+    gap = wide.view(-1)[w:w + 2 * h * hd].view(2, h * hd)
+    assert torch.equal(ops.attn_window_fwd(wide[:2, :w], 1, 2, h, hd, kv_heads=kv, out=gap)[0], ops.attn_window_fwd(qkv[:2], 1, 2, h, hd, kv_heads=kv)[0])
+    # and a single row may be computed in place
+    row = qkv[3:4].clone()
+    alone, _ = ops.attn_window_fwd(row, 1, 1, h, hd, kv_heads=kv)
+    one = torch.zeros(2, 1, kv, 8, hd, dtype=dtype, device=DEV)
+    step = ops.attn_window_step(row, one, lengths[:1], h)
+    for call in (lambda r: ops.attn_window_fwd(r, 1, 1, h, hd, kv_heads=kv, out=r[:, :h * hd]), lambda r: ops.attn_window_step(r, one, lengths[:1], h, out=r[:, :h * hd])):
+        r = row.clone()
+        call(r)
+        assert torch.equal(r[:, :h * hd], alone) and torch.equal(r[:, :h * hd], step) and torch.equal(r[:, h * hd:], row[:, h * hd:])
+    assert torch.equal(ops.attn_window_bwd(qkv, out, dout, lse, 1, n, h, hd, kv_heads=kv), want)
