@@ -402,6 +402,14 @@ def _at_home(fn):
     return call
 
 
+def _ints(*values):
+    """values for int32 parameters.  ctypes would keep the low 32 bits of a longer one; it is handed over as the nearest that fits, which says
+    the same (a bound over any length) or is refused."""
+    if min(values) < 0 or max(values) > 0x7fffffff:
+        return [max(-1, min(v, 0x7fffffff)) for v in values]
+    return values
+
+
 def _profiled(tag, nbytes, fn, *args):
     with _timed(tag, 0.0, float(nbytes)):
         return fn(*args)
@@ -463,7 +471,7 @@ def _rope(home, x, pos, rot_heads, hd, sections, base, per_axis, interleaved, ou
         assert out.shape == shape and out.dtype == x.dtype
         out_ld = _rows2d(out, shape, "out")
     if r:
-        args = (x.data_ptr(), ld, out.data_ptr(), out_ld, pos.data_ptr(), pos_ld, plan, r, w, rot_heads, hd, inverse, L.dt_of(x), _raw_stream(home))
+        args = (x.data_ptr(), ld, out.data_ptr(), out_ld, pos.data_ptr(), pos_ld, plan, r, *_ints(w, rot_heads, hd), inverse, L.dt_of(x), _raw_stream(home))
         rc = L.lib().star_rope(*args) if PROFILER is None else _profiled("rope", 2 * r * w * x.element_size(), L.lib().star_rope, *args)
         if rc:
             L.check(rc)
@@ -495,8 +503,9 @@ def _window(qkv, nb, l, h, hd, kv, left, right, sinks, offsets, scale):
     r, w = shape
     assert w == (h + 2 * kv) * hd, "qkv rows of %d columns are not %d + 2 * %d heads of %d" % (w, h, kv, hd)
     assert offsets is not None or r == nb * l, "%d rows for %d sequences of %d" % (r, nb, l)
-    return L.StarAttnWindow(qkv.data_ptr(), None if offsets is None else _offsets(offsets, nb), None, None, None, None, None, ld, r, nb, l, h, kv, hd,
-                            l if left is None else left, l if right is None else right, sinks, hd ** -0.5 if scale is None else scale, L.dt_of(qkv))
+    return L.StarAttnWindow(qkv.data_ptr(), None if offsets is None else _offsets(offsets, nb), None, None, None, None, None, ld, r,
+                            *_ints(nb, l, h, kv, hd, l if left is None else left, l if right is None else right, sinks),
+                            hd ** -0.5 if scale is None else scale, L.dt_of(qkv))
 
 
 @_at_home
@@ -546,7 +555,7 @@ def _window_bwd(home, qkv, out, dout, lse, nb, l, h, hd, kv_heads, left, right, 
         assert dqkv.shape == qkv.shape and dqkv.dtype == qkv.dtype and dqkv.is_contiguous()
     if r:
         lib = L.lib()
-        ws = qkv.new_empty(lib.star_attn_window_bwd_ws(r, nb, l, h, g.KV, hd, g.left, sinks, g.dt), dtype=torch.float32)
+        ws = qkv.new_empty(lib.star_attn_window_bwd_ws(r, g.NB, g.L, g.H, g.KV, g.hd, g.left, g.sinks, g.dt), dtype=torch.float32)
         g.out, g.lse, g.dout, g.dqkv, g.ws = out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dqkv.data_ptr(), ws.data_ptr()
         fn, stream = lib.star_attn_window_bwd, _raw_stream(home)
         rc = fn(g, stream) if PROFILER is None else _profiled("attn_window_bwd", 2 * r * (qkv.shape[1] + h * hd) * qkv.element_size(), fn, g, stream)
@@ -579,8 +588,8 @@ def _kv_append(home, qkv, cache, lengths, l, h, sinks, offsets):
     nb, kv, cap, hd = _cache_dims(cache, qkv, shape[1], h, lengths)
     assert offsets is not None or r == nb * l, "%d rows for %d sequences of %d" % (r, nb, l)
     if r and nb:
-        args = (qkv.data_ptr(), ld, None if offsets is None else _offsets(offsets, nb), cache.data_ptr(), lengths.data_ptr(), r, nb, l, h, kv, hd, cap, sinks,
-                L.dt_of(qkv), _raw_stream(home))
+        args = (qkv.data_ptr(), ld, None if offsets is None else _offsets(offsets, nb), cache.data_ptr(), lengths.data_ptr(), r,
+                *_ints(nb, l, h, kv, hd, cap, sinks), L.dt_of(qkv), _raw_stream(home))
         rc = L.lib().star_kv_append(*args) if PROFILER is None else _profiled("kv_append", 4 * r * kv * hd * qkv.element_size(), L.lib().star_kv_append, *args)
         if rc:
             L.check(rc)
@@ -617,10 +626,11 @@ def _window_step(home, qkv, cache, lengths, h, left, sinks, pos, sections, base,
         if left is None:
             left = cap - sinks - 1
         dt = L.dt_of(qkv)
-        need = _step_ws(home, nb, h, kv, hd, cap, left, sinks, dt)
+        sizes = nb, h, kv, hd, cap, left, sinks = _ints(nb, h, kv, hd, cap, left, sinks)
+        need = _step_ws(home, *sizes, dt)
         ws = qkv.new_empty(need, dtype=torch.float32) if need else None
-        g = L.StarAttnStep(qkv.data_ptr(), cache.data_ptr(), lengths.data_ptr(), None, None, out.data_ptr(), None if ws is None else ws.data_ptr(), ld, 0, nb, h, kv,
-                           hd, cap, left, sinks, hd ** -0.5 if scale is None else scale, dt)
+        g = L.StarAttnStep(qkv.data_ptr(), cache.data_ptr(), lengths.data_ptr(), None, None, out.data_ptr(), None if ws is None else ws.data_ptr(), ld, 0, *sizes,
+                           hd ** -0.5 if scale is None else scale, dt)
         if sections is not None:
             g.h_rope, axes = _rope_ref(tuple(sections), base, per_axis, interleaved)
             pos, g.pos_ld = _positions(pos, axes, nb)

@@ -3,8 +3,10 @@ bits, grids past the hardware's, plans, launch forms.  No GPU: every refused cal
 import ctypes as C
 
 import pytest
+import torch
 
 from star_amd import _lib as L
+from star_amd import ops
 
 A = 1 << 20          # operands A apart, none of them longer
 
@@ -52,3 +54,16 @@ def test_step_refuses_shared_memory(change, words):
 @pytest.mark.parametrize("cache", [A, A + 40 * 1024 - 16, A - 2 * 2 * 2 * 64 * 64 * 2 + 16])
 def test_append_refuses_shared_memory(cache):
     _refused(L.lib().star_kv_append(A, 8 * 64, None, cache, 8 * A, 40, 2, 20, 4, 2, 64, 64, 4, L.BF16, None), "star_kv_append", "cache overlaps")
+
+
+# ---- bounds past 32 bits: ctypes alone would keep their low half ----------------------------------------------------------------
+@pytest.mark.parametrize("over", [(1 << 31), (1 << 32), (1 << 32) + 5, (1 << 63) + 1])
+def test_bounds_past_32_bits_stay_bounds(over):
+    x = torch.zeros(20, 8 * 16)
+    g = ops._window(x, 1, 20, 4, 16, 2, over, over, over, None, None)
+    assert (g.left, g.right, g.sinks, g.L, g.NB) == (2147483647, 2147483647, 2147483647, 20, 1)
+    g = ops._window(x, 1, 20, 4, 16, 2, -over, -over, -over, None, None)
+    assert (g.left, g.right, g.sinks) == (-1, -1, -1)
+    g = ops._window(x, 1, over, 4, 16, 2, None, 0, 0, torch.zeros(2, dtype=torch.int64), None)
+    assert (g.L, g.left) == (2147483647, 2147483647)
+    assert list(ops._ints(5, over, 0, -over)) == [5, 2147483647, 0, -1] and list(ops._ints(0, 7, 2147483647)) == [0, 7, 2147483647]

@@ -54,3 +54,29 @@ def test_results_on_operands_are_refused(dtype):
         call(r)
         assert torch.equal(r[:, :h * hd], alone) and torch.equal(r[:, :h * hd], step) and torch.equal(r[:, h * hd:], row[:, h * hd:])
     assert torch.equal(ops.attn_window_bwd(qkv, out, dout, lse, 1, n, h, hd, kv_heads=kv), want)
+
+
+def test_bounds_past_32_bits():
+    """a bound of any size over the sequence is no bound; lengths, heads and sizes past 32 bits are refused, not cut to their low half"""
+    g = _gen(2)
+    n, h, kv, hd = 90, 4, 2, 32
+    qkv, dout = _rand(g, n, (h + 2 * kv) * hd), _rand(g, n, h * hd)
+    for over in (1 << 31, 1 << 32, (1 << 32) + 5, 1 << 63):
+        got = []
+        for big in (None, over):
+            kw = dict(kv_heads=kv, left=big, right=big)
+            out, lse = ops.attn_window_fwd(qkv, 1, n, h, hd, **kw)
+            got += [(out, lse, ops.attn_window_bwd(qkv, out, dout, lse, 1, n, h, hd, **kw))]
+        out, lse = ops.attn_window_fwd(qkv, 1, n, h, hd, kv_heads=kv, left=3, right=0, sinks=over)
+        ref, _ = ops.attn_window_fwd(qkv, 1, n, h, hd, kv_heads=kv, left=None, right=0)
+        assert all(torch.equal(a, b) for a, b in zip(*got)) and torch.equal(out, ref)
+        offsets = torch.tensor([0, n], device=DEV)
+        cache, n32 = torch.zeros(2, 1, kv, 100, hd, device=DEV), torch.full((1,), n, dtype=torch.int32, device=DEV)
+        pos = torch.zeros(1, n, dtype=torch.int32, device=DEV)
+        for call in (lambda: ops.attn_window_fwd(qkv, 1, over, h, hd, kv_heads=kv, offsets=offsets), lambda: ops.attn_window_fwd(qkv, 1, n, h, hd, kv_heads=kv, left=-over),
+                     lambda: ops.kv_append(qkv, cache, n32, over, h, offsets=offsets), lambda: ops.kv_append(qkv, cache, n32, n, h, sinks=over),
+                     lambda: ops.attn_window_step(qkv[:1], cache, n32, h, left=over), lambda: ops.attn_window_step(qkv[:1], cache, n32, h, left=3, sinks=over),
+                     lambda: ops.rope_fwd(qkv, pos, over + 2, hd, (8,)), lambda: ops.rope_fwd(qkv, pos, 2, over + 32, (8,))):
+            with pytest.raises(RuntimeError, match="libstar_hip"):
+                call()
+        assert not cache.any()
