@@ -423,9 +423,8 @@ def _rows2d(t, shape, name):
 
 
 @functools.lru_cache(maxsize=256)
-def rope_plan(sections, base=10000.0, per_axis=False, interleaved=False):
-    """The frequencies of a rotation as star_rope takes them.  sections: how many pairs of a head turn by each position axis, in order;
-    pair i of all n turns by pos[its axis] * base**(-i / n), or with per_axis by base**(-k / m) for the k-th of its axis' m pairs."""
+def _rope_plan(sections, base, per_axis, interleaved):
+    """the plan that the calls share"""
     n = sum(sections)
     if any(s < 0 for s in sections) or not 0 < n <= 64 or n % 8 or len(sections) > 8:
         raise ValueError("sections of at most 8 axes must add up to a multiple of 8 pairs, at most 64 (got %r)" % (sections,))
@@ -441,9 +440,16 @@ def rope_plan(sections, base=10000.0, per_axis=False, interleaved=False):
     return f
 
 
+def rope_plan(sections, base=10000.0, per_axis=False, interleaved=False):
+    """The frequencies of a rotation as star_rope takes them.  sections: how many pairs of a head turn by each position axis, in order;
+    pair i of all n turns by pos[its axis] * base**(-i / n), or with per_axis by base**(-k / m) for the k-th of its axis' m pairs.  The caller's
+    own: what is written to it reaches no other call."""
+    return L.StarRope.from_buffer_copy(_rope_plan(tuple(sections), base, per_axis, interleaved))
+
+
 @functools.lru_cache(maxsize=256)
 def _rope_ref(sections, base, per_axis, interleaved):
-    plan = rope_plan(sections, base, per_axis, interleaved)
+    plan = _rope_plan(sections, base, per_axis, interleaved)
     return C.pointer(plan), plan.axes
 
 
@@ -463,7 +469,7 @@ def _rope(home, x, pos, rot_heads, hd, sections, base, per_axis, interleaved, ou
     ld = _rows2d(x, shape, "x")
     r, w = shape
     assert r < 1 << 31, "%d rows" % r
-    plan = rope_plan(tuple(sections), base, per_axis, interleaved)
+    plan = _rope_plan(tuple(sections), base, per_axis, interleaved)
     pos, pos_ld = _positions(pos, plan.axes, r)
     if out is None:
         out, out_ld = x.new_empty(r, w), w

@@ -67,3 +67,15 @@ def test_bounds_past_32_bits_stay_bounds(over):
     g = ops._window(x, 1, over, 4, 16, 2, None, 0, 0, torch.zeros(2, dtype=torch.int64), None)
     assert (g.L, g.left) == (2147483647, 2147483647)
     assert list(ops._ints(5, over, 0, -over)) == [5, 2147483647, 0, -1] and list(ops._ints(0, 7, 2147483647)) == [0, 7, 2147483647]
+
+
+def test_a_plan_is_the_callers_own():
+    first = ops.rope_plan((8, 8), base=500.0)
+    kept = list(first.rev)
+    first.rev[3] = 0.25
+    first.axis[3] = 7
+    again = ops.rope_plan((8, 8), base=500.0)
+    assert list(again.rev) == kept and again.axis[3] == 0
+    held, axes = ops._rope_ref((8, 8), 500.0, False, False)          # what the single-token step hands over
+    assert list(held.contents.rev) == kept and axes == 2
+    assert list(ops._rope_plan((8, 8), 500.0, False, False).rev) == kept
