@@ -405,9 +405,10 @@ def _at_home(fn):
 def _ints(*values):
     """values for int32 parameters.  ctypes would keep the low 32 bits of a longer one; it is handed over as the nearest that fits, which says
     the same (a bound over any length) or is refused."""
-    if min(values) < 0 or max(values) > 0x7fffffff:
-        return [max(-1, min(v, 0x7fffffff)) for v in values]
-    return values
+    every = 0
+    for v in values:
+        every |= v
+    return [max(-1, min(v, 0x7fffffff)) for v in values] if every >> 31 else values
 
 
 def _profiled(tag, nbytes, fn, *args):
