@@ -405,10 +405,7 @@ def _at_home(fn):
 def _ints(*values):
     """values for int32 parameters.  ctypes would keep the low 32 bits of a longer one; it is handed over as the nearest that fits, which says
     the same (a bound over any length) or is refused."""
-    every = 0
-    for v in values:
-        every |= v
-    return [max(-1, min(v, 0x7fffffff)) for v in values] if every >> 31 else values
+    return [max(-1, min(v, 0x7fffffff)) for v in values]
 
 
 def _profiled(tag, nbytes, fn, *args):
@@ -510,9 +507,15 @@ def _window(qkv, nb, l, h, hd, kv, left, right, sinks, offsets, scale):
     r, w = shape
     assert w == (h + 2 * kv) * hd, "qkv rows of %d columns are not %d + 2 * %d heads of %d" % (w, h, kv, hd)
     assert offsets is not None or r == nb * l, "%d rows for %d sequences of %d" % (r, nb, l)
-    return L.StarAttnWindow(qkv.data_ptr(), None if offsets is None else _offsets(offsets, nb), None, None, None, None, None, ld, r,
-                            *_ints(nb, l, h, kv, hd, l if left is None else left, l if right is None else right, sinks),
-                            hd ** -0.5 if scale is None else scale, L.dt_of(qkv))
+    if left is None:
+        left = l
+    if right is None:
+        right = l
+    sizes = nb, l, h, kv, hd, left, right, sinks
+    if (nb | l | h | kv | hd | left | right | sinks) >> 31:          # one of them negative or over 31 bits
+        sizes = _ints(*sizes)
+    return L.StarAttnWindow(qkv.data_ptr(), None if offsets is None else _offsets(offsets, nb), None, None, None, None, None, ld, r, *sizes, hd ** -0.5 if scale is None else scale,
+                            L.dt_of(qkv))
 
 
 @_at_home
@@ -633,7 +636,9 @@ def _window_step(home, qkv, cache, lengths, h, left, sinks, pos, sections, base,
         if left is None:
             left = cap - sinks - 1
         dt = L.dt_of(qkv)
-        sizes = nb, h, kv, hd, cap, left, sinks = _ints(nb, h, kv, hd, cap, left, sinks)
+        sizes = nb, h, kv, hd, cap, left, sinks
+        if (nb | h | kv | hd | cap | left | sinks) >> 31:
+            sizes = _ints(*sizes)
         need = _step_ws(home, *sizes, dt)
         ws = qkv.new_empty(need, dtype=torch.float32) if need else None
         g = L.StarAttnStep(qkv.data_ptr(), cache.data_ptr(), lengths.data_ptr(), None, None, out.data_ptr(), None if ws is None else ws.data_ptr(), ld, 0, *sizes,
