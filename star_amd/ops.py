@@ -417,7 +417,7 @@ def _rows2d(t, shape, name):
     """row stride of a matrix whose rows are dense and may lie apart: what the kernels take of packed qkv rows"""
     st = t.stride()
     assert len(shape) == 2 and (st[1] == 1 or shape[1] <= 1), "%s must be a matrix with dense rows" % name
-    return st[0] if shape[0] > 1 else max(st[0], shape[1])
+    return st[0] if shape[0] > 1 else shape[1]          # (what a single row's stride is says nothing: it may be odd, or millions)
 
 
 @functools.lru_cache(maxsize=256)

@@ -79,3 +79,9 @@ def test_a_plan_is_the_callers_own():
     held, axes = ops._rope_ref((8, 8), 500.0, False, False)          # what the single-token step hands over
     assert list(held.contents.rev) == kept and axes == 2
     assert list(ops._rope_plan((8, 8), 500.0, False, False).rev) == kept
+
+
+def test_the_stride_of_a_single_row_does_not_matter():
+    for ld in (65, 1 << 20):
+        wide = torch.zeros(2, ld)
+        assert ops._rows2d(wide[:1, :64], (1, 64), "x") == 64 and ops._rows2d(wide[:, :64], (2, 64), "x") == ld

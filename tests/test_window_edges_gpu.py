@@ -80,3 +80,30 @@ def test_bounds_past_32_bits():
             with pytest.raises(RuntimeError, match="libstar_hip"):
                 call()
         assert not cache.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_single_row_of_any_stride(dtype):
+    """one token out of a matrix whose rows are no multiple of 16 bytes apart, or over 2^24 bytes: the stride of a single row does not matter"""
+    g = _gen(3)
+    h, kv, hd, sections = 4, 2, 32, (4, 6, 6)
+    w = (h + 2 * kv) * hd
+    lone = _rand(g, 1, w, dtype=dtype)
+    pos = torch.full((3, 1), 77, dtype=torch.int32, device=DEV)
+    n32 = torch.ones(1, dtype=torch.int32, device=DEV)
+
+    def run(x):
+        out, lse = ops.attn_window_fwd(x, 1, 1, h, hd, kv_heads=kv)
+        cache = torch.zeros(2, 1, kv, 8, hd, dtype=dtype, device=DEV)
+        ops.kv_append(x, cache, n32, 1, h)
+        step = ops.attn_window_step(x, cache, n32, h, pos=pos, sections=sections)
+        return out, lse, ops.attn_window_bwd(x, out, out, lse, 1, 1, h, hd, kv_heads=kv), cache, step, ops.rope_fwd(x, pos, h + kv, hd, sections)
+
+    want = run(lone)
+    for ld in (w + 1, (1 << 24) + 8):
+        wide = torch.zeros(2, ld, dtype=dtype, device=DEV)
+        wide[0, :w] = lone[0]
+        for a, b in zip(run(wide[:1, :w]), want):
+            assert torch.equal(a, b)
+        view = wide[:1, :w]
+        assert ops.rope_fwd(view, pos, h + kv, hd, sections, out=view) is view and torch.equal(view, want[-1])
