@@ -632,7 +632,7 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_FWD(sizeof(T) * 
             const float mw = st[w * 128 + lane];
             l += st[w * 128 + 64 + lane] * (mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * c));       // -inf: 0, or NaN of a NaN score
         }
-        const float f = own_m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((own_m - m) * c) / l;
+        const float f = (own_m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((own_m - m) * c)) / l;        // every score -inf: 0 / 0, as in the row form
         const bool bad = any_wave_bad(any_bad<C>(o), st, wave, lane) && l == l;
         join_rows<C>(o, f, st + 512, q < len && !bad, (T*)a.out + (start + q) * a.H * HD + h * HD, wave, lane);
         if (bad && q < len && wave == 0) {

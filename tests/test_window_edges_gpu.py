@@ -107,3 +107,25 @@ def test_a_single_row_of_any_stride(dtype):
             assert torch.equal(a, b)
         view = wide[:1, :w]
         assert ops.rope_fwd(view, pos, h + kv, hd, sections, out=view) is view and torch.equal(view, want[-1])
+
+
+# ---- rows without a finite score ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("nb", [1, 200])
+def test_a_row_whose_scores_are_all_minus_infinity_is_nan(dtype, hd, nb):
+    """the softmax of such a row is 0 / 0, in few sequences as in many; its neighbours keep their results"""
+    g = _gen(hd)
+    n, h, left = 70, 4, 3
+    qkv = _rand(g, nb * n, 3 * h * hd, dtype=dtype)
+    qkv[:, :h * hd] = qkv[:, :h * hd].abs() + 0.1
+    clean = qkv.clone()
+    x = qkv.view(nb, n, -1)
+    x[:, [0, 40, 41, 42, 43], h * hd:2 * h * hd] = -float("inf")          # query 0 sees key 0 alone, query 43 keys 40 .. 43
+    hit = torch.zeros(n, dtype=torch.bool)
+    hit[[0, 43]] = True
+    out, lse = ops.attn_window_fwd(qkv, nb, n, h, hd, left=left)
+    out, lse = out.view(nb, n, -1).cpu(), lse.view(h, nb, n).cpu()
+    assert out[:, hit].isnan().all() and (lse[:, :, hit] == -float("inf")).all()
+    assert out[:, ~hit].isfinite().all() and lse[:, :, ~hit].isfinite().all()
+    assert torch.equal(out[:, 50:], ops.attn_window_fwd(clean, nb, n, h, hd, left=left)[0].view(nb, n, -1)[:, 50:].cpu())
