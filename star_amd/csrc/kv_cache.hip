@@ -289,9 +289,9 @@ __global__ __launch_bounds__(NT) void step_kernel(StepArgs a) {
         } else {
             float* w = a.ws + (((int64_t)b * a.H + h0 + g) * a.splits + split) * (HD + 2);
             w[d] = t;
-            if (d == 0) {
-                w[HD] = mn;
-                w[HD + 1] = ls;
+            if (d == 0) {       // an idle entry: weights of one, so that the join divides its zeros by something
+                w[HD] = seen.vis > 0 ? mn : 0.f;
+                w[HD + 1] = seen.vis > 0 ? ls : 1.f;
             }
         }
     }
@@ -316,8 +316,8 @@ __global__ __launch_bounds__(KT_) void step_join_kernel(const float* __restrict_
     if (tid < 64) {
         const float m = lane < splits ? w[lane * (HD + 2) + HD] : -INFINITY, l = lane < splits ? w[lane * (HD + 2) + HD + 1] : 0.f;
         const float mn = wave_max(m);
-        const float f = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn), sum = wave_sum(l * f);
-        sf[lane] = mn == -INFINITY ? 0.f : f / sum;         // an idle entry saw nothing: zeros
+        const float f = __builtin_amdgcn_exp2f(m - mn);         // every score -inf: NaN, as without splits
+        sf[lane] = f / wave_sum(l * f);
     }
     __syncthreads();
     float2 t = make_float2(0.f, 0.f);

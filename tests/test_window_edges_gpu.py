@@ -129,3 +129,21 @@ def test_a_row_whose_scores_are_all_minus_infinity_is_nan(dtype, hd, nb):
     assert out[:, hit].isnan().all() and (lse[:, :, hit] == -float("inf")).all()
     assert out[:, ~hit].isfinite().all() and lse[:, :, ~hit].isfinite().all()
     assert torch.equal(out[:, 50:], ops.attn_window_fwd(clean, nb, n, h, hd, left=left)[0].view(nb, n, -1)[:, 50:].cpu())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("nb,cap", [(3, 6000), (3, 40), (300, 40)])
+def test_a_step_whose_scores_are_all_minus_infinity_is_nan(dtype, hd, nb, cap):
+    """over split sequences as over whole ones; idle entries stay zeros"""
+    g = _gen(hd + cap)
+    h = kv = 4
+    qkv = _rand(g, nb, 3 * h * hd, dtype=dtype)
+    qkv[:, :h * hd] = qkv[:, :h * hd].abs() + 0.1
+    cache = torch.randn(2, nb, kv, cap, hd, generator=torch.Generator(DEV).manual_seed(3), device=DEV).to(dtype)
+    lengths = torch.full((nb,), cap, dtype=torch.int32, device=DEV)
+    cache[0, 0] = -float("inf")
+    qkv[0, h * hd:2 * h * hd] = -float("inf")
+    lengths[1] = 0
+    out = ops.attn_window_step(qkv, cache, lengths, h)
+    assert out[0].isnan().all() and not out[1].any() and out[2:].isfinite().all()
