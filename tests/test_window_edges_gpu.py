@@ -49,10 +49,11 @@ def test_results_on_operands_are_refused(dtype):
     alone, _ = ops.attn_window_fwd(row, 1, 1, h, hd, kv_heads=kv)
     one = torch.zeros(2, 1, kv, 8, hd, dtype=dtype, device=DEV)
     step = ops.attn_window_step(row, one, lengths[:1], h)
-    for call in (lambda r: ops.attn_window_fwd(r, 1, 1, h, hd, kv_heads=kv, out=r[:, :h * hd]), lambda r: ops.attn_window_step(r, one, lengths[:1], h, out=r[:, :h * hd])):
+    for call, result in ((lambda r: ops.attn_window_fwd(r, 1, 1, h, hd, kv_heads=kv, out=r[:, :h * hd]), alone),
+                         (lambda r: ops.attn_window_step(r, one, lengths[:1], h, out=r[:, :h * hd]), step)):
         r = row.clone()
         call(r)
-        assert torch.equal(r[:, :h * hd], alone) and torch.equal(r[:, :h * hd], step) and torch.equal(r[:, h * hd:], row[:, h * hd:])
+        assert torch.equal(r[:, :h * hd], result) and torch.equal(r[:, h * hd:], row[:, h * hd:])
     assert torch.equal(ops.attn_window_bwd(qkv, out, dout, lse, 1, n, h, hd, kv_heads=kv), want)
 
 
