@@ -148,3 +148,28 @@ def test_a_step_whose_scores_are_all_minus_infinity_is_nan(dtype, hd, nb, cap):
     lengths[1] = 0
     out = ops.attn_window_step(qkv, cache, lengths, h)
     assert out[0].isnan().all() and not out[1].any() and out[2:].isfinite().all()
+
+
+# ---- data that has gone NaN -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,hd,left", [(torch.bfloat16, 64, None), (torch.bfloat16, 128, 600), (torch.float32, 32, None)])
+def test_gradients_that_are_all_nan_take_no_sweep_of_their_own(dtype, hd, left):
+    """a gradient of the result that is NaN everywhere: so is every gradient, in about the time of an ordinary pass.  (Rows formed again one
+    visible row at a time would take 80 times as long.)"""
+    g = _gen(hd)
+    nb, n, h, kv = 2, 2048, 8, 2
+    qkv, dout = _rand(g, nb * n, (h + 2 * kv) * hd, dtype=dtype), _rand(g, nb * n, h * hd, dtype=dtype)
+    kw = dict(kv_heads=kv, left=left)
+    out, lse = ops.attn_window_fwd(qkv, nb, n, h, hd, **kw)
+    took = []
+    for grad in (dout, torch.full_like(dout, float("nan"))):
+        times = []
+        for _ in range(6):
+            marks = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            marks[0].record()
+            dqkv = ops.attn_window_bwd(qkv, out, grad, lse, nb, n, h, hd, **kw)
+            marks[1].record()
+            torch.cuda.synchronize()
+            times.append(marks[0].elapsed_time(marks[1]))
+        took.append(min(times))
+        assert (dqkv.isnan().all() if grad is not dout else dqkv.isfinite().all())
+    assert took[1] < 10 * took[0], took
