@@ -1186,18 +1186,22 @@ template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t
 }
 
 // How the far queries of the sinks are cut: about two blocks of four waves per compute unit in all, no more than 16 parts to add up, and at least
-// two 32-query tiles for a wave.  With over 256 sinks, or very many heads, there are enough key blocks with a long sweep to fill the chip: no parts.
-// Nor with under 24 tiles per key head, which the sinks' own block takes in the time of the other launches (without parts / with: float32, 500 rows,
-// 8 heads of 64, 13 tiles: 49 / 75 us; 4 x 700 rows, 16 heads, 18 tiles: 212 / 226; 2 x 1000 rows, 12 heads of 32, 24 tiles: 91.7 / 88.5; 4 x 1000 rows,
-// 16 heads of 64, 29 tiles: 390 / 263; bf16, 20 x 900 rows, 12 heads of 64, 27 tiles: 192 / 169).
-static void far_plan(int NB, int L, int H, int KV, int left, int sinks, int& groups, int& parts) {
+// two 32-query tiles for a wave.  No parts with under 24 tiles per key head, which the sinks' own block takes in the time of the other launches
+// (without parts / with: float32, 500 rows, 8 heads of 64, 13 tiles: 49 / 75 us; 4 x 700 rows, 16 heads, 18 tiles: 212 / 226; 2 x 1000 rows, 12
+// heads of 32, 24 tiles: 91.7 / 88.5; 4 x 1000 rows, 16 heads of 64, 29 tiles: 390 / 263; bf16, 20 x 900 rows, 12 heads of 64, 27 tiles: 192 / 169).
+// Over 256 sinks: none where their own blocks are enough to fill the chip or a third of all keys, so that no few of them are waited for (backward,
+// without / with: 1 x 8192 rows, 4 heads on 1, 257 sinks, 9 lists of 32: bf16 of 64 288 / 87 us, of 128 419 / 118, float32 of 128 2519 / 535; 1 x 4096, 8
+// heads, 300 sinks, 80 lists: 75 / 82, 244 / 140, 1366 / 553; 1 x 4096, 8 heads, 1000 sinks, 256 lists: 89 / 101, 262 / 175, 1496 / 832; 8 x 2048, 16
+// heads, 300 sinks, 1280 lists: 250 / 259, 491 / 511, 3296 / 2879; 2 x 1024, 4 heads, 500 sinks, 128 lists: 30 / 37, 40 / 60, 144 / 149).
+static void far_plan(int NB, int L, int H, int KV, int left, int sinks, int row_bytes, int& groups, int& parts) {
     groups = parts = 0;
     sinks = sinks < L ? sinks : L;
-    if (sinks <= 0 || sinks > 256 || left >= L - 1) return;
-    const int64_t lists = (int64_t)NB * KV * cdiv(sinks, 32), tiles = (int64_t)(H / KV) * cdiv(L - left - 1, 32);
+    if (sinks <= 0 || left >= L - 1) return;
+    const int64_t lists = (int64_t)NB * KV * cdiv(sinks, 32), tiles = (int64_t)(H / KV) * cdiv(L - left - 1, 32), cus = star_num_cus();
     if (lists > 65535 || tiles < 24) return;
+    if (sinks > 256 && (3 * (int64_t)sinks > L || 2 * lists > (row_bytes < 256 ? 1 : 4) * cus)) return;
     groups = cdiv(sinks, 32);
-    int64_t p = cdiv(2 * (int64_t)star_num_cus(), lists);
+    int64_t p = cdiv(2 * cus, lists);
     if (p > tiles / 8) p = tiles / 8;
     parts = p < 1 ? 1 : p > 16 ? 16 : (int)p;
 }
@@ -1252,7 +1256,7 @@ extern "C" int star_attn_window_fwd(const StarAttnWindow* g, void* stream) {
 extern "C" int64_t star_attn_window_bwd_ws(int64_t R, int NB, int L, int H, int KV, int hd, int left, int sinks, int dt) {
     if (R < 0 || NB <= 0 || L <= 0 || H <= 0 || KV <= 0 || H % KV || hd <= 0 || left < 0 || sinks < 0) return 0;
     int groups, parts;
-    far_plan(NB, longest(L, R), H, KV, left, sinks, groups, parts);
+    far_plan(NB, longest(L, R), H, KV, left, sinks, hd * (dt == STAR_BF16 ? 2 : 4), groups, parts);
     return (H * R + 63) / 64 * 64 + (int64_t)NB * KV * groups * parts * 2 * 32 * (hd < 32 ? 32 : hd);
 }
 
@@ -1274,7 +1278,7 @@ extern "C" int star_attn_window_bwd(const StarAttnWindow* g, void* stream) {
     a.dqkv = g->dqkv;
     a.ndelta = g->ws;
     a.rest_blocks = rest_blocks(g, (int64_t)(g->H + 2 * g->KV) * g->hd);
-    far_plan(g->NB, a.L, g->H, g->KV, g->left, g->sinks, a.far_groups, a.far_parts);
+    far_plan(g->NB, a.L, g->H, g->KV, g->left, g->sinks, g->hd * (int)es, a.far_groups, a.far_parts);
     a.far_ws = g->ws + (g->H * g->R + 63) / 64 * 64;
     hipStream_t s = (hipStream_t)stream;
     return g->dt == STAR_BF16 ? BY_HD(run_bwd, bf16_t) : BY_HD(run_bwd, float);

@@ -85,3 +85,20 @@ def test_the_stride_of_a_single_row_does_not_matter():
     for ld in (65, 1 << 20):
         wide = torch.zeros(2, ld)
         assert ops._rows2d(wide[:1, :64], (1, 64), "x") == 64 and ops._rows2d(wide[:, :64], (2, 64), "x") == ld
+
+
+# ---- launch forms ---------------------------------------------------------------------------------------------------------------
+def _far_floats(rows, nb, l, h, kv, hd, left, sinks, dt=L.BF16):
+    """what the far queries of the sinks take of the backward pass' workspace, behind the row dots; 0: they are left to the sinks' own blocks"""
+    return L.lib().star_attn_window_bwd_ws(rows, nb, l, h, kv, hd, left, sinks, dt) - (h * rows + 63) // 64 * 64
+
+
+def test_far_queries_of_many_sinks():
+    """one sink more or less does not decide it: few blocks with a long sweep among many with short ones are shared out whatever their sinks' number"""
+    for hd, dt in ((64, L.BF16), (128, L.BF16), (16, L.BF16), (128, L.F32)):
+        for sinks in (1, 256, 257, 512, 2000):
+            lists, per = (sinks + 31) // 32, 2 * 32 * max(32, hd)
+            assert _far_floats(8192, 1, 8192, 4, 1, hd, 512, sinks, dt) in [lists * parts * per for parts in range(2, 17)], sinks
+        assert _far_floats(8192, 1, 8192, 4, 1, hd, 512, 3000, dt) == 0                  # over a third of the keys
+        assert _far_floats(16 * 8192, 16, 8192, 16, 16, hd, 512, 600, dt) == 0           # 4864 blocks of sinks
+        assert _far_floats(8192, 1, 8192, 4, 1, hd, 8191, 300, dt) == 0                  # no query beyond the window

@@ -3,6 +3,7 @@ without a finite score, data that has gone NaN, the far queries of many sinks, v
 import pytest
 import torch
 
+from window_util import assert_within, heads, reference, seen, unpack
 
 pytestmark = pytest.mark.gpu
 
@@ -173,3 +174,63 @@ def test_gradients_that_are_all_nan_take_no_sweep_of_their_own(dtype, hd, left):
         took.append(min(times))
         assert (dqkv.isnan().all() if grad is not dout else dqkv.isfinite().all())
     assert took[1] < 10 * took[0], took
+
+
+# ---- the far queries of the sinks -----------------------------------------------------------------------------------------------
+def _passes(qkv, dout, nb, n, h, hd, **kw):
+    out, lse = ops.attn_window_fwd(qkv, nb, n, h, hd, **kw)
+    return out, lse, ops.attn_window_bwd(qkv, out, dout, lse, nb, n, h, hd, **kw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("nb,sinks", [(1, 2), (48, 33), (1, 280), (1, 256), (1, 320), (40, 280)])
+def test_far_queries(dtype, hd, nb, sinks):
+    """sinks whose sweeps run far beyond the window, in few and in many sequences: shared out over blocks of their own, or (320 of 900 keys; 40 sequences
+    of 280) left to the sinks' blocks"""
+    g = _gen(hd + sinks)
+    n, h, kv, left, right = 900, 4, 2, 20, 3
+    qkv, dout = _rand(g, nb * n, (h + 2 * kv) * hd, dtype=dtype, mul=1.2), _rand(g, nb * n, h * hd, dtype=dtype)
+    out, lse, dqkv = _passes(qkv, dout, nb, n, h, hd, kv_heads=kv, left=left, right=right, sinks=sinks)
+    for b in sorted({0, nb - 1}):
+        rows = slice(b * n, (b + 1) * n)
+        want = reference(*unpack(qkv[rows], h, kv, hd), left, right, sinks, None, heads(dout[rows], hd), dtype)
+        assert_within(heads(out[rows], hd), want["out"], want["tol_out"], "out")
+        assert_within(heads(dqkv[rows], hd), want["dqkv"], want["tol_dqkv"], "dqkv")
+    again = _passes(qkv, dout, nb, n, h, hd, kv_heads=kv, left=left, right=right, sinks=sinks)
+    assert torch.equal(out, again[0]) and torch.equal(dqkv, again[2])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("nb", [1, 48])
+def test_far_queries_that_are_not_finite_reach_their_sinks_alone(dtype, hd, nb):
+    """infinities and NaN in rows far behind the sinks: the sinks and whoever else sees them take them, the keys beside the sinks do not"""
+    g = _gen(hd + nb)
+    n, h, kv, left, sinks = 1000, 4, 2, 24, 5
+    see = seen(n, left, 0, sinks)
+    clean, dout = _rand(g, nb * n, (h + 2 * kv) * hd, dtype=dtype), _rand(g, nb * n, h * hd, dtype=dtype)
+    wild = torch.zeros(n, dtype=torch.bool)
+    wild[[300, 301, 650] + list(range(960, 964))] = True
+    at = wild.to(DEV)
+    # every column of the rows and of the gradient NaN; values alone infinite; the gradient of the result alone
+    for what, value in (("rows", float("nan")), ("values", float("inf")), ("gradient", float("nan")), ("gradient", float("inf"))):
+        qkv, grad = clean.clone().view(nb, n, -1), dout.clone().view(nb, n, -1)
+        if what != "gradient":
+            qkv[:, at, 0 if what == "rows" else (h + kv) * hd:] = value
+        if what != "values":
+            grad[:, at] = value
+        out, lse, dqkv = _passes(qkv.view(nb * n, -1), grad.view(nb * n, -1), nb, n, h, hd, kv_heads=kv, left=left, sinks=sinks)
+        hit = (see & wild).any(1) if what != "gradient" else torch.zeros(n, dtype=torch.bool)          # queries whose result is not finite
+        hit_q = hit | wild if what != "values" else hit
+        hit_key = (see & hit_q[:, None]).any(0) | (wild if what != "gradient" else False)
+        assert hit_key[:sinks].all() and not hit_key[sinks:250].any()
+        for b in sorted({0, nb - 1}):
+            rows = slice(b * n, (b + 1) * n)
+            want = reference(*unpack(clean[rows], h, kv, hd), left, 0, sinks, None, heads(dout[rows], hd), dtype)
+            o, d = heads(out[rows], hd), heads(dqkv[rows], hd)
+            assert_within(o[:, ~hit], want["out"][:, ~hit], want["tol_out"][:, ~hit], "out")
+            assert_within(d[:h, ~hit_q], want["dqkv"][:h, ~hit_q], want["tol_dqkv"][:h, ~hit_q], "dq")
+            assert_within(d[h:, ~hit_key], want["dqkv"][h:, ~hit_key], want["tol_dqkv"][h:, ~hit_key], "dk, dv")
+            if what == "rows" or what == "gradient":
+                assert not torch.isfinite(d[h:, :sinks]).any()
