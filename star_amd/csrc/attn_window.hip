@@ -1151,9 +1151,13 @@ template <typename T, int HD, int FORM> static int launch_dkv(const WArgs& a, hi
     const int64_t blocks = FORM == FAR_FORM ? (int64_t)a.NB * a.KV * a.far_groups * a.far_parts : grid_of(a, OWN ? 32 : WROWS, a.KV);
     return launch<window_dkv_kernel<T, HD, FORM>>("star_attn_window_bwd", blocks, OWN && LDS < 18432 ? 18432 : LDS, a, s);
 }
+// the hardware counts a launch's threads in 32 bits: checked before the first launch of a call
+static bool grid_fits(const WArgs& a, bool split, int heads) { return (grid_of(a, split ? 32 : WROWS, heads) + a.rest_blocks) * WT < (1ll << 32); }
 template <typename T, int HD> static int run_fwd(const WArgs& a, hipStream_t s) {
     using S = SplitUpTo<T, HD>;
-    if (few_blocks(a, a.H, S::rows(sweep_class(a)))) return launch_fwd<T, HD, true>(a, s);
+    const bool split = few_blocks(a, a.H, S::rows(sweep_class(a)));
+    STAR_CHECK(grid_fits(a, split, a.H), "star_attn_window_fwd: NB, H, L too large for the grid");
+    if (split) return launch_fwd<T, HD, true>(a, s);
     return launch_fwd<T, HD, false>(a, s);
 }
 template <typename T, int HD> static int run_dq(const WArgs& a, hipStream_t s) {
@@ -1168,6 +1172,10 @@ template <typename T, int HD> static int run_dkv(const WArgs& a, hipStream_t s) 
 }
 template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t s) {
     const char* who = "star_attn_window_bwd";
+    using S = SplitUpTo<T, HD>;
+    const int sweep = sweep_class(first);
+    STAR_CHECK(grid_fits(first, few_blocks(first, first.H, S::rows(sweep)), first.H) && grid_fits(first, few_blocks(first, first.KV, S::keys(sweep)), first.KV),
+               "%s: NB, H, L too large for the grid", who);
     int rc = run_dq<T, HD>(first, s);
     if (rc) return rc;
     WArgs a = first;
@@ -1176,7 +1184,7 @@ template <typename T, int HD> static int run_bwd(const WArgs& first, hipStream_t
         if ((rc = launch_dkv<T, HD, FAR_FORM>(a, s))) return rc;
         // the split form adds the parts up itself where a row is under 256 bytes (7 sequences of 0 .. 2043 rows, 16 heads on 4 of 64: 122 us against
         // 128; 128-wide heads have too few registers to keep the loads in flight: 102 against 48)
-        if (a.far_parts > 1 && !(HD * sizeof(T) < 256 && few_blocks(a, a.KV, SplitUpTo<T, HD>::keys(sweep_class(a))))) {
+        if (a.far_parts > 1 && !(HD * sizeof(T) < 256 && few_blocks(a, a.KV, S::keys(sweep)))) {
             const int size = 2 * WCfg<T, HD>::DB * 1024;
             hipLaunchKernelGGL(window_far_fold_kernel, dim3(size / WT, a.NB * a.KV * a.far_groups), dim3(WT), 0, s, a.far_ws, a.far_parts, size);
             STAR_LAUNCH_CHECK(who);

@@ -449,7 +449,8 @@ extern "C" int star_attn_window_step(const StarAttnStep* g, void* stream) {
     a.splits = plan.splits;
     STAR_CHECK(a.splits == 1 || g->ws, "star_attn_window_step: null workspace (star_attn_window_step_ws)");
     const int64_t blocks = ((int64_t)g->NB * g->KV * a.splits + 7) / 8 * 8 * a.chunks;
-    STAR_CHECK(blocks < (1ll << 31), "star_attn_window_step: NB, KV too large for the grid");
+    // the hardware counts a launch's threads in 32 bits
+    STAR_CHECK(blocks * plan.threads < (1ll << 32) && (a.splits == 1 || (int64_t)g->NB * g->H * KT_ < (1ll << 32)), "star_attn_window_step: NB, H too large for the grid");
     // (a single row in place: the blocks of a head alone read its query)
     const int64_t out_bytes = (int64_t)g->NB * g->H * g->hd * es, cache_bytes = 2 * (int64_t)g->NB * g->KV * g->cap * g->hd * es, row = (int64_t)(g->H + 2 * g->KV) * g->hd * es;
     const int64_t ws_bytes = a.splits == 1 ? 0 : (int64_t)g->NB * g->H * a.splits * (g->hd + 2) * 4;

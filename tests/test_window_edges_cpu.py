@@ -102,3 +102,14 @@ def test_far_queries_of_many_sinks():
         assert _far_floats(8192, 1, 8192, 4, 1, hd, 512, 3000, dt) == 0                  # over a third of the keys
         assert _far_floats(16 * 8192, 16, 8192, 16, 16, hd, 512, 600, dt) == 0           # 4864 blocks of sinks
         assert _far_floats(8192, 1, 8192, 4, 1, hd, 8191, 300, dt) == 0                  # no query beyond the window
+
+
+# ---- grids: the hardware counts a launch's threads in 32 bits -------------------------------------------------------------------
+def test_grids_past_the_hardwares_are_refused():
+    far = [(i + 1) << 44 for i in range(6)]
+    for nb, l, offsets in ((1 << 20, 1, None), (1 << 14, 128 * 64, None), (1 << 20, 100, 1 << 20)):          # 2^24 blocks of 256 threads
+        a = _attn(qkv=far[0], out=far[1], lse=far[2], dout=far[3], dqkv=far[4], ws=far[5], ld=48 * 16, NB=nb, L=l, R=nb * l, H=16, KV=16, hd=16, offsets=offsets)
+        for name in ("star_attn_window_fwd", "star_attn_window_bwd"):
+            _refused(getattr(L.lib(), name)(C.byref(a), None), name, "grid")
+    a = L.StarAttnStep(qkv=far[0], cache=far[1], lengths=far[2], out=far[3], ws=far[4], ld=48, NB=1 << 22, H=1, KV=1, hd=16, cap=64, left=31, sinks=4, scale=0.25, dt=L.F32)
+    _refused(L.lib().star_attn_window_step(C.byref(a), None), "star_attn_window_step", "grid")
