@@ -118,10 +118,15 @@ extern "C" int star_rope(const void* x, int64_t x_ld, void* y, int64_t y_ld, con
     // a few rows per block so that the angle pass fills its threads; single rows while there are fewer blocks than compute units
     int rows = MAX_ROWS;
     while (rows > 1 && cdiv(R, rows) < 2 * star_num_cus()) rows /= 2;
-    const RopeArgs a = {x, y, pos, x_ld, y_ld, pos_ld, R, W, rot_heads, hd, rows, inverse ? -1.0f : 1.0f, *h_rope};
+    // the hardware counts a launch's threads in 32 bits: 2^26 rows at a time
+    const int most = 1 << 26;
     hipStream_t s = (hipStream_t)stream;
-    if (dt == STAR_BF16) hipLaunchKernelGGL(rope_kernel<bf16_t>, dim3(cdiv(R, rows)), dim3(RT), 0, s, a);
-    else hipLaunchKernelGGL(rope_kernel<float>, dim3(cdiv(R, rows)), dim3(RT), 0, s, a);
-    STAR_LAUNCH_CHECK("star_rope");
+    for (int64_t r0 = 0; r0 < R; r0 += most) {
+        const int part = R - r0 < most ? (int)(R - r0) : most;
+        const RopeArgs a = {(const char*)x + r0 * x_ld * es, (char*)y + r0 * y_ld * es, pos + r0, x_ld, y_ld, pos_ld, part, W, rot_heads, hd, rows, inverse ? -1.0f : 1.0f, *h_rope};
+        if (dt == STAR_BF16) hipLaunchKernelGGL(rope_kernel<bf16_t>, dim3(cdiv(part, rows)), dim3(RT), 0, s, a);
+        else hipLaunchKernelGGL(rope_kernel<float>, dim3(cdiv(part, rows)), dim3(RT), 0, s, a);
+        STAR_LAUNCH_CHECK("star_rope");
+    }
     return 0;
 }

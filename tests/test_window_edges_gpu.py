@@ -234,3 +234,19 @@ def test_far_queries_that_are_not_finite_reach_their_sinks_alone(dtype, hd, nb):
             assert_within(d[h:, ~hit_key], want["dqkv"][h:, ~hit_key], want["tol_dqkv"][h:, ~hit_key], "dk, dv")
             if what == "rows" or what == "gradient":
                 assert not torch.isfinite(d[h:, :sinks]).any()
+
+
+# ---- very many rows -------------------------------------------------------------------------------------------------------------
+def test_rope_of_more_rows_than_one_grid_holds():
+    """2^27 rows and some, of one head: blocks of 256 threads for eight rows each are over 2^32 threads"""
+    rows, hd, sections, part = (1 << 27) + 1003, 16, (4, 4), 1 << 25
+    g = torch.Generator(DEV).manual_seed(7)
+    x = torch.empty(rows, hd, dtype=torch.bfloat16, device=DEV)
+    for at in range(0, rows, part):
+        x[at:at + part] = torch.randn(min(part, rows - at), hd, generator=g, device=DEV)
+    pos = torch.randint(0, 100000, (2, rows), generator=g, device=DEV, dtype=torch.int32)
+    y = ops.rope_fwd(x, pos, 1, hd, sections)
+    for at in range(0, rows, part):
+        assert torch.equal(y[at:at + part], ops.rope_fwd(x[at:at + part], pos[:, at:at + part].contiguous(), 1, hd, sections)), at
+    ops.rope_fwd(x, pos, 1, hd, sections, out=x)
+    assert torch.equal(x, y)
