@@ -250,3 +250,55 @@ def test_rope_of_more_rows_than_one_grid_holds():
         assert torch.equal(y[at:at + part], ops.rope_fwd(x[at:at + part], pos[:, at:at + part].contiguous(), 1, hd, sections)), at
     ops.rope_fwd(x, pos, 1, hd, sections, out=x)
     assert torch.equal(x, y)
+
+
+# ---- prompts among idle entries -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nb", [40, 3000])
+def test_append_of_unequal_prompts_among_many(dtype, nb):
+    """more rows than a sequence's blocks take in one go, the sinks among them, beside empty and short sequences"""
+    g = _gen(nb)
+    h, kv, hd, cap, sinks = 2, 2, 64, 300, 5
+    lens = [0] * nb
+    lens[3], lens[nb // 2], lens[nb - 1], lens[7] = 20000, 1, 400, 290
+    before = [(17 * b) % 700 for b in range(nb)]
+    rows = sum(lens)
+    qkv = torch.randn(rows, (h + 2 * kv) * hd, generator=torch.Generator(DEV).manual_seed(nb), device=DEV).to(dtype)
+    cache = torch.randn(2, nb, kv, cap, hd, generator=torch.Generator(DEV).manual_seed(1), device=DEV).to(dtype)
+    want = cache.clone()
+    ends = torch.tensor(lens).cumsum(0)
+    lengths = [n + c for n, c in zip(lens, before)]
+    x = qkv.view(rows, h + 2 * kv, hd)
+    for b, n in enumerate(lens):
+        p = torch.arange(lengths[b] - n, lengths[b])
+        keep = (p < sinks) | (p >= lengths[b] - (cap - sinks))
+        slot = torch.where(p < sinks, p, sinks + (p - sinks) % (cap - sinks))[keep].to(DEV)
+        src = x[int(ends[b]) - n:int(ends[b])][keep.to(DEV)]
+        want[0, b][:, slot], want[1, b][:, slot] = src[:, h:h + kv].transpose(0, 1), src[:, h + kv:].transpose(0, 1)
+    offsets = torch.cat((torch.zeros(1, dtype=torch.int64), ends)).to(DEV)
+    ops.kv_append(qkv, cache, torch.tensor(lengths, dtype=torch.int32, device=DEV), max(lens), h, sinks=sinks, offsets=offsets)
+    assert torch.equal(cache, want)
+
+
+def test_append_takes_no_time_for_idle_entries():
+    """one prompt among thousands of idle entries, against a call for the prompt alone.  (Entries that walk the longest one's rows take 2000 times
+    its time.)"""
+    rows, kv, hd, cap = 200000, 2, 64, 64
+    qkv = torch.randn(rows, 3 * kv * hd, device=DEV)
+    took = []
+    for nb in (1, 4096):
+        cache = torch.zeros(2, nb, kv, cap, hd, device=DEV)
+        offsets = torch.full((nb + 1,), rows, dtype=torch.int64, device=DEV)
+        offsets[0] = 0
+        lengths = torch.zeros(nb, dtype=torch.int32, device=DEV)
+        lengths[0] = rows
+        times = []
+        for _ in range(6):
+            marks = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            marks[0].record()
+            ops.kv_append(qkv, cache, lengths, rows, kv, offsets=offsets)
+            marks[1].record()
+            torch.cuda.synchronize()
+            times.append(marks[0].elapsed_time(marks[1]))
+        took.append(min(times))
+    assert took[1] < 100 * took[0] and took[1] < 3.0, took
