@@ -1105,7 +1105,7 @@ static int64_t grid_of(const WArgs& a, int rows, int heads) {
 // A window open to one side leaves blocks with long and with short sweeps, and the launch waits for the longest, which the split form cuts in four:
 // higher limits from 1024 and from 2048 keys on (causal, 4096 rows: hd 32 47 / 68 at 512 blocks, 71 / 89 at 768; hd 64 36 / 65 at 256, 97 / 106 at
 // 768; hd 128 69 / 79 at 256, 136 / 113 at 512; float32 hd 32 165 / 309 at 512, 247 / 442 at 768, hd 128 325 / 561 at 256, 629 / 644 at 512, 952 /
-1201 at 768, 1243 / 1215 at 1024; 1536 rows: 121 / 224 at 192, 318 / 431 at 576; with a window of 1024 as for the others.  The
+// 1201 at 768, 1243 / 1215 at 1024; 1536 rows: 121 / 224 at 192, 318 / 431 at 576; with a window of 1024 as for the others.  The
 // whole backward pass, dK/dV split / row: hd 32 114 / 144 at 512, hd 64 174 / 203, hd 128 214 / 290 at 256, 4 heads a group 599 / 959; float32 hd
 // 64 1124 / 1476 at 512, hd 128 1137 / 1968 at 256, 3436 / 4209 at 768, 1536 rows 407 / 754 at 192, 1137 / 1512 at 576).
 template <typename T, int HD> struct SplitUpTo {
