@@ -371,7 +371,10 @@ extern "C" int star_kv_append(const void* qkv, int64_t ld, const int64_t* offset
 
 // Query heads of a key head that one block serves: they share every row it reads, but its one or two rounds of rows cost the more arithmetic.  More
 // than two only where the key heads alone fill the chip (1 sequence, 32 heads of 128 on 8, 1000 tokens: 11.8 us with four, 9.1 with two, 8.5 with one; 16 x
-// 8 heads of 64 on 1, 2000 tokens: 12.8, 11.7, 11.0; 8 x 32 on 8, 4096 tokens: 33.6, 31.5, 82.3).
+// 8 heads of 64 on 1, 2000 tokens: 12.8, 11.7, 11.0; 8 x 32 on 8, 4096 tokens: 33.6, 31.5, 82.3).  Eight for groups over four heads, or four where the
+// sequences are split and four twice hold the group (64 x 64 heads of 128 on 8, 4096 tokens: 318 us with eight, 340 with four, 407 with two; 64 x 64 of 64 on
+// 8, 500 tokens: 36, 47; 260 x 32 of 64 on 2, 1500 tokens, split: 129, 163; but 34 x 64 of 64 on 8, 2400 tokens, split: 73, 59, 63; 300 x 8 of 128 on 1,
+// 1000 tokens, split: 78, 59).
 static int step_group(int NB, int H, int KV) {
     const int rep = H / KV;
     if ((int64_t)NB * KV < star_num_cus()) return rep > 1 ? 2 : 1;
@@ -384,20 +387,26 @@ static int step_group(int NB, int H, int KV) {
 // 32 heads on 8 of 128, 1000 tokens 14.9 us against 18.2 with eight; 33 x 8 heads of 128, 6000 tokens 152 us, 195 with whole sequences, which
 // leave the second round of compute units nearly empty); no more splits than hold rows.
 struct StepPlan {
-    int threads, splits;
+    int group, threads, splits;
 };
 static StepPlan step_plan(int NB, int H, int KV, int hd, int es, int cap, int left, int sinks) {
-    const int rep = H / KV, G = step_group(NB, H, KV), wide = G == 8 ? 512 : 1024;
-    const int64_t blocks = (int64_t)NB * KV * cdiv(rep, G);
+    const int rep = H / KV;
+    int G = step_group(NB, H, KV);
+    const int wide = G == 8 ? 512 : 1024;
+    int64_t blocks = (int64_t)NB * KV * cdiv(rep, G);
     const int64_t vis = (int64_t)left + 1 + sinks < cap ? (int64_t)left + 1 + sinks : cap;
     const int per = 4 * 64 / (hd * es / 16);              // rows of a wave's round
     const int64_t cus = star_num_cus();
-    if (vis <= 3 * per * (wide / 64) || (blocks >= cus && blocks * 10 >= cdiv(blocks, cus) * cus * 9)) return {wide, 1};
+    if (vis <= 3 * per * (wide / 64) || (blocks >= cus && blocks * 10 >= cdiv(blocks, cus) * cus * 9)) return {G, wide, 1};
+    if (G == 8 && rep <= 8) {
+        G = 4;
+        blocks *= 2;
+    }
     const int64_t rounds = (vis + per * 4 - 1) / (per * 4);
     int64_t s = ((blocks < cus ? 4 : 8) * cus + blocks - 1) / blocks;
     s = s < 1 ? 1 : s > 64 ? 64 : s > rounds ? rounds : s;
     const int64_t each = (rounds + s - 1) / s;
-    return {KT_, (int)((rounds + each - 1) / each)};
+    return {G, KT_, (int)((rounds + each - 1) / each)};
 }
 
 extern "C" int64_t star_attn_window_step_ws(int NB, int H, int KV, int hd, int cap, int left, int sinks, int dt) {
@@ -446,9 +455,9 @@ extern "C" int star_attn_window_step(const StarAttnStep* g, void* stream) {
             STAR_CHECK(g->h_rope->axis[i] < g->h_rope->axes, "star_attn_window_step: pair %d turns by axis %d of %d", i, g->h_rope->axis[i], g->h_rope->axes);
         a.f = *g->h_rope;
     }
-    const int rep = g->H / g->KV, G = step_group(g->NB, g->H, g->KV);
-    a.chunks = cdiv(rep, G);
     const StepPlan plan = step_plan(g->NB, g->H, g->KV, g->hd, es, g->cap, g->left, g->sinks);
+    const int G = plan.group;
+    a.chunks = cdiv(g->H / g->KV, G);
     a.splits = plan.splits;
     STAR_CHECK(a.splits == 1 || g->ws, "star_attn_window_step: null workspace (star_attn_window_step_ws)");
     const int64_t blocks = ((int64_t)g->NB * g->KV * a.splits + 7) / 8 * 8 * a.chunks;
