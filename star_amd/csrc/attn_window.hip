@@ -667,9 +667,11 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_FWD(sizeof(T) * 
 }
 
 // dQ, the query on the lane; also -delta = -rowsum(dO * O), which the dK/dV kernels launched behind this one read.
-// In bf16 the rows of O are rounded, and with few visible keys that is felt: dP - delta cancels, and dQ and dK are up to 1.9 times as far off as one
-// rounding of the results leaves them (7 keys a row 1.72, 33 on average 1.55, 184 1.48, 258 and more 1.45).  The sum of the row's dS, which is
-// zero by the formula, is just what delta is short of: blocks whose rows see at most FEW_KEYS take it in a sweep of its own first.
+// In bf16 the rows of O are rounded, and with few visible keys that is felt: dP - delta cancels, and dQ and dK are up to 1.84 times as far off as one
+// rounding of the results leaves them.  The sum of the row's dS, which is zero by the formula, is just what delta is short of: blocks whose rows see
+// at most FEW_KEYS take it in a sweep of its own first.  Error of dQ against one rounding, and the whole backward pass at 8 x 2048 rows, 16 heads of 64,
+// without and with that sweep: 7 keys 1.84 and 1.42, 114 and 127 us; 33: 1.60 and 1.44, 117 and 129; 64: 1.54 and 1.43, 121 and 134; 128: 1.54 and
+// 1.43, 133 and 154; 255: 1.53 and 1.44, 161 and 190 (128-wide heads 259 and 282 .. 339 and 386).
 #define FEW_KEYS 256
 template <typename T, int HD, bool SPLIT>
 __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DQ(sizeof(T) * HD), sizeof(T) * HD, SPLIT && sizeof(T) == 2)) void window_dq_kernel(WArgs a) {
