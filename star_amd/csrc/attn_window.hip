@@ -868,12 +868,17 @@ __device__ __forceinline__ void dkv_block(unsigned ql, unsigned gl, unsigned cst
     mma_tr<C, BLK>(ql, tr, Block<T>(dp), dk);
 }
 
-// the lane's dV row, then its dK row, from the queries that see the key alone (see redo_query)
-template <class C> __device__ __forceinline__ void redo_key(const WArgs& a, const typename C::Type* base, int64_t start, int hk, int key, int k0, int len, int h2, typename C::Type* row) {
+// The lane's dV row, then its dK row, from the queries that see the key alone (see redo_query).  A sink's far queries are not swept again: where they
+// have parts (`far`, `parts` of them), those hold their sums, and what a part has masked for a sink are queries of its window, which it sees.  (Swept, one
+// NaN in one row of dO would cost every head and row of the sequence, one after the other: 650 ms at 32768 rows, 8 heads of 64 on 1, window 100, 4 sinks,
+// where the window's keys take 2.)
+template <class C> __device__ __forceinline__ void redo_key(const WArgs& a, const typename C::Type* base, int64_t start, int hk, int key, int k0, int len, int h2, const float* far, int parts,
+                                                            typename C::Type* row) {
     using T = typename C::Type;
     constexpr int HD = C::HDIM;
     const float c = a.scale * LOG2E;
-    const int rep = a.H / a.KV, last = k0 < a.sinks ? len - 1 : min(len - 1, min(k0 + 31, len - 1) + a.left);
+    const bool sink = key < a.sinks;
+    const int rep = a.H / a.KV, last = sink && !a.far_parts ? len - 1 : min(len - 1, key + a.left);
     f32x16_t kv[C::DB], vv[C::DB], acc[C::DB];
     read_half<C>(base + (int64_t)key * a.ld + (a.H + hk) * HD, h2, kv);
     read_half<C>(base + (int64_t)key * a.ld + (a.H + a.KV + hk) * HD, h2, vv);
@@ -892,6 +897,12 @@ template <class C> __device__ __forceinline__ void redo_key(const WArgs& a, cons
     for (int grad = 0; grad < 2; ++grad) {          // 0: dV, 1: dK
 #pragma unroll
         for (int db = 0; db < C::DB; ++db) acc[db] = splat16(0.f);
+        if (sink && a.far_parts)
+            for (int p = 0; p < parts; ++p)
+#pragma unroll
+                for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[db][e] += far[(int64_t)p * (2 * C::DB * 1024) + (((grad ? 0 : C::DB) + db) * 16 + e) * 64 + (threadIdx.x & 63)];
         bool open = true;
         for (int h = hk * rep; open && h < (hk + 1) * rep; ++h)
             for (int i = max(0, k0 - a.right); open && i <= last; ++i) {
@@ -960,15 +971,16 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DKV(sizeof(T) * 
 #pragma unroll
     for (int db = 0; db < C::DB; ++db) dk[db] = dv[db] = splat16(0.f);
     constexpr bool ADD = OWN && C::RB < 256;          // a split block's waves each add up a share of the far parts; else they come folded, to one wave
+    const int parts = ADD ? a.far_parts : 1;
+    const float* w = a.far_ws + ((int64_t)(b * a.KV + hk) * a.far_groups + k0 / 32) * a.far_parts * (2 * C::DB * 1024);
     if (!FAR && a.far_parts && k0 < min(a.sinks, len) && (ADD || !OWN || wave == 0)) {
-        const float* w = a.far_ws + ((int64_t)(b * a.KV + hk) * a.far_groups + k0 / 32) * a.far_parts * (2 * C::DB * 1024) + lane;
-        for (int p = ADD ? wave : 0; p < (ADD ? a.far_parts : 1); p += 4)
+        for (int p = ADD ? wave : 0; p < parts; p += 4)
 #pragma unroll
             for (int db = 0; db < C::DB; ++db)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    dk[db][e] += w[(int64_t)p * (2 * C::DB * 1024) + (db * 16 + e) * 64];
-                    dv[db][e] += w[(int64_t)p * (2 * C::DB * 1024) + ((C::DB + db) * 16 + e) * 64];
+                    dk[db][e] += w[(int64_t)p * (2 * C::DB * 1024) + (db * 16 + e) * 64 + lane];
+                    dv[db][e] += w[(int64_t)p * (2 * C::DB * 1024) + ((C::DB + db) * 16 + e) * 64 + lane];
                 }
     }
 #pragma unroll
@@ -1054,12 +1066,12 @@ __global__ __launch_bounds__(WT) WAVES_PER_SIMD(WAVES_OWN(WAVES_DKV(sizeof(T) * 
         const bool bad = any_wave_bad(any_bad<C>(dk) || any_bad<C>(dv), st, wave, lane);
         join_rows<C>(dk, a.scale, st + 512, key < len && !bad, row, wave, lane);
         join_rows<C>(dv, 1.0f, st + 512, key < len && !bad, row + a.KV * HD, wave, lane);
-        if (bad && key < len && wave == 0) redo_key<C>(a, base, start, hk, key, k0, len, h2, row);
+        if (bad && key < len && wave == 0) redo_key<C>(a, base, start, hk, key, k0, len, h2, w, parts, row);
         return;
     }
     if (key < len) {
         if (pair_sum(any_bad<C>(dk) || any_bad<C>(dv) ? 1.0f : 0.f) != 0.f) {
-            redo_key<C>(a, base, start, hk, key, k0, len, h2, row);
+            redo_key<C>(a, base, start, hk, key, k0, len, h2, w, parts, row);
         } else {
             store_rows<T, HD>(dk, a.scale, row, h2);
             store_rows<T, HD>(dv, 1.0f, row + a.KV * HD, h2);

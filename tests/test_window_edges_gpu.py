@@ -302,3 +302,51 @@ def test_append_takes_no_time_for_idle_entries():
             times.append(marks[0].elapsed_time(marks[1]))
         took.append(min(times))
     assert took[1] < 100 * took[0] and took[1] < 3.0, took
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("nb", [1, 48])
+def test_one_element_that_is_not_finite_stays_in_its_column(dtype, hd, nb):
+    """one NaN in one head's gradient of one result row, far behind the sinks: a column of dV, and dK, of the keys that the row sees, sinks included;
+    the row's dQ; nothing else"""
+    g = _gen(hd + nb)
+    n, h, kv, left, sinks, row, col = 1300, 4, 2, 40, 5, 700, 11
+    qkv, dout = _rand(g, nb * n, (h + 2 * kv) * hd, dtype=dtype), _rand(g, nb * n, h * hd, dtype=dtype)
+    wild = dout.clone()
+    wild.view(nb, n, h, hd)[:, row, 1, col] = float("nan")
+    out, lse, dqkv = _passes(qkv, wild, nb, n, h, hd, kv_heads=kv, left=left, sinks=sinks)
+    seen_keys = seen(n, left, 0, sinks)[row]
+    for b in sorted({0, nb - 1}):
+        rows = slice(b * n, (b + 1) * n)
+        want = reference(*unpack(qkv[rows], h, kv, hd), left, 0, sinks, None, heads(dout[rows], hd), dtype)
+        hit = torch.zeros(h + 2 * kv, n, hd, dtype=torch.bool)
+        hit[1, row] = True                         # dQ of query head 1
+        hit[h, seen_keys] = True                   # dK of its key head, 0
+        hit[h + kv, seen_keys, col] = True         # and dV
+        d = heads(dqkv[rows], hd)
+        assert d[hit].isnan().all()
+        assert_within(d[~hit], want["dqkv"][~hit], want["tol_dqkv"][~hit], "dqkv")
+
+
+def test_a_far_element_that_is_not_finite_costs_no_sweep_of_the_sequence():
+    """the sinks see every row: formed again one row at a time, their sums would take a second here.  The same element without sinks has the window's
+    keys alone to form again."""
+    g = _gen(9)
+    n, h, hd, left = 32768, 8, 64, 100
+    qkv, dout = _rand(g, n, (h + 2) * hd, dtype=torch.bfloat16), _rand(g, n, h * hd, dtype=torch.bfloat16)
+    dout[20000, 5] = float("nan")
+    took = []
+    for sinks in (0, 4):
+        kw = dict(kv_heads=1, left=left, sinks=sinks)
+        out, lse = ops.attn_window_fwd(qkv, 1, n, h, hd, **kw)
+        times = []
+        for _ in range(3):
+            marks = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            marks[0].record()
+            ops.attn_window_bwd(qkv, out, dout, lse, 1, n, h, hd, **kw)
+            marks[1].record()
+            torch.cuda.synchronize()
+            times.append(marks[0].elapsed_time(marks[1]))
+        took.append(min(times))
+    assert took[1] < 5 * took[0], took
