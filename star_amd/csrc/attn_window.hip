@@ -13,11 +13,11 @@
 // bf16 runs on v_mfma_f32_32x32x16_bf16, float32 on v_mfma_f32_32x32x2_f32 (full float32 products): an operand fragment is 16 bytes
 // per lane in both, so the tile layout and the address arithmetic are shared.
 //
-// Measured (kernels alone): forward 5 x 4096 rows, 12 heads of 64, window 1024: 94 us = 0.61 PFLOP/s; 8192 rows, 32 heads of 128 on 8, window 4096:
-// 412 .. 490 us = 1.0 .. 0.85 PFLOP/s (a large library product reaches 1.29).  2 x 8192 rows, 16 heads of 128, window 2048: forward 302 us, dQ 433,
-// dK/dV 622 = 0.8 PFLOP/s each.  What bounds them: the softmax's vector instructions and the matrix pipe add up (64-wide heads: 207 instructions a
-// 64 x 32 tile, 65 % and 35 % of the busy time; wave priorities around either change nothing); for 128-wide heads, backward, the LDS reads
-// of the fragments beside the products (dK/dV without its transposed products 470 us, without its score products 431, without both 300).
+// Measured (kernels alone under the profiler, mean of 12): forward 5 x 4096 rows, 12 heads of 64, window 1024: 94 us = 0.61 PFLOP/s; 8192 rows, 32 heads of
+// 128 on 8, window 4096: 405 .. 514 us = 1.0 .. 0.8 PFLOP/s (a large library product reaches 1.29).  2 x 8192 rows, 16 heads of 128, window 2048: forward
+// 275 .. 302 us, dQ 422, dK/dV 583 = 0.8 PFLOP/s and more each.  What bounds them: the softmax's vector instructions and the matrix pipe take turns (64-wide
+// heads: 207 instructions a 64 x 32 tile, 65 % and 35 % of the busy time; wave priorities around either change nothing); for 128-wide heads, backward, the
+// LDS reads of the fragments beside the products (dK/dV without its transposed products 470 us, without its score products 431, without both 300).
 // Short sequences are bound by the latency of few tiles per wave.
 // P and dS are rounded to bf16 for the second products (the matrix instruction's operand): with the rounding of the result the backward pass
 // is sqrt 2 as far off as that rounding alone.  Sums, statistics and row dots are float32.

@@ -4,7 +4,7 @@
 // sinks + (p - sinks) % (cap - sinks), so the ring behind the sinks holds the newest cap - sinks tokens (cap >= the longest sequence: an
 // ordinary cache).  lengths [NB] counts a sequence's tokens including the new ones; 0 marks an idle entry.
 //
-// Both kernels are bound by the bytes of the cache rows they touch: 16 prompts of 301 .. 6000 rows, 8 heads of 128 in bf16: 76 us = 4.8 TB/s;
+// Both kernels are bound by the bytes of the cache rows they touch: 16 prompts of 301 .. 6000 rows, 8 heads of 128 in bf16: 70 us = 5.2 TB/s;
 // a step of 64 sequences of 3000 .. 20000 tokens (8196 slots), 32 heads on 8 of 128: 359 us = 5.4 TB/s (a copy: 4.7, reads only need no turn-around).  Small calls
 // are bound by latency and by what one compute unit reads: 5 sequences, 12 heads of 64, up to 1040 tokens: 9.9 us in one launch.
 #include "common.h"

@@ -545,7 +545,8 @@ def attn_window_fwd(qkv, nb, l, h, hd, kv_heads=None, left=None, right=0, sinks=
     reads key/value head i // (h // kv_heads).  Key j is visible to query i iff j <= i + right and (j >= i - left or j < sinks); None: no
     bound (right=0: causal; left=right=None: everything).  nb sequences of l rows, or ragged: offsets int64 [nb + 1] on the device, l >= the
     longest sequence (of a longer one only the first l rows take part).  Rows outside every sequence are neither read nor written (zeros in an
-    out that is made here), and what a row does not see does not reach its result, infinities and NaN included (rows that meet such in a tile cost more time).
+    out that is made here; their lse holds nothing), and what a row does not see does not reach its result, infinities and NaN included (rows that meet such in a tile cost more time).
+    A given out shares no memory with qkv (a single row's may lie on it).
     -> (out [R, h*hd], lse float32 [h, R] or None)"""
     return _window_fwd(qkv, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale, want_lse, out)
 
@@ -576,7 +577,7 @@ def _window_bwd(home, qkv, out, dout, lse, nb, l, h, hd, kv_heads, left, right, 
 
 def attn_window_bwd(qkv, out, dout, lse, nb, l, h, hd, kv_heads=None, left=None, right=0, sinks=0, offsets=None, scale=None, dqkv=None):
     """Gradient of attn_window_fwd (the same arguments): dout [R, h*hd] -> dqkv [R, (h + 2 kv_heads) hd].  The scores are recomputed from the stored
-    row log-sum-exp; no atomics, bitwise reproducible."""
+    row log-sum-exp; no atomics, bitwise reproducible.  A given dqkv shares no memory with the operands."""
     return _window_bwd(qkv, out, dout, lse, nb, l, h, hd, kv_heads, left, right, sinks, offsets, scale, dqkv)
 
 
