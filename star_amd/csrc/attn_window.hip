@@ -387,8 +387,8 @@ template <class C> struct KvRing {
 // paid where all results are finite.  Where the row's own statistics are NaN (or, for a key, its own row), so is the result by the formula, and
 // it stays, and a sum all of whose elements have become NaN is not taken further: data that has gone NaN altogether takes about as long as other
 // data (dO all NaN: 2 x 2048 rows, causal, 16 heads on 4 of 64, backward 138 -> 197 us; 16 heads of 128, window 512: 131 -> 460).  A sum of which
-// some elements alone are not finite is formed to its end, and that takes its time (one NaN in one value row of the first of these: forward 53 -> 2570 us,
-// backward 138 -> 8000).  A lane works on its half of a row, the partner on the other (the layout of an accumulator).
+// some elements alone are not finite is formed to its end, and that takes its time, 1 to 3 us a visible row and head (one NaN in one value row of the first
+// of these: forward 53 -> 2570 us, backward 138 -> 8000).  A lane works on its half of a row, the partner on the other (the layout of an accumulator).
 template <class C> __device__ __forceinline__ bool any_bad(const f32x16_t (&acc)[C::DB]) {
     float t = 0.f;
 #pragma unroll
